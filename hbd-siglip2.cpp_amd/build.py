@@ -26,7 +26,11 @@ SOURCES = [
     "s2x_misc.hip",
     "s2x_naflex.hip",
     "s2x_static.hip",
+    "s2x_tokens.hip",
+    "s2x_paged.hip",
+    "s2x_q4.hip",
     "s2x_abi.cpp",
+    "s2x_decode.cpp",
     "s2x_encoders.cpp",
     "s2x_gguf.cpp",
     "siglip2_api.cpp",

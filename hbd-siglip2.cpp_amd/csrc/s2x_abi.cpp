@@ -34,6 +34,57 @@ bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) %
 
 WeightView view_of(const s2x_weight *w) { return w->view; }
 
+int check_epi(const s2x_epilogue *epi, int64_t N, EpiParams &p) {
+    p = EpiParams{EPI_NONE, nullptr, nullptr, 0, 0, 0};
+    if (!epi) return S2X_OK;
+    p.kind = epi->kind;
+    p.bias = epi->bias;
+    p.resid = epi->resid;
+    p.ld_resid = epi->ld_resid;
+    p.resid_rows = epi->resid_rows;
+    switch (epi->kind) {
+    case S2X_EPI_NONE: return S2X_OK;
+    case S2X_EPI_BIAS:
+    case S2X_EPI_BIAS_GELU:
+        if (!epi->bias) return fail(S2X_ERR_INVALID_ARG, "epilogue: bias is null");
+        return S2X_OK;
+    case S2X_EPI_BIAS_RESID:
+        if (!epi->bias || !epi->resid || epi->ld_resid < N || epi->resid_rows < 0)
+            return fail(S2X_ERR_INVALID_ARG, "epilogue: bias/resid/ld_resid invalid");
+        return S2X_OK;
+    case S2X_EPI_GELU_Q81:
+        if (!epi->bias || !epi->q_out || !epi->q_ds || epi->q_kpad % QK_ || epi->q_kpad < N ||
+            epi->q_kpad - N >= QK_)
+            return fail(S2X_ERR_INVALID_ARG, "epilogue GELU_Q81: bias/q_out/q_ds/q_kpad invalid");
+        if (!aligned(epi->q_out, 16) || !aligned(epi->q_ds, 4))
+            return fail(S2X_ERR_INVALID_ARG, "epilogue GELU_Q81: q_out must be 16-byte aligned");
+        p.kind = EPI_GELU_Q81;
+        p.q_out8 = (int8_t *)epi->q_out;
+        p.q_ds = (uint32_t *)epi->q_ds;
+        p.q_kpad = epi->q_kpad;
+        p.q_ldds = epi->q_kpad / QK_;
+        return S2X_OK;
+    case S2X_EPI_GELU_F16:
+        if (!epi->bias || !epi->q_out || epi->q_kpad % QK_ || epi->q_kpad < N ||
+            epi->q_kpad - N >= QK_ || !aligned(epi->q_out, 2))
+            return fail(S2X_ERR_INVALID_ARG, "epilogue GELU_F16: bias/q_out/q_kpad invalid");
+        p.kind = EPI_GELU_F16;
+        p.h_out = (_Float16 *)epi->q_out;
+        p.h_ld = p.h_kpad = epi->q_kpad;
+        return S2X_OK;
+    default: return fail(S2X_ERR_INVALID_ARG, "epilogue: unknown kind %d", epi->kind);
+    }
+}
+
+int check_q81_planes(const void *qs, const void *ds, int64_t M, const char *who) {
+    if (M < 0) return fail(S2X_ERR_INVALID_ARG, "%s: M < 0", who);
+    if (M > (1 << 30)) return fail(S2X_ERR_UNSUPPORTED, "%s: M too large", who);
+    if (M > 0 && (!qs || !ds)) return fail(S2X_ERR_INVALID_ARG, "%s: null qs/ds", who);
+    if (!aligned(qs, 16) || !aligned(ds, 4))
+        return fail(S2X_ERR_INVALID_ARG, "%s: qs must be 16-byte and ds 4-byte aligned", who);
+    return S2X_OK;
+}
+
 }  // namespace s2x
 
 using namespace s2x;
@@ -137,57 +188,10 @@ int64_t s2x_weight_n(const s2x_weight *w) { return w ? w->view.N : 0; }
 // ---------------------------------------------------------------------------
 // a3
 // ---------------------------------------------------------------------------
-static int check_epi(const s2x_epilogue *epi, int64_t N, EpiParams &p) {
-    p = EpiParams{EPI_NONE, nullptr, nullptr, 0, 0, 0};
-    if (!epi) return S2X_OK;
-    p.kind = epi->kind;
-    p.bias = epi->bias;
-    p.resid = epi->resid;
-    p.ld_resid = epi->ld_resid;
-    p.resid_rows = epi->resid_rows;
-    switch (epi->kind) {
-    case S2X_EPI_NONE: return S2X_OK;
-    case S2X_EPI_BIAS:
-    case S2X_EPI_BIAS_GELU:
-        if (!epi->bias) return fail(S2X_ERR_INVALID_ARG, "epilogue: bias is null");
-        return S2X_OK;
-    case S2X_EPI_BIAS_RESID:
-        if (!epi->bias || !epi->resid || epi->ld_resid < N || epi->resid_rows < 0)
-            return fail(S2X_ERR_INVALID_ARG, "epilogue: bias/resid/ld_resid invalid");
-        return S2X_OK;
-    case S2X_EPI_GELU_Q81:
-        if (!epi->bias || !epi->q_out || !epi->q_ds || epi->q_kpad % QK_ || epi->q_kpad < N ||
-            epi->q_kpad - N >= QK_)
-            return fail(S2X_ERR_INVALID_ARG, "epilogue GELU_Q81: bias/q_out/q_ds/q_kpad invalid");
-        if (!aligned(epi->q_out, 16) || !aligned(epi->q_ds, 4))
-            return fail(S2X_ERR_INVALID_ARG, "epilogue GELU_Q81: q_out must be 16-byte aligned");
-        p.kind = EPI_GELU_Q81;
-        p.q_out8 = (int8_t *)epi->q_out;
-        p.q_ds = (uint32_t *)epi->q_ds;
-        p.q_kpad = epi->q_kpad;
-        p.q_ldds = epi->q_kpad / QK_;
-        return S2X_OK;
-    case S2X_EPI_GELU_F16:
-        if (!epi->bias || !epi->q_out || epi->q_kpad % QK_ || epi->q_kpad < N ||
-            epi->q_kpad - N >= QK_ || !aligned(epi->q_out, 2))
-            return fail(S2X_ERR_INVALID_ARG, "epilogue GELU_F16: bias/q_out/q_kpad invalid");
-        p.kind = EPI_GELU_F16;
-        p.h_out = (_Float16 *)epi->q_out;
-        p.h_ld = p.h_kpad = epi->q_kpad;
-        return S2X_OK;
-    default: return fail(S2X_ERR_INVALID_ARG, "epilogue: unknown kind %d", epi->kind);
-    }
-}
-
 static int check_q81_input(const s2x_weight *w, const void *qs, const void *ds, int64_t M,
                            const char *who) {
     if (!w) return fail(S2X_ERR_INVALID_ARG, "%s: weight is null", who);
-    if (M < 0) return fail(S2X_ERR_INVALID_ARG, "%s: M < 0", who);
-    if (M > (1 << 30)) return fail(S2X_ERR_UNSUPPORTED, "%s: M too large", who);
-    if (M > 0 && (!qs || !ds)) return fail(S2X_ERR_INVALID_ARG, "%s: null qs/ds", who);
-    if (!aligned(qs, 16) || !aligned(ds, 4))
-        return fail(S2X_ERR_INVALID_ARG, "%s: qs must be 16-byte and ds 4-byte aligned", who);
-    return S2X_OK;
+    return check_q81_planes(qs, ds, M, who);
 }
 
 int s2x_mul_mat_q8_0_q8_1(const s2x_weight *w, const void *qs, const void *ds, int64_t M,

@@ -22,6 +22,10 @@ namespace s2x {
 int fail(int status, const char *fmt, ...);
 int hip_fail(hipError_t e, const char *what);
 bool aligned(const void *p, size_t a);
+// argument checks shared by the products: the epilogue struct (translated
+// into the kernels' parameters) and the Q8_1 activation planes
+int check_epi(const s2x_epilogue *epi, int64_t N, EpiParams &p);
+int check_q81_planes(const void *qs, const void *ds, int64_t M, const char *who);
 
 inline int64_t round_up_i(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 

@@ -14,7 +14,7 @@ import os
 __all__ = [
     "S2XError", "lib", "Epilogue", "LayerWeights", "VisionWeights", "TextWeights",
     "EPI_NONE", "EPI_BIAS", "EPI_BIAS_GELU", "EPI_BIAS_RESID", "EPI_GELU_Q81", "POOL_MEAN",
-    "POOL_PROBE",
+    "POOL_PROBE", "KVCache", "TYPE_F32", "TYPE_F16", "TYPE_BF16", "ROPE_HALVES", "ROPE_PAIRS",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -22,6 +22,8 @@ LIB_PATH = os.path.join(os.path.dirname(_HERE), "libs2x.so")
 
 EPI_NONE, EPI_BIAS, EPI_BIAS_GELU, EPI_BIAS_RESID, EPI_GELU_Q81, EPI_GELU_F16 = 0, 1, 2, 3, 4, 5
 POOL_MEAN, POOL_PROBE = 0, 1
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 2
+ROPE_HALVES, ROPE_PAIRS = 0, 1
 
 if not os.path.exists(LIB_PATH):
     raise ImportError(
@@ -99,6 +101,12 @@ class TextWeights(ctypes.Structure):
     ]
 
 
+class KVCache(ctypes.Structure):
+    _fields_ = [("k", _p), ("v", _p), ("type", _i32), ("page_size", _i32), ("n_pages", _i64),
+                ("n_head", _i64), ("d_head", _i64), ("ld_page", _i64), ("ld_head", _i64),
+                ("ld_tok", _i64)]
+
+
 def _sig(name, argtypes, restype=ctypes.c_int):
     f = getattr(lib, name)
     f.argtypes = argtypes
@@ -146,6 +154,20 @@ _sig("s2x_attn_fp64", [_p, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _f32, _
 _sig("s2x_attn_1q", [_p, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _f32, _p, _p])
 _sig("s2x_resize_pos_embed", [_p, _i64, _i64, _i64, _i64, _p, _p])
 _sig("s2x_get_rows_q8_0", [_p, _i64, _i64, _p, _i64, _p, _i64, _p, _p])
+_sig("s2x_weight_q4_0_bytes", [_i64, _i64], _sz)
+_sig("s2x_weight_q4_0_create", [_p, ctypes.c_int, _i64, _i64, _p, ctypes.POINTER(_p)])
+_sig("s2x_weight_q4_0_create_in", [_p, _i64, _i64, _p, _p, ctypes.POINTER(_p)])
+_sig("s2x_weight_q4_0_destroy", [_p], None)
+_sig("s2x_weight_q4_0_k", [_p], _i64)
+_sig("s2x_weight_q4_0_n", [_p], _i64)
+_sig("s2x_mul_mat_q4_0_workspace_size", [_i64, _i64, _i64], _sz)
+_sig("s2x_mul_mat_q4_0_q8_1", [_p, _p, _p, _i64, _p, _i64, ctypes.POINTER(Epilogue), _p, _sz, _p])
+_sig("s2x_kv_slots", [_p, _p, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _p])
+_sig("s2x_qk_norm_rope_kv", [_p, _i32, _i64, _i64, _i64, _p, _p, _f32, _p, _i64, _i32, _p, _p, _p,
+                             _i64, ctypes.POINTER(KVCache), _p])
+_sig("s2x_attn_paged_workspace_size", [_i64, _i64, _i64, _i64, _i64], _sz)
+_sig("s2x_attn_paged", [_p, _i64, ctypes.POINTER(KVCache), _p, _i64, _p, _i64, _i64, _i64, _f32,
+                        _i64, _p, _i32, _i64, _p, _p, _sz, _p])
 _sig("s2x_vision_create", [ctypes.POINTER(VisionWeights), ctypes.POINTER(_p)])
 _sig("s2x_vision_destroy", [_p], None)
 _sig("s2x_vision_set_stream", [_p, _p])

@@ -347,6 +347,135 @@ int s2x_get_rows_q8_0(const void *table_raw, int64_t K, int64_t n_rows_table,
                       int64_t add_rows, float *out, void *stream);
 
 /* ------------------------------------------------------------------------ */
+/* Decode step: one new token per sequence, for a generating model behind the */
+/* encoders.  No counterpart in the reference.  The step's calls, in order:    */
+/* s2x_kv_slots (where the new tokens' keys and values go), a projection       */
+/* (s2x_mul_mat_q4_0_q8_1 or any other product), s2x_qk_norm_rope_kv (norms,   */
+/* position rotation, write into the cache), s2x_attn_paged.                   */
+/* All run on the current device, allocate nothing and may be captured into a  */
+/* graph.  Values that only the device knows (lengths, page ids, slots,        */
+/* positions) are checked there: none makes a kernel read or write outside the */
+/* memory its arguments describe.  Outputs overlap no input and no other       */
+/* output.                                                                     */
+/* ------------------------------------------------------------------------ */
+typedef enum { S2X_TYPE_F32 = 0, S2X_TYPE_F16 = 1, S2X_TYPE_BF16 = 2 } s2x_type;
+
+/* Q4_0 weights: a raw matrix W (K, N) is N rows of K/32 18-byte block_q4_0
+ * (fp16 d, then 16 bytes of nibbles: value i of the block in the low half of
+ * byte i, value 16 + i in its high half; a nibble v stands for (v - 8) * d).
+ * The repack is lossless; it reorders the nibbles for the int8 MFMA.
+ * K % 32 == 0.  create: new device memory of s2x_weight_q4_0_bytes(), raw in
+ * host or device memory, synchronises `stream`.  create_in: into `dev_buf`
+ * (256-byte aligned), raw on the device, asynchronous, no allocation on the
+ * device. */
+typedef struct s2x_weight_q4 s2x_weight_q4;
+size_t s2x_weight_q4_0_bytes(int64_t K, int64_t N);
+int s2x_weight_q4_0_create(const void *raw, int raw_is_host, int64_t K, int64_t N, void *stream,
+                           s2x_weight_q4 **out);
+int s2x_weight_q4_0_create_in(const void *raw_dev, int64_t K, int64_t N, void *dev_buf,
+                              void *stream, s2x_weight_q4 **out);
+void s2x_weight_q4_0_destroy(s2x_weight_q4 *w);
+int64_t s2x_weight_q4_0_k(const s2x_weight_q4 *w);
+int64_t s2x_weight_q4_0_n(const s2x_weight_q4 *w);
+
+/* Y = epilogue(acc): acc = sum over 32-blocks of (float)I_kb * d_w * d_x with
+ * the exact I_kb = sum q_w*q_x, q_w = nibble - 8, over the Q8_1 activation of
+ * s2x_mul_mat_q8_0_q8_1 (same planes and alignments); epilogues NONE, BIAS,
+ * BIAS_GELU and BIAS_RESID.  Up to S2X_Q4_FEW_ROWS rows the weight is read as
+ * it lies, 18 bytes per 32 values, and the blocks are summed in f32 in ranges
+ * of K that depend on K alone: a row's bits depend on neither M nor the other
+ * rows within that limit.  More rows expand the weight into `workspace` as
+ * Q8_0 (exact: same blocks, same scales) and run s2x_mul_mat_q8_0_q8_1's
+ * kernel, with its bits.  workspace: s2x_mul_mat_q4_0_workspace_size() bytes,
+ * 256-byte aligned; 0 bytes, and NULL is taken, up to S2X_Q4_FEW_ROWS. */
+#define S2X_Q4_FEW_ROWS 64
+size_t s2x_mul_mat_q4_0_workspace_size(int64_t K, int64_t N, int64_t M);
+int s2x_mul_mat_q4_0_q8_1(const s2x_weight_q4 *w, const void *qs, const void *ds, int64_t M,
+                          float *y, int64_t ldy, const s2x_epilogue *epi, void *workspace,
+                          size_t ws_bytes, void *stream);
+
+/* A paged key/value cache.  Token t of a sequence lies in page
+ * block_table[t / page_size] at place t % page_size; "slot" s is place
+ * s % page_size of page s / page_size.  Head h of that token's key is the
+ * d_head values at k + page*ld_page + h*ld_head + place*ld_tok (elements; v
+ * alike), so a page may hold its tokens by head (ld_head = page_size*d_head,
+ * ld_tok = d_head) or by token (ld_tok = n_head*d_head, ld_head = d_head).
+ * page_size: a power of two up to 65,536; d_head: a multiple of 8 up to 256;
+ * k and v 16-byte aligned, strides multiples of 8 that keep all rows apart. */
+typedef struct {
+    void   *k, *v;
+    int32_t type;       /* S2X_TYPE_F16 or S2X_TYPE_BF16 */
+    int32_t page_size;
+    int64_t n_pages, n_head, d_head;
+    int64_t ld_page, ld_head, ld_tok;
+} s2x_kv_cache;
+
+/* Block tables and slot maps from the lengths of a batch, on the device.
+ * Sequence b holds kv_len[b] tokens in the first ceil(kv_len[b] / page_size)
+ * entries of its row of block_table (n_seq rows, ld_table apart) and gets
+ * n_new[b] more (negative lengths count as 0).  The pages it needs beyond
+ * those it has are taken from the front of free_pages, sequence after
+ * sequence, and written into its row; no other entry is touched.
+ *   len_out[b]    kv_len[b] + n_new[b]
+ *   tok_start[b]  first row of sequence b's new tokens, n_seq + 1 entries
+ *   pos[t], slots[t]  of row t < max_tok: the token's position and its slot;
+ *                 rows behind the last token get 0 and -1
+ *   used[0]       pages that the batch needs, used[1] new tokens in all
+ * A page that free_pages does not have (used[0] > n_free) is entered as -1, so
+ * is an id of free_pages outside 0 .. n_pages - 1; a token whose page is
+ * missing, outside 0 .. n_pages - 1 or behind the row's end gets slot -1.
+ * Tokens past max_tok get no row (tok_start stops there).  n_seq <= 8,192. */
+int s2x_kv_slots(const int32_t *kv_len, const int32_t *n_new, int64_t n_seq,
+                 const int32_t *free_pages, int64_t n_free, int64_t page_size, int64_t n_pages,
+                 int32_t *block_table, int64_t ld_table, int64_t max_tok, int32_t *len_out,
+                 int32_t *tok_start, int32_t *pos, int64_t *slots, int64_t *used, void *stream);
+
+/* The projections' rows to attention operands, in one pass: x holds n_tok
+ * rows of [q heads | k heads | v heads] (n_q_head + 2*cache->n_head heads of
+ * cache->d_head values, ld_x apart, x_type any s2x_type).  Every query and key
+ * head is normalised, h * (1/sqrt(mean(h^2) + eps)) * w with q_norm / k_norm
+ * (d_head floats; NULL: that kind of head is left as it is), and its first
+ * d_rot values are turned by the row's position: pair j by the angle
+ * pos[row] * freq[j] radians (freq: d_rot/2 doubles on the device; the angle
+ * and its reduction are in f64).  Pair j is values (j, j + d_rot/2) with
+ * S2X_ROPE_HALVES, (2j, 2j + 1) with S2X_ROPE_PAIRS.  All in f32, rounded once
+ * to cache->type: queries to q (n_tok rows, ld_q apart), keys and values to
+ * slot slots[row] of the cache.  A slot outside the cache (-1) leaves the
+ * cache alone; its row of q is written all the same.  Two rows with one slot
+ * leave either's values there.  x and q 16-byte aligned, ld_x and ld_q
+ * multiples of 8; d_rot even, 0 <= d_rot <= d_head. */
+typedef enum { S2X_ROPE_HALVES = 0, S2X_ROPE_PAIRS = 1 } s2x_rope_style;
+int s2x_qk_norm_rope_kv(const void *x, int32_t x_type, int64_t ld_x, int64_t n_tok,
+                        int64_t n_q_head, const float *q_norm, const float *k_norm, float eps,
+                        const double *freq, int64_t d_rot, int32_t rope_style, const int32_t *pos,
+                        const int64_t *slots, void *q, int64_t ld_q, const s2x_kv_cache *cache,
+                        void *stream);
+
+/* Attention of one new token per sequence over its cached tokens: for
+ * sequence s and query head h (key head h / (n_q_head / cache->n_head)),
+ *   out[s, h] = sum_t softmax_t(q[s,h] . k_t * scale) v_t,  t < kv_len[s]
+ * (with window > 0 the last `window` of them), q in cache->type (n_seq rows of
+ * n_q_head*d_head, ld_q apart), out in out_type (F32 or cache->type, rows
+ * ld_out apart), lse (optional, n_seq x n_q_head floats) = log sum_t
+ * exp(q . k_t * scale).  kv_len counts the new token where
+ * s2x_qk_norm_rope_kv has written it.  Scores, softmax and sums are in f32;
+ * the probabilities enter the second product as a sum of two terms of the
+ * cache's type (three where out is f32 and the cache bf16), so that their
+ * rounding stays below the output's.  Lengths above max_len or beyond the
+ * table's row count as that; pages outside 0 .. n_pages - 1 are not seen; a
+ * sequence that sees nothing gets zeros and lse = -inf.  Keys and values of
+ * unseen places are never read.  q and out 16-byte aligned, ld_q and ld_out
+ * multiples of 8.  n_seq <= 65,535; workspace (256-byte aligned, own to the call until it has finished) of
+ * s2x_attn_paged_workspace_size() bytes; NULL where that is 0. */
+size_t s2x_attn_paged_workspace_size(int64_t n_seq, int64_t max_len, int64_t n_q_head,
+                                     int64_t n_kv_head, int64_t d_head);
+int s2x_attn_paged(const void *q, int64_t ld_q, const s2x_kv_cache *cache,
+                   const int32_t *block_table, int64_t ld_table, const int32_t *kv_len,
+                   int64_t n_seq, int64_t max_len, int64_t n_q_head, float scale, int64_t window,
+                   void *out, int32_t out_type, int64_t ld_out, float *lse, void *workspace,
+                   size_t ws_bytes, void *stream);
+
+/* ------------------------------------------------------------------------ */
 /* a10  encoders (replace siglip2::VisionEncoder / TextEncoder,               */
 /* src/siglip2_vision.h:37-68, src/siglip2_text.h:25-75).                     */
 /* Weights come from host memory: raw Q8_0 blocks for every matrix, f32 for  */
