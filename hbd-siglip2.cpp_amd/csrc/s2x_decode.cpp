@@ -57,10 +57,10 @@ static int check_cache(const s2x_kv_cache *c, KvView &v, const char *who) {
                     (long long)c->n_pages, (long long)c->n_head, (long long)c->d_head);
     if (c->d_head % 8 || c->d_head > 256 || c->n_head > 1024)
         return fail(S2X_ERR_UNSUPPORTED, "%s: d_head %% 8 == 0, d_head <= 256, at most 1,024 heads", who);
-    const int64_t most = (int64_t)1 << 40, ps = c->page_size;
+    const int64_t most = INT32_MAX, ps = c->page_size;  // (32-bit strides, 64-bit offsets)
     if (c->ld_page < 8 || c->ld_head < 8 || c->ld_tok < 8 || c->ld_page % 8 || c->ld_head % 8 ||
         c->ld_tok % 8 || c->ld_page > most || c->ld_head > most || c->ld_tok > most)
-        return fail(S2X_ERR_INVALID_ARG, "%s: cache strides must be positive multiples of 8", who);
+        return fail(S2X_ERR_INVALID_ARG, "%s: cache strides must be positive multiples of 8 below 2^31", who);
     const int64_t heads = (c->n_head - 1) * c->ld_head, toks = (ps - 1) * c->ld_tok;
     const bool by_tok = (c->n_head == 1 || c->ld_head >= c->d_head) &&
                         (ps == 1 || c->ld_tok >= heads + c->d_head);
@@ -68,8 +68,6 @@ static int check_cache(const s2x_kv_cache *c, KvView &v, const char *who) {
                          (c->n_head == 1 || c->ld_head >= toks + c->d_head);
     if ((!by_tok && !by_head) || (c->n_pages > 1 && c->ld_page < heads + toks + c->d_head))
         return fail(S2X_ERR_INVALID_ARG, "%s: cache rows overlap", who);
-    if (c->ld_page > INT64_MAX / 4 / c->n_pages)
-        return fail(S2X_ERR_UNSUPPORTED, "%s: cache too large", who);
     if (!c->k || !c->v || !aligned(c->k, 16) || !aligned(c->v, 16))
         return fail(S2X_ERR_INVALID_ARG, "%s: k / v null or not 16-byte aligned", who);
     v = KvView{c->k, c->v, c->type, shift, c->n_pages, c->ld_page, c->ld_head, c->ld_tok,

@@ -401,7 +401,8 @@ int s2x_mul_mat_q4_0_q8_1(const s2x_weight_q4 *w, const void *qs, const void *ds
  * alike), so a page may hold its tokens by head (ld_head = page_size*d_head,
  * ld_tok = d_head) or by token (ld_tok = n_head*d_head, ld_head = d_head).
  * page_size: a power of two up to 65,536; d_head: a multiple of 8 up to 256;
- * k and v 16-byte aligned, strides multiples of 8 that keep all rows apart. */
+ * k and v 16-byte aligned, strides multiples of 8 below 2^31 that keep all
+ * rows apart. */
 typedef struct {
     void   *k, *v;
     int32_t type;       /* S2X_TYPE_F16 or S2X_TYPE_BF16 */

@@ -25,8 +25,8 @@ BAD_CACHES = [
     (dict(n_head=2000), UNSUPPORTED), (dict(d_head=0), INVALID), (dict(d_head=100), UNSUPPORTED),
     (dict(d_head=264), UNSUPPORTED), (dict(ld_tok=0), INVALID), (dict(ld_tok=120), INVALID),
     (dict(ld_tok=132), INVALID), (dict(ld_head=16 * 128 - 8), INVALID), (dict(ld_page=2 * 16 * 128 - 8), INVALID),
-    (dict(ld_head=-8), INVALID), (dict(ld_page=1 << 41), INVALID), (dict(k=None), INVALID), (dict(v=None), INVALID),
-    (dict(k=(1 << 20) + 8), INVALID), (dict(n_pages=2 ** 31 - 1, ld_page=1 << 40), UNSUPPORTED),
+    (dict(ld_head=-8), INVALID), (dict(ld_page=1 << 31), INVALID), (dict(k=None), INVALID), (dict(v=None), INVALID),
+    (dict(k=(1 << 20) + 8), INVALID),
     (dict(ld_head=128, ld_tok=128), INVALID),  # a token's heads over the next tokens
 ]
 
