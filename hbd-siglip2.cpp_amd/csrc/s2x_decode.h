@@ -81,10 +81,10 @@ hipError_t launch_attn_paged(const AttnPaged &p, hipStream_t stream);
 
 // A Q4_0 weight (K, N) repacked for the int8 MFMA.  A tile is 16 columns n by
 // 128 values of K (4 blocks), 1,024 bytes: lane l = 16 g + n % 16 has the 16
-// bytes at 16 l, word j of them values 8 g .. 8 g + 7 of the tile's block j,
-// value i < 4 in the low half of byte i, 4 + i in its high half, nibbles in
-// two's complement (v - 8).  Tiles of one column group follow each other along
-// K.  Scales: per tile 64 halves, [g][j][i] of column 4 g + i and block j.
+// bytes at 16 l, word j of them 8 values of the tile's block j, from 16 (g & 1)
+// + 8 (g >> 1) on, the first 4 in the low halves of its bytes, the others in
+// the high ones, nibbles in two's complement (v - 8).  Tiles of one column group follow each other along
+// K.  Scales: per tile 64 halves, [j][c] of block j and column c.
 // Columns past N and blocks past K / 32 are zeros.
 struct Q4View {
     const uint8_t  *qs;

@@ -18,18 +18,19 @@ __global__ __launch_bounds__(256) void k_repack_q4_0(const uint8_t *__restrict__
     for (int j = 0; j < 4; ++j) {
         const int64_t kb = tk * 4 + j;
         if (n >= N || kb >= KB) continue;
-        const uint8_t *b = raw + (n * KB + kb) * 18 + 2 + (g & 1) * 8;  // bytes of values 8 (g & 1) ..
+        // values 16 (g & 1) + 8 (g >> 1) ..: a half of 8 bytes
+        const uint8_t *b = raw + (n * KB + kb) * 18 + 2 + 8 * (g >> 1);
         for (int k = 0; k < 4; ++k) {
-            const uint32_t lo = g < 2 ? b[k] & 15 : b[k] >> 4, hi = g < 2 ? b[4 + k] & 15 : b[4 + k] >> 4;
+            const uint32_t lo = g & 1 ? b[k] >> 4 : b[k] & 15, hi = g & 1 ? b[4 + k] >> 4 : b[4 + k] & 15;
             w[j] |= ((lo | hi << 4) ^ 0x88) << (8 * k);
         }
     }
     reinterpret_cast<uint4 *>(qs)[i] = make_uint4(w[0], w[1], w[2], w[3]);
-    // scale l of the tile: column 4 (l / 16) + l % 4, block l % 16 / 4
-    const int64_t ns = tn * 16 + 4 * g + l % 4, kb = tk * 4 + l % 16 / 4;
+    // scale l of the tile: column l % 16, block g
+    const int64_t kb = tk * 4 + g;
     uint16_t v = 0;
-    if (ns < N && kb < KB) {
-        const uint8_t *b = raw + (ns * KB + kb) * 18;
+    if (n < N && kb < KB) {
+        const uint8_t *b = raw + (n * KB + kb) * 18;
         v = (uint16_t)(b[0] | b[1] << 8);
     }
     d[i] = v;
@@ -42,72 +43,195 @@ hipError_t launch_repack_q4_0(const void *raw, const Q4View &w, hipStream_t stre
     return hipGetLastError();
 }
 
+// The weight as the Q8_0 planes of the int8 GEMM, for more rows: exact, a block
+// keeps its scale.  A wave a tile: 16 bytes in, 8 values of each of 4 blocks;
+// the halves of blocks that lie 32 lanes apart change places
+// (v_permlane32_swap), so that a lane stores 16 bytes of one block and a row
+// gets 64 bytes a store.  Columns past N (to the plane's whole 128) get zero
+// scales alone.
 __global__ __launch_bounds__(256) void k_expand_q4(const uint8_t *__restrict__ qs, const uint16_t *__restrict__ d,
-                                                   int64_t n_block, int64_t KB, int64_t N, int64_t tiles_k,
+                                                   int64_t n_tile, int KB, int64_t N, int tiles_k,
                                                    int8_t *__restrict__ out, int64_t ld_qs,
                                                    uint16_t *__restrict__ dT, int64_t ldT) {
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= n_block) return;
-    const int64_t n = i / KB, kb = i - n * KB;
-    const int64_t tile = n / 16 * tiles_k + kb / 4;
-    const int c = (int)(n % 16), j = (int)(kb % 4);
-    uint32_t o[8];
+    const int64_t tile = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / WAVE;
+    if (tile >= n_tile) return;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const int64_t n = tile / tiles_k * 16 + c;
+    const int tk = (int)(tile % tiles_k);
+    if (4 * tk + g < KB)  // (the position of column n's scale in a dT row: WeightView)
+        dT[(4 * tk + g) * ldT + ((n & ~(int64_t)63) | ((n & 31) << 1) | ((n >> 5) & 1))] =
+            n < N ? d[tile * 64 + lane] : (uint16_t)0;
+    if (n - c >= N) return;  // (uniform)
+    const v4u w = *reinterpret_cast<const v4u *>(qs + tile * 1024 + lane * 16);
+    uint32_t o[4][2];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(qs + tile * 1024 + (16 * g + c) * 16 + 4 * j);
+    for (int j = 0; j < 4; ++j) {
         // a nibble v of two's complement: (v ^ 8) - 8 in each byte, borrows kept apart
-        const uint32_t lo = (w & 0x0f0f0f0fu) ^ 0x08080808u, hi = ((w >> 4) & 0x0f0f0f0fu) ^ 0x08080808u;
-        o[2 * g] = ((lo | 0x80808080u) - 0x08080808u) ^ 0x80808080u;
-        o[2 * g + 1] = ((hi | 0x80808080u) - 0x08080808u) ^ 0x80808080u;
+        const uint32_t lo = (w[j] & 0x0f0f0f0fu) ^ 0x08080808u, hi = ((w[j] >> 4) & 0x0f0f0f0fu) ^ 0x08080808u;
+        o[j][0] = ((lo | 0x80808080u) - 0x08080808u) ^ 0x80808080u;
+        o[j][1] = ((hi | 0x80808080u) - 0x08080808u) ^ 0x80808080u;
     }
-    uint4 *dst = reinterpret_cast<uint4 *>(out + n * ld_qs + kb * QK);
-    dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
-    // (the position of column n's scale in a dT row: WeightView)
-    dT[kb * ldT + ((n & ~(int64_t)63) | ((n & 31) << 1) | ((n >> 5) & 1))] = d[tile * 64 + c / 4 * 16 + j * 4 + c % 4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        // lanes 0 - 31: 16 (g & 1) .. + 7 of block 2 h, and its next 8 from the lane 32 on; 32 - 63: of 2 h + 1
+        const auto p0 = __builtin_amdgcn_permlane32_swap(o[2 * h][0], o[2 * h + 1][0], false, false);
+        const auto p1 = __builtin_amdgcn_permlane32_swap(o[2 * h][1], o[2 * h + 1][1], false, false);
+        const int kb = 4 * tk + 2 * h + (g >> 1);
+        if (n < N && kb < KB)
+            *reinterpret_cast<uint4 *>(out + n * ld_qs + (int64_t)kb * QK + 16 * (g & 1)) =
+                make_uint4(p0[0], p1[0], p0[1], p1[1]);
+    }
 }
 hipError_t launch_expand_q4(const Q4View &w, const WeightView &dst, hipStream_t stream) {
-    const int64_t nb = w.N * (w.K / QK);
-    uint16_t *dT = const_cast<uint16_t *>(dst.dT);
-    hipError_t e = launch_fill_zero(dT, (size_t)(w.K / QK * dst.ldT) * 2, stream);
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k_expand_q4, dim3((unsigned)((nb + 255) / 256)), dim3(256), 0, stream, w.qs, w.d, nb,
-                       w.K / QK, w.N, w.tiles_k(), const_cast<int8_t *>(dst.qs), dst.ld_qs, dT, dst.ldT);
+    const int64_t n = dst.ldT / 16 * w.tiles_k();
+    hipLaunchKernelGGL(k_expand_q4, dim3((unsigned)((n + 3) / 4)), dim3(256), 0, stream, w.qs, w.d, n,
+                       (int)(w.K / QK), w.N, (int)w.tiles_k(), const_cast<int8_t *>(dst.qs), dst.ld_qs,
+                       const_cast<uint16_t *>(dst.dT), dst.ldT);
     return hipGetLastError();
 }
 
-// One thread per output, blocks in order.
-__global__ __launch_bounds__(256) void k_mul_mat_q4(Q4View w, int64_t tiles_k, const int8_t *__restrict__ xq,
-                                                    const uint32_t *__restrict__ xds, int64_t M, float *y,
-                                                    int64_t ldy, EpiParams epi) {
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= M * w.N) return;
-    const int64_t m = i / w.N, n = i - m * w.N, KB = w.K / QK;
-    const int c = (int)(n % 16);
-    float acc = 0.0f;
-    for (int64_t kb = 0; kb < KB; ++kb) {
-        const int64_t tile = n / 16 * tiles_k + kb / 4;
-        const int j = (int)(kb % 4);
-        int dot = 0;
-        for (int g = 0; g < 4; ++g) {
-            const uint8_t *b = w.qs + tile * 1024 + (16 * g + c) * 16 + 4 * j;
-            const int8_t *x = xq + m * w.K + kb * QK + 8 * g;
-            for (int k = 0; k < 4; ++k)
-                dot += ((int)((b[k] & 15) ^ 8) - 8) * x[k] + ((int)((b[k] >> 4) ^ 8) - 8) * x[4 + k];
-        }
-        const float dw = f16_bits_to_f32(w.d[tile * 64 + c / 4 * 16 + j * 4 + c % 4]);
-        acc = fmaf((float)dot, dw * f16_bits_to_f32((uint16_t)(xds[m * KB + kb] & 0xffff)), acc);
+// ---------------------------------------------------------------------------
+// Products of few rows: the weight is read as it lies.
+//
+// v_mfma_i32_16x16x32_i8 takes a block of 32 values at 16 columns (A) and 16
+// rows (B) and leaves lane l columns 4 g + i (g = l / 16) of row l % 16.
+//  * A: a nibble in the high half of a byte is 16 (v - 8) as int8, so two
+//    operations make 8 operand bytes of a word: w << 4 and w, both
+//    & 0xf0f0f0f0; the sums carry the 16 to the end.
+//  * B: a lane loads 16 bytes, half a block: lanes 0 - 31 of the tile's even
+//    block, 32 - 63 of its odd one; v_permlane32_swap gives every lane 8 bytes
+//    of both, those from 16 (g & 1) + 8 (g >> 1) on.
+//  * the blocks' scales d_w d_x by v_mfma_f32_16x16x16_f16: lane group g holds
+//    block g's d_w and d_x in the first of its four slots of k, and A is zeroed
+//    but for the block wanted: one exact product per output.
+// So acc = fmaf((float)I, d_w d_x, acc) is 8 VALU operations on 4 outputs, and a
+// tile's 1,152 bytes of weight come with 5 load instructions.  With the scales
+// multiplied on the VALU and loaded as each lane needs them it was 11, and those
+// loads' lanes (64 bytes a clock and CU) bound it: 1 x 1152 x 256000 53 us
+// against 34.6 (4.8 TB/s, a copy's rate), 7 x 4096 x 14336 16 against 9.4.  One
+// group of 16 rows is bound by the weight's bytes, several by their VALU and
+// matrix operations (some 7 us a group at 4096 x 14336).  Loads of the next
+// tiles ahead of a tile's products changed nothing: the waves of the other
+// workgroups on a CU cover each other's.
+//
+// A wave takes 16 rows and NT groups of 16 columns over a range of K, wk waves
+// of a workgroup share their columns' K and join in LDS in order.  Further rows
+// are further workgroups, next to each other on one XCD, so that the weight
+// comes out of its L2 again (more rows a wave: slower at every size up to 64).
+// ---------------------------------------------------------------------------
+constexpr int Q4_NW = 8, Q4_NT = Q4_NW * WAVE;
+
+struct Q4Grid {
+    int wk, lwk;  // waves along K (a power of two) and its logarithm
+    int tiles_k, KB, M, N, row_groups;
+};
+
+template <int NT>
+__global__ __launch_bounds__(Q4_NT) void k_mul_mat_q4(const uint8_t *__restrict__ wq, const uint16_t *__restrict__ wd,
+                                                      Q4Grid G, const int8_t *__restrict__ xq,
+                                                      const uint32_t *__restrict__ xds, float *y, int64_t ldy,
+                                                      EpiParams epi) {
+    constexpr int COLS = NT * 16, P = COLS + 4;
+    __shared__ __align__(16) float part[Q4_NW][16][P];  // [wave][row][column]
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wk = wave & (G.wk - 1), wn = wave >> G.lwk;  // this wave's part of K, column group
+    const int groups = Q4_NW >> G.lwk;                     // column groups of the workgroup
+    const int id = xcd_linear(blockIdx.x, gridDim.x), col = id / G.row_groups;
+    const int m0 = (id - col * G.row_groups) * 16, tn0 = (col * groups + wn) * NT;
+    const int tiles_n = (G.N + 15) / 16, per = (G.tiles_k + G.wk - 1) >> G.lwk;
+    const int k0 = wk * per, k1 = min(k0 + per, G.tiles_k);
+
+    const int64_t m = min(m0 + r, G.M - 1);  // (rows past M: computed, not stored)
+    const int8_t *xr = xq + m * G.KB * QK + 16 * (g & 1);
+    const uint32_t *dr = xds + m * G.KB;
+    const uint8_t *wp[NT];
+    const uint16_t *dp[NT];
+#pragma unroll
+    for (int b = 0; b < NT; ++b) {
+        const int64_t t = (int64_t)min(tn0 + b, tiles_n - 1) * G.tiles_k;
+        wp[b] = wq + t * 1024 + lane * 16;
+        dp[b] = wd + t * 64 + lane;
     }
-    if (epi.kind != EPI_NONE) acc = acc + epi.bias[n];
-    if (epi.kind == EPI_BIAS_GELU) acc = gelu_tanh(acc);
-    if (epi.kind == EPI_BIAS_RESID)
-        acc = acc + epi.resid[(epi.resid_rows > 0 ? m % epi.resid_rows : m) * epi.ld_resid + n];
-    y[m * ldy + n] = acc;
+    v4f acc[NT];
+#pragma unroll
+    for (int b = 0; b < NT; ++b) acc[b] = v4f{0, 0, 0, 0};
+
+    for (int t = k0; t < k1; ++t) {
+        v4u w[NT], x[2];
+        uint32_t d[NT];
+#pragma unroll
+        for (int b = 0; b < NT; ++b) {
+            w[b] = *reinterpret_cast<const v4u *>(wp[b] + (int64_t)t * 1024);
+            d[b] = dp[b][(int64_t)t * 64];
+        }
+        // blocks past K: the last one again, against zero nibbles and scales
+        const int kb = 4 * t + (g >> 1), last = G.KB - 1;
+        x[0] = *reinterpret_cast<const v4u *>(xr + min(kb, last) * QK);
+        x[1] = *reinterpret_cast<const v4u *>(xr + min(kb + 2, last) * QK);
+        const v2i dx = {(int)(dr[min(4 * t + g, last)] & 0xffffu), 0};
+        // x[h]: 16 bytes of block 2 h + (g >> 1) -> xb[j]: 8 of block j
+        v2i xb[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const auto p = __builtin_amdgcn_permlane32_swap(x[h][c], x[h][c + 2], false, false);
+                xb[2 * h][c] = (int)p[0];
+                xb[2 * h + 1][c] = (int)p[1];
+            }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int b = 0; b < NT; ++b) {
+                const v2i wv = {(int)((w[b][j] << 4) & 0xf0f0f0f0u), (int)(w[b][j] & 0xf0f0f0f0u)};
+                const v2i dw = {g == j ? (int)d[b] : 0, 0};
+                const v4i I = __builtin_amdgcn_mfma_i32_16x16x32_i8(
+                    __builtin_bit_cast(long, wv), __builtin_bit_cast(long, xb[j]), v4i{0, 0, 0, 0}, 0, 0, 0);
+                const v4f s = __builtin_amdgcn_mfma_f32_16x16x16f16(
+                    __builtin_bit_cast(v4h, dw), __builtin_bit_cast(v4h, dx), v4f{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[b][i] = fmaf((float)I[i], s[i], acc[b][i]);
+            }
+    }
+
+#pragma unroll
+    for (int b = 0; b < NT; ++b) *reinterpret_cast<v4f *>(&part[wave][r][16 * b + 4 * g]) = acc[b] * 0.0625f;
+    __syncthreads();
+    const int cols = COLS * groups, rows = min(16, G.M - m0);
+    for (int i = tid; i < rows * cols; i += Q4_NT) {
+        const int row = i / cols, c = i - row * cols, grp = c / COLS;
+        const int64_t mr = m0 + row, n = (int64_t)col * cols + c;
+        if (n >= G.N) continue;
+        float v = part[grp << G.lwk][row][c % COLS];
+        for (int k = 1; k < G.wk; ++k) v = v + part[(grp << G.lwk) + k][row][c % COLS];
+        if (epi.kind != EPI_NONE) v = v + epi.bias[n];
+        if (epi.kind == EPI_BIAS_GELU) v = gelu_tanh(v);
+        if (epi.kind == EPI_BIAS_RESID)
+            v = v + epi.resid[(epi.resid_rows > 0 ? mr % epi.resid_rows : mr) * epi.ld_resid + n];
+        y[mr * ldy + n] = v;
+    }
 }
+
 hipError_t launch_mul_mat_q4(const Q4View &w, const int8_t *xq, const uint32_t *xds, int64_t M, float *y,
                              int64_t ldy, const EpiParams &epi, hipStream_t stream) {
-    hipLaunchKernelGGL(k_mul_mat_q4, dim3((unsigned)((M * w.N + 255) / 256)), dim3(256), 0, stream, w,
-                       w.tiles_k(), xq, xds, M, y, ldy, epi);
+    // Parts of K: until the column groups' waves are 14 a CU (4096 x 14336, one
+    // row: 10.5 us in 8 parts, 10.1 in 4, 10.4 in 2, 17 in 1).  From the weight's
+    // shape alone, so that a row's sums are grouped the same whatever M is.
+    int wk = 1, lwk = 0;
+    for (; wk < Q4_NW && wk < w.tiles_k() && w.tiles_n() * wk < 3584; ++lwk) wk *= 2;
+    const int64_t rg = (M + 15) / 16;
+    // two column groups a wave, one read of the rows for both, where that leaves
+    // a workgroup for half of the CUs: 16 x 4096 x 14336 10.2 us (one group
+    // 14.9), 64 x 4320 x 1152 5.9 (7.3); below, 16 x 4096 x 4096 6.2 (5.7),
+    // 43 x 4320 x 1152 5.8 (4.8)
+    const bool two = w.tiles_n() * rg * wk / Q4_NW > 256;
+    const int nt = two ? 2 : 1;
+    const int64_t per_wg = (int64_t)(Q4_NW / wk) * nt;
+    const Q4Grid G{wk, lwk, (int)w.tiles_k(), (int)(w.K / QK), (int)M, (int)w.N, (int)rg};
+    auto kern = two ? k_mul_mat_q4<2> : k_mul_mat_q4<1>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)((w.tiles_n() + per_wg - 1) / per_wg * rg)), dim3(Q4_NT), 0, stream, w.qs,
+                       w.d, G, xq, xds, y, ldy, epi);
     return hipGetLastError();
 }
 
