@@ -275,6 +275,8 @@ static int check_paged_shape(int64_t n_seq, int64_t max_len, int64_t n_q_head, i
     if (n_seq > 65535 || max_len > (1 << 30) || n_q_head > 1024 || d_head % 8 || d_head > 256)
         return fail(S2X_ERR_UNSUPPORTED,
                     "%s: n_seq <= 65,535, max_len <= 2^30, n_q_head <= 1,024, d_head %% 8 == 0 up to 256", who);
+    if (n_seq * n_kv_head * ((n_q_head / n_kv_head + 15) / 16) > (1 << 22))
+        return fail(S2X_ERR_UNSUPPORTED, "%s: at most 2^22 sequences x key heads (in 16 query heads each)", who);
     return S2X_OK;
 }
 

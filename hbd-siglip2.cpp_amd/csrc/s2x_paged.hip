@@ -18,20 +18,22 @@
 //    rows as they lie, staged in a part of LDS that is the wave's own.
 //  * The next tile's keys and values are loaded once the scores have freed
 //    the registers, and the page ids of the one after.
-// A workgroup's four waves join in LDS; a sequence's chunks, where there is
-// more than one, in k_attn_join.
+// A workgroup's waves join in LDS; a sequence's chunks, where there is more than
+// one, in k_attn_join.  Measured (both launches): one sequence of 131,071
+// tokens, 32 / 8 heads of 128, 103 us = 5.2 TB/s of keys and values, what a
+// large copy reaches; 60 sequences up to 8,000 in pages of 16, 133 us = 4.2.
 #include "s2x_decode.h"
 #include "s2x_device.h"
 
 namespace s2x {
 
-constexpr int PA_NT = 256, PA_NW = PA_NT / WAVE;
-constexpr int PA_TILE = 32;             // keys of a wave's tile
-constexpr int PA_STEP = PA_NW * PA_TILE;  // ... of a workgroup's
+constexpr int PA_ALIGN = 32;  // chunks begin at multiples of the largest tile
+constexpr int PJ_NT = 256;    // threads of the join
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef short v8s __attribute__((ext_vector_type(8)));
+typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
 
 template <typename T> struct Pa;
 // Terms of the cache's type that a probability enters the second product as:
@@ -43,12 +45,18 @@ template <> struct Pa<_Float16> {
     static __device__ __forceinline__ v4f mfma(vec a, vec b, v4f c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
+    static __device__ __forceinline__ v4f mfma4(v4s a, v4s b, v4f c) {
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(v4h, a), __builtin_bit_cast(v4h, b), c, 0, 0, 0);
+    }
 };
 template <> struct Pa<__bf16> {
     typedef v8bf vec;
     static constexpr float up = 1.0f, down = 1.0f;
     static __device__ __forceinline__ v4f mfma(vec a, vec b, v4f c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ v4f mfma4(v4s a, v4s b, v4f c) {
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
     }
 };
 
@@ -60,13 +68,8 @@ __device__ __forceinline__ PaRange pa_range(const AttnPaged &p, int s) {
     PaRange r;
     r.len = min((int64_t)min(max(p.kv_len[s], 0), p.max_len), p.ld_table << p.kv.page_shift);
     r.first = p.window > 0 ? max(r.len - p.window, (int64_t)0) : 0;
-    r.begin = r.first & ~(int64_t)(PA_TILE - 1);
+    r.begin = r.first & ~(int64_t)(PA_ALIGN - 1);
     return r;
-}
-
-constexpr int pa_lds_bytes(int DC) {
-    const int v = PA_NW * PA_TILE * DC * 64 + 64, o = PA_NW * 16 * (DC * 32 + 4) * 4;
-    return v > o ? v : o;
 }
 
 // Values 4 e .. 4 e + 3 of head h: the sums over its keys by the sum of the
@@ -87,26 +90,46 @@ __device__ __forceinline__ void pa_write(const AttnPaged &p, int s, int h, int d
     if (e == 0 && p.lse) p.lse[(int64_t)s * p.n_q_head + h] = (M + log2f(L)) * 0.693147180559945309f;
 }
 
-// DC: 32-value chunks of a head; EXACT: d_head = 32 DC; NP: terms of P.
-template <typename TC, int DC, bool EXACT, int NP>
-__global__ __launch_bounds__(PA_NT) void k_attn_paged(AttnPaged p, int chunk, int n_split) {
+// DC: 32-value chunks of a head; EXACT: d_head = 32 DC; NP: terms of P; KT: 16-key
+// parts of a tile; NW: waves of a workgroup.
+template <typename TC, int DC, bool EXACT, int NP, int KT, int NW>
+__global__ __launch_bounds__(NW * WAVE) void k_attn_paged(AttnPaged p, int chunk, int n_split) {
     typedef typename Pa<TC>::vec vec;
-    constexpr int DP = 32 * DC, DT = 2 * DC;
-    __shared__ __align__(16) uint8_t lds[pa_lds_bytes(DC)];
-    __shared__ float ml[PA_NW][2][16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
-    const int split = blockIdx.x, s = blockIdx.z, d = EXACT ? DP : p.kv.d_head, nch = d / 8;
-    const int group = p.n_q_head / p.kv.n_head, parts = (group + 15) / 16;
-    const int hk = blockIdx.y / parts, h0 = hk * group + (blockIdx.y - hk * parts) * 16;
+    constexpr int DP = 32 * DC, DT = 2 * DC, VT = DC * KT;  // values padded, 16-value parts, V loads of a tile
+    constexpr int TILE = 16 * KT, STEP = NW * TILE, NT = NW * WAVE;
+    extern __shared__ __align__(16) uint8_t lds[];  // V tiles of the waves, then their sums
+    __shared__ float ml[NW][2][16];
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int d = EXACT ? DP : p.kv.d_head, nch = d / 8;
+    const int group = p.n_q_head / p.kv.n_head, parts = (group + 15) / 16, H = p.kv.n_head * parts;
+    // Workgroup -> (sequence, chunk), head.  Workgroups go round the 8 XCDs: the
+    // heads of one chunk follow each other on one XCD (a token-major row's
+    // cache lines are shared between heads), and the chunks of a sequence
+    // lie on different ones (u = chunk n_seq + (s + chunk) % n_seq), since
+    // ragged sequences leave the later chunks empty.
+    const int U = p.n_seq * n_split, octs = U / 8 * 8;
+    int u, hp;
+    if ((int)blockIdx.x < octs * H) {
+        const int q8 = blockIdx.x / 8, o = q8 / H;
+        u = 8 * o + blockIdx.x % 8;
+        hp = q8 - o * H;
+    } else {
+        const int b = blockIdx.x - octs * H;
+        hp = b / (U - octs);
+        u = octs + b - hp * (U - octs);
+    }
+    const int split = u / p.n_seq, s = (u - split * p.n_seq + split) % p.n_seq;
+    const int hk = hp / parts, h0 = hk * group + (hp - hk * parts) * 16;
     const int R = min(16, (hk + 1) * group - h0);
     const PaRange kr = pa_range(p, s);
     const int64_t start = kr.begin + (int64_t)split * chunk, end = min(start + chunk, kr.len);
-    if (start >= end && (n_split > 1)) return;  // (uniform; the only chunk writes zeros)
+    if (start >= end && n_split > 1) return;  // (uniform; an only chunk writes zeros)
 
     const TC *kp = (const TC *)p.kv.k + hk * p.kv.ld_head, *vp = (const TC *)p.kv.v + hk * p.kv.ld_head;
     const int32_t *row = p.table + s * p.ld_table;
     const uint32_t pmask = (1u << p.kv.page_shift) - 1, ldp = (uint32_t)p.kv.ld_page, ldt = (uint32_t)p.kv.ld_tok;
-    TC *vl = reinterpret_cast<TC *>(lds) + wave * PA_TILE * d;
+    TC *vl = reinterpret_cast<TC *>(lds) + wave * TILE * d;
 
     vec q[DC];
 #pragma unroll
@@ -116,9 +139,9 @@ __global__ __launch_bounds__(PA_NT) void k_attn_paged(AttnPaged p, int chunk, in
             q[c] = *reinterpret_cast<const vec *>((const TC *)p.q + s * p.ld_q + (int64_t)(h0 + r) * d + 32 * c + 8 * g);
     }
 
-    // page of key t0 + lane % 32, -1 unseen
+    // page of key t0 + lane % TILE, -1 unseen
     auto page_of = [&](int64_t t0) {
-        const int64_t t = t0 + (lane & 31);
+        const int64_t t = t0 + (lane & (TILE - 1));
         int32_t id = -1;
         if (t >= kr.first && t < end) {
             id = row[t >> p.kv.page_shift];
@@ -126,14 +149,14 @@ __global__ __launch_bounds__(PA_NT) void k_attn_paged(AttnPaged p, int chunk, in
         }
         return id;
     };
-    vec k[2][DC], v[DT];
+    vec k[KT][DC], v[VT];
     const uint32_t magic = (65536u + nch - 1) / nch;  // f / nch for f < 1,024
     uint32_t seen = 0;
     auto load = [&](int64_t t0, int32_t id) {
-        seen = (uint32_t)__builtin_amdgcn_ballot_w64(id >= 0);
+        seen = (uint32_t)__builtin_amdgcn_ballot_w64(id >= 0);  // (lanes repeat the tile's keys)
         const bool all = EXACT && seen == ~0u;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < KT; ++j) {
             const int key = 16 * j + r;
             const uint32_t pid = (uint32_t)__shfl(id, key);
             const TC *src = kp + ((uint64_t)pid * ldp + (((uint32_t)t0 + key) & pmask) * (uint64_t)ldt + 8 * g);
@@ -145,12 +168,12 @@ __global__ __launch_bounds__(PA_NT) void k_attn_paged(AttnPaged p, int chunk, in
             }
         }
 #pragma unroll
-        for (int i = 0; i < DT; ++i) {
+        for (int i = 0; i < VT; ++i) {
             const uint32_t f = i * WAVE + lane, key = EXACT ? f / (DP / 8) : f * magic >> 16;
-            const uint32_t pid = (uint32_t)__shfl(id, (int)(key & 31));
+            const uint32_t pid = (uint32_t)__shfl(id, (int)(key & (TILE - 1)));
             const TC *src = vp + ((uint64_t)pid * ldp + (((uint32_t)t0 + key) & pmask) * (uint64_t)ldt + 8 * (f - key * nch));
             v[i] = vec{};
-            if (all || (key < PA_TILE && (int32_t)pid >= 0)) v[i] = *reinterpret_cast<const vec *>(src);
+            if (all || (key < TILE && (int32_t)pid >= 0)) v[i] = *reinterpret_cast<const vec *>(src);
         }
     };
 
@@ -160,34 +183,34 @@ __global__ __launch_bounds__(PA_NT) void k_attn_paged(AttnPaged p, int chunk, in
     for (int i = 0; i < DT; ++i) o[i] = v4f{0, 0, 0, 0};
     const float sc = p.scale * 1.44269504088896341f;  // log2(e)
 
-    int64_t t0 = start + wave * PA_TILE;
+    int64_t t0 = start + wave * TILE;
     int32_t id_next = -1;
     if (t0 < end) {
         load(t0, page_of(t0));
-        id_next = page_of(t0 + PA_STEP);
+        id_next = page_of(t0 + STEP);
     }
-    for (; t0 < end; t0 += PA_STEP) {
+    for (; t0 < end; t0 += STEP) {
         const uint32_t mask = seen;
 #pragma unroll
-        for (int i = 0; i < DT; ++i) {
-            if (EXACT || i * WAVE + lane < PA_TILE * nch)
+        for (int i = 0; i < VT; ++i) {
+            if (EXACT || i * WAVE + lane < TILE * nch)
                 *reinterpret_cast<vec *>(vl + (i * WAVE + lane) * 8) = v[i];
         }
-        v4f st[2];
+        v4f st[KT];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < KT; ++j) {
             st[j] = v4f{0, 0, 0, 0};
 #pragma unroll
             for (int c = 0; c < DC; ++c) st[j] = Pa<TC>::mfma(k[j][c], q[c], st[j]);
         }
-        if (t0 + PA_STEP < end) {
-            load(t0 + PA_STEP, id_next);
-            id_next = page_of(t0 + 2 * PA_STEP);
+        if (t0 + STEP < end) {  // (k and v are free)
+            load(t0 + STEP, id_next);
+            id_next = page_of(t0 + 2 * STEP);
         }
         // the softmax of head r over keys 4 g + i, 16 + 4 g + i
         float mt = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < KT; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 st[j][i] = st[j][i] * sc;
@@ -200,9 +223,9 @@ __global__ __launch_bounds__(PA_NT) void k_attn_paged(AttnPaged p, int chunk, in
         const float alpha = __builtin_amdgcn_exp2f(m - base);
         m = mn;
         l = l * alpha;
-        vec pt[NP];
+        vec pt[NP];  // (KT = 1: its first four)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < KT; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float e = __builtin_amdgcn_exp2f(st[j][i] - base);
@@ -220,17 +243,22 @@ __global__ __launch_bounds__(PA_NT) void k_attn_paged(AttnPaged p, int chunk, in
 #pragma unroll
         for (int i = 0; i < DT; ++i) {
             if (!EXACT && 16 * i >= d) break;
-            v8s a;
+            v4s a[KT];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < KT; ++j) {
                 TC *src = vl + (16 * j + 4 * g + (r >> 2)) * d + 16 * i + (r & 3) * 4;
-                const v4s t = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) v4s *)src);
-#pragma unroll
-                for (int n = 0; n < 4; ++n) a[4 * j + n] = t[n];
+                a[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)src);
             }
 #pragma unroll
-            for (int n = 0; n < NP; ++n) o[i] = Pa<TC>::mfma(__builtin_bit_cast(vec, a), pt[n], o[i]);
+            for (int n = 0; n < NP; ++n) {
+                const v8s pn = __builtin_bit_cast(v8s, pt[n]);
+                if constexpr (KT == 2) {
+                    const v8s a8 = __builtin_shufflevector(a[0], a[KT - 1], 0, 1, 2, 3, 4, 5, 6, 7);
+                    o[i] = Pa<TC>::mfma(__builtin_bit_cast(vec, a8), pt[n], o[i]);
+                } else {
+                    o[i] = Pa<TC>::mfma4(a[0], __builtin_shufflevector(pn, pn, 0, 1, 2, 3), o[i]);
+                }
+            }
         }
         __builtin_amdgcn_wave_barrier();
     }
@@ -238,31 +266,31 @@ __global__ __launch_bounds__(PA_NT) void k_attn_paged(AttnPaged p, int chunk, in
     // join the waves: o[i] is values 16 i + 4 g .. + 3 of head r
     l = l + __shfl_xor(l, 16);
     l = l + __shfl_xor(l, 32);
-    float *ol = reinterpret_cast<float *>(lds);  // [wave][head][DP + 4]
+    float *ol = reinterpret_cast<float *>(lds);  // [wave][head < R][DP + 4]
     __syncthreads();
     if (r < R) {
 #pragma unroll
         for (int i = 0; i < DT; ++i)
-            *reinterpret_cast<v4f *>(ol + (wave * 16 + r) * (DP + 4) + 16 * i + 4 * g) = o[i];
+            *reinterpret_cast<v4f *>(ol + (wave * R + r) * (DP + 4) + 16 * i + 4 * g) = o[i];
         if (g == 0) {
             ml[wave][0][r] = m;
             ml[wave][1][r] = l;
         }
     }
     __syncthreads();
-    for (int i = tid; i < R * nch * 2; i += PA_NT) {
+    for (int i = tid; i < R * nch * 2; i += NT) {
         const int h = i / (nch * 2), e = i - h * (nch * 2);
         float M = ml[0][0][h];
 #pragma unroll
-        for (int w = 1; w < PA_NW; ++w) M = fmaxf(M, ml[w][0][h]);
+        for (int w = 1; w < NW; ++w) M = fmaxf(M, ml[w][0][h]);
         const float base = M == -INFINITY ? 0.0f : M;
         v4f a = {0, 0, 0, 0};
         float L = 0.0f;
 #pragma unroll
-        for (int w = 0; w < PA_NW; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float f = __builtin_amdgcn_exp2f(ml[w][0][h] - base);
             L = fmaf(ml[w][1][h], f, L);
-            const v4f x = *reinterpret_cast<const v4f *>(ol + (w * 16 + h) * (DP + 4) + 4 * e);
+            const v4f x = *reinterpret_cast<const v4f *>(ol + (w * R + h) * (DP + 4) + 4 * e);
 #pragma unroll
             for (int n = 0; n < 4; ++n) a[n] = fmaf(x[n], f, a[n]);
         }
@@ -279,96 +307,128 @@ __global__ __launch_bounds__(PA_NT) void k_attn_paged(AttnPaged p, int chunk, in
     }
 }
 
-// Chunks of a sequence joined, one workgroup per sequence and query head: the
-// chunks in PA_NT / (d / 4) groups, a thread 4 values of one.
+// Chunks of a sequence joined: a workgroup per query head and 32 values of it,
+// 8 lanes of 4 values by 32 groups of chunks, each with its own running maximum.
+// The first loads are of chunks that the launch has room for, whether the
+// sequence has them or not, so that they do not wait for its length.
 template <typename TC>
-__global__ __launch_bounds__(PA_NT) void k_attn_join(AttnPaged p, int chunk, int n_split) {
-    __shared__ __align__(16) float part[PA_NT * 4];
-    __shared__ float red[PA_NW], lsum[PA_NT];
-    const int h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, d = p.kv.d_head, nq = d / 4;
+__global__ __launch_bounds__(PJ_NT) void k_attn_join(AttnPaged p, int chunk, int n_split) {
+    constexpr int LANES = 8, GROUPS = PJ_NT / LANES;
+    __shared__ __align__(16) float part[GROUPS][LANES * 4 + 4];
+    __shared__ float gm[GROUPS], gl[GROUPS];
+    const int tid = threadIdx.x, d = p.kv.d_head, nq = d / 4, pieces = (nq + LANES - 1) / LANES;
+    const int h = blockIdx.x / pieces, s = blockIdx.y;
+    const int grp = tid / LANES, e = (blockIdx.x - h * pieces) * LANES + tid % LANES;
+    const int64_t at = ((int64_t)s * p.n_q_head + h) * n_split;
+    const v4f *ov = reinterpret_cast<const v4f *>(p.ws) + at * nq + min(e, nq - 1);
+    const float2 *mlp = reinterpret_cast<const float2 *>((const float *)p.ws + (int64_t)p.n_seq * p.n_q_head * n_split * d) + at;
+    float2 t = mlp[min(grp, n_split - 1)];
+    v4f x = ov[(int64_t)min(grp, n_split - 1) * nq];
     const PaRange kr = pa_range(p, s);
     const int n = kr.len > kr.begin ? (int)((kr.len - kr.begin + chunk - 1) / chunk) : 0;
-    const int64_t at = ((int64_t)s * p.n_q_head + h) * n_split;
-    const float *ws = (const float *)p.ws;
-    const float2 *mlp = reinterpret_cast<const float2 *>(ws + (int64_t)p.n_seq * p.n_q_head * n_split * d) + at;
-    float M = -INFINITY;
-    for (int i = tid; i < n; i += PA_NT) M = fmaxf(M, mlp[i].x);
-    M = group_max<64>(M);
-    if ((tid & 63) == 0) red[tid >> 6] = M;
-    __syncthreads();
-    M = red[0];
-#pragma unroll
-    for (int w = 1; w < PA_NW; ++w) M = fmaxf(M, red[w]);
-    const float base = M == -INFINITY ? 0.0f : M;
-    const int groups = PA_NT / nq, grp = tid / nq, e = tid - grp * nq;
     v4f a = {0, 0, 0, 0};
-    float L = 0.0f;
-    if (grp < groups) {
-        for (int i = grp; i < n; i += groups) {
-            const float2 t = mlp[i];
-            const float f = __builtin_amdgcn_exp2f(t.x - base);
-            L = fmaf(t.y, f, L);
-            const v4f x = reinterpret_cast<const v4f *>(ws)[(at + i) * nq + e];
+    float M = -INFINITY, L = 0.0f;
+    for (int i = grp; i < n; i += GROUPS) {
+        const int next = min(i + GROUPS, n - 1);
+        const float2 tn = mlp[next];
+        const v4f xn = ov[(int64_t)next * nq];
+        const float mn = fmaxf(M, t.x), base = mn == -INFINITY ? 0.0f : mn;
+        const float f0 = __builtin_amdgcn_exp2f(M - base), f1 = __builtin_amdgcn_exp2f(t.x - base);
+        L = fmaf(t.y, f1, L * f0);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) a[c] = fmaf(x[c], f, a[c]);
-        }
-        reinterpret_cast<v4f *>(part)[tid] = a;
-        lsum[tid] = L;
+        for (int c = 0; c < 4; ++c) a[c] = fmaf(x[c], f1, a[c] * f0);
+        M = mn;
+        t = tn;
+        x = xn;
+    }
+    *reinterpret_cast<v4f *>(&part[grp][(tid % LANES) * 4]) = a;
+    if (tid % LANES == 0) {
+        gm[grp] = M;
+        gl[grp] = L;
     }
     __syncthreads();
-    if (grp == 0) {
-        for (int i = 1; i < groups; ++i) {
-            L = L + lsum[i * nq + e];
-            a = a + reinterpret_cast<const v4f *>(part)[i * nq + e];
-        }
-        pa_write<TC>(p, s, h, d, e, a, M, L);
-    }
+    // a wave's half: 32 lanes' groups of one maximum, 4 values each for the
+    // first 8 lanes
+    if (tid >= 32) return;
+    M = gm[tid];
+    const float top = group_max<32>(M), base = top == -INFINITY ? 0.0f : top;
+    const float f = __builtin_amdgcn_exp2f(M - base);
+    L = group_sum<32>(gl[tid] * f);
+    // lane tid: value tid of the piece
+    float y = 0.0f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) y = fmaf(part[g][tid], __shfl(f, g, 32), y);
+    v4f yv;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) yv[c] = __shfl(y, (tid & 7) * 4 + c, 32);
+    if (tid < LANES && e < nq) pa_write<TC>(p, s, h, d, e, yv, top, L);
 }
 
-// Chunk length and their number for a launch: about 4 workgroups a CU where
-// the lengths allow it, whole steps of a workgroup's four waves.
-static void pa_plan(int64_t n_seq, int64_t max_len, int64_t n_q_head, int64_t n_kv_head, int &chunk, int &n_split) {
+// Chunk length, number of chunks and waves of a workgroup.  A CU takes some 31
+// bytes a ns, whatever its waves have in flight (one step of 128 keys of 128
+// halves 2.1 us), so a launch wants all CUs at work to the end; a second
+// launch, the join, is 3 us and its gap.
+//  * no split, 8 waves a workgroup, for what a split does not speed up: up to
+//    320 tokens (3 sequences up to 300, 16 heads of 72: 7.3 us, in two chunks
+//    8.4) and, from 128 workgroups on, up to 1,024 (32 x 1,000, 8 key heads of
+//    128: 16.0 us, in chunks of 256 18.9).
+//  * one sequence: two workgroups a CU (131,071 tokens, 8 key heads: chunks of
+//    2,048 103 us, of 1,024 105, of 512 108, of 4,096 110; 2,000 tokens: of
+//    128 8.9 us, of 256 10.6), a batch, whose lengths differ: up to 16 a CU,
+//    chunks of 256 to 1,024 (60 up to 8,000: 1,024 133 us, 2,048 155; 16 up
+//    to 8,000: 256 36.7, 512 40, 1,024 43; 8 up to 4,000: 256 17.5, 128 20).
+//  * more waves a workgroup, loads of the next tile before the first product:
+//    no faster; the bytes a CU can take bound it.
+struct PaPlan {
+    int chunk, n_split, nw;
+};
+static PaPlan pa_plan(int64_t n_seq, int64_t max_len, int64_t n_q_head, int64_t n_kv_head) {
     const int64_t units = n_seq * n_kv_head * ((n_q_head / n_kv_head + 15) / 16);
-    const int64_t span = max_len + PA_TILE;  // (the first tile may begin before a window)
-    int64_t c = (span * units + 1023) / 1024;
-    c = (c + PA_STEP - 1) / PA_STEP * PA_STEP;
-    if (c < 2 * PA_STEP) c = 2 * PA_STEP;
-    if (c > 4096) c = 4096;
-    chunk = (int)c;
-    n_split = (int)((span + c - 1) / c);
+    const int64_t span = max_len + PA_ALIGN;  // (the first tile may begin before a window)
+    if (max_len <= 320 || (units >= 128 && max_len <= 1024))
+        return PaPlan{(int)((span + 127) / 128 * 128), 1, 8};
+    const int64_t wgs = 512 * (n_seq < 8 ? n_seq : 8);
+    const int64_t least = span * units < 65536 ? 128 : 256, most = n_seq == 1 ? 2048 : 1024;
+    int64_t c = span * units / wgs;
+    c = c < least ? least : c > most ? most : c;
+    if (c < span * units >> 22) c = span * units >> 22;  // (a grid of at most 2^23)
+    c = (c + 127) / 128 * 128;
+    return PaPlan{(int)c, (int)((span + c - 1) / c), 4};
 }
 
 size_t attn_paged_workspace(int64_t n_seq, int64_t max_len, int64_t n_q_head, int64_t n_kv_head, int64_t d_head) {
-    int chunk, n_split;
-    pa_plan(n_seq, max_len, n_q_head, n_kv_head, chunk, n_split);
-    return n_split > 1 ? (size_t)(n_seq * n_q_head) * n_split * (d_head + 2) * 4 : 0;
+    const int n = pa_plan(n_seq, max_len, n_q_head, n_kv_head).n_split;
+    return n > 1 ? (size_t)(n_seq * n_q_head) * n * (d_head + 2) * 4 : 0;
 }
 
+template <typename TC, int DC, bool EXACT, int KT, int NW>
+static hipError_t run_paged_w(const AttnPaged &p, const PaPlan &P, hipStream_t stream) {
+    const int group = p.n_q_head / p.kv.n_head, R = group < 16 ? group : 16;
+    const int64_t wgs = (int64_t)P.n_split * p.kv.n_head * ((group + 15) / 16) * p.n_seq;
+    const int v = NW * KT * 16 * p.kv.d_head * 2 + 64, o = NW * R * (DC * 32 + 4) * 4, lds = v > o ? v : o;
+    constexpr bool BF = sizeof(TC) == 2 && Pa<TC>::up == 1.0f;
+    auto kern = BF && p.out_f32 ? k_attn_paged<TC, DC, EXACT, BF ? 3 : 2, KT, NW> : k_attn_paged<TC, DC, EXACT, 2, KT, NW>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(NW * WAVE), lds, stream, p, P.chunk, P.n_split);
+    return hipGetLastError();
+}
 template <typename TC, int DC, bool EXACT>
-static void run_paged(const AttnPaged &p, int chunk, int n_split, hipStream_t stream) {
-    const int group = p.n_q_head / p.kv.n_head;
-    const dim3 grid(n_split, p.kv.n_head * ((group + 15) / 16), p.n_seq);
-    constexpr int NP = sizeof(TC) == 2 && Pa<TC>::up == 1.0f ? 3 : 2;
-    if (NP == 3 && p.out_f32)
-        hipLaunchKernelGGL((k_attn_paged<TC, DC, EXACT, NP>), grid, dim3(PA_NT), 0, stream, p, chunk, n_split);
-    else
-        hipLaunchKernelGGL((k_attn_paged<TC, DC, EXACT, 2>), grid, dim3(PA_NT), 0, stream, p, chunk, n_split);
+static hipError_t run_paged(const AttnPaged &p, const PaPlan &P, hipStream_t stream) {
+    constexpr int KT = DC > 4 ? 1 : 2;
+    return P.nw == 8 ? run_paged_w<TC, DC, EXACT, KT, 8>(p, P, stream) : run_paged_w<TC, DC, EXACT, KT, 4>(p, P, stream);
 }
 template <typename TC>
 static hipError_t run_paged_d(const AttnPaged &p, hipStream_t stream) {
-    int chunk, n_split;
-    pa_plan(p.n_seq, p.max_len, p.n_q_head, p.kv.n_head, chunk, n_split);
+    const PaPlan P = pa_plan(p.n_seq, p.max_len, p.n_q_head, p.kv.n_head);
     const int d = p.kv.d_head;
-    if (d == 64) run_paged<TC, 2, true>(p, chunk, n_split, stream);
-    else if (d == 128) run_paged<TC, 4, true>(p, chunk, n_split, stream);
-    else if (d == 256) run_paged<TC, 8, true>(p, chunk, n_split, stream);
-    else if (d < 64) run_paged<TC, 2, false>(p, chunk, n_split, stream);
-    else if (d <= 96) run_paged<TC, 3, false>(p, chunk, n_split, stream);
-    else if (d <= 192) run_paged<TC, 6, false>(p, chunk, n_split, stream);
-    else run_paged<TC, 8, false>(p, chunk, n_split, stream);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || n_split == 1) return e;
-    hipLaunchKernelGGL(k_attn_join<TC>, dim3(p.n_q_head, p.n_seq), dim3(PA_NT), 0, stream, p, chunk, n_split);
+    const hipError_t e = d == 64   ? run_paged<TC, 2, true>(p, P, stream)
+                         : d == 128 ? run_paged<TC, 4, true>(p, P, stream)
+                         : d == 256 ? run_paged<TC, 8, true>(p, P, stream)
+                         : d < 64   ? run_paged<TC, 2, false>(p, P, stream)
+                         : d <= 96  ? run_paged<TC, 3, false>(p, P, stream)
+                         : d <= 192 ? run_paged<TC, 6, false>(p, P, stream)
+                                    : run_paged<TC, 8, false>(p, P, stream);
+    if (e != hipSuccess || P.n_split == 1) return e;
+    hipLaunchKernelGGL(k_attn_join<TC>, dim3(p.n_q_head * ((d + 31) / 32), p.n_seq), dim3(PJ_NT), 0, stream, p, P.chunk, P.n_split);
     return hipGetLastError();
 }
 hipError_t launch_attn_paged(const AttnPaged &p, hipStream_t stream) {

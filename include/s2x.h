@@ -468,7 +468,8 @@ int s2x_qk_norm_rope_kv(const void *x, int32_t x_type, int64_t ld_x, int64_t n_t
  * table's row count as that; pages outside 0 .. n_pages - 1 are not seen; a
  * sequence that sees nothing gets zeros and lse = -inf.  Keys and values of
  * unseen places are never read.  q and out 16-byte aligned, ld_q and ld_out
- * multiples of 8.  n_seq <= 65,535; workspace (256-byte aligned, own to the call until it has finished) of
+ * multiples of 8.  n_seq <= 65,535, n_seq * n_head of the cache <= 2^22;
+ * workspace (256-byte aligned, the call's own until it has finished) of
  * s2x_attn_paged_workspace_size() bytes; NULL where that is 0. */
 size_t s2x_attn_paged_workspace_size(int64_t n_seq, int64_t max_len, int64_t n_q_head,
                                      int64_t n_kv_head, int64_t d_head);

@@ -87,7 +87,9 @@ def test_no_rows_is_no_work():
     (dict(n_q_head=0), INVALID), (dict(out_type=s2x.TYPE_BF16), UNSUPPORTED), (dict(out_type=9), UNSUPPORTED),
     (dict(window=-1), INVALID), (dict(ld_table=-1), INVALID), (dict(ld_q=504), INVALID), (dict(ld_out=516), INVALID),
     (dict(q=None), INVALID), (dict(out=None), INVALID), (dict(kv_len=None), INVALID), (dict(table=None), INVALID),
-    (dict(q=ODD), INVALID), (dict(out=ODD), INVALID)])
+    (dict(q=ODD), INVALID), (dict(out=ODD), INVALID),
+    (dict(n_seq=65535, n_q_head=128, ld_q=1 << 14, ld_out=1 << 14,
+          cache=cache(n_head=128, ld_page=128 * 16 * 128)), UNSUPPORTED)])
 def test_attn_refusals(change, status):
     assert attn(**change) == status, s2x.lib.s2x_last_error()
 
@@ -95,12 +97,13 @@ def test_attn_refusals(change, status):
 def test_attn_workspace_refusals():
     size = s2x.lib.s2x_attn_paged_workspace_size
     assert size(-1, 100, 4, 2, 128) == 0 and size(1, 100, 3, 2, 128) == 0 and size(1, 100, 4, 2, 100) == 0
+    assert size(100, 100, 4, 2, 128) == 0  # one chunk a sequence
+    assert size(65535, 1 << 30, 64, 64, 128) < 1 << 42
     need = size(1, 1 << 17, 4, 2, 128)
-    assert need < 1 << 30
-    if need:
-        assert attn(max_len=1 << 17, ws_bytes=need - 1) == WORKSPACE
-        assert attn(max_len=1 << 17, ws=None, ws_bytes=need) == INVALID
-        assert attn(max_len=1 << 17, ws=ODD, ws_bytes=need) == INVALID
+    assert 0 < need < 1 << 30
+    assert attn(max_len=1 << 17, ws_bytes=need - 1) == WORKSPACE
+    assert attn(max_len=1 << 17, ws=None, ws_bytes=need) == INVALID
+    assert attn(max_len=1 << 17, ws=ODD, ws_bytes=need) == INVALID
 
 
 @pytest.mark.parametrize("change,status", [
