@@ -249,8 +249,8 @@ int s2x_qk_norm_rope_kv(const void *x, int32_t x_type, int64_t ld_x, int64_t n_t
     if (n_tok < 0 || n_q_head <= 0 || d_rot < 0 || d_rot % 2 || d_rot > v.d_head)
         return fail(S2X_ERR_INVALID_ARG, "%s: n_tok=%lld n_q_head=%lld d_rot=%lld", who, (long long)n_tok,
                     (long long)n_q_head, (long long)d_rot);
-    if (n_tok > (1 << 24) || n_q_head > 1024)
-        return fail(S2X_ERR_UNSUPPORTED, "%s: at most 2^24 rows and 1,024 query heads", who);
+    if (n_tok > (1 << 23) || n_q_head > 1024)
+        return fail(S2X_ERR_UNSUPPORTED, "%s: at most 2^23 rows and 1,024 query heads", who);
     if (ld_x < (n_q_head + 2 * v.n_head) * v.d_head || ld_x % 8 || ld_q < n_q_head * v.d_head || ld_q % 8)
         return fail(S2X_ERR_INVALID_ARG, "%s: ld_x=%lld / ld_q=%lld below the row or no multiple of 8", who,
                     (long long)ld_x, (long long)ld_q);

@@ -307,13 +307,14 @@ __global__ __launch_bounds__(NW * WAVE) void k_attn_paged(AttnPaged p, int chunk
     }
 }
 
-// Chunks of a sequence joined: a workgroup per query head and 32 values of it,
-// 8 lanes of 4 values by 32 groups of chunks, each with its own running maximum.
-// The first loads are of chunks that the launch has room for, whether the
-// sequence has them or not, so that they do not wait for its length.
-template <typename TC>
+// Chunks of a sequence joined: a workgroup per query head and 4 LANES values of
+// it, LANES lanes of 4 values by PJ_NT / LANES groups of chunks, each with its
+// own running maximum.  The first loads are of chunks that the launch has room
+// for, whether the sequence has them or not, so that they do not wait for its
+// length.
+template <typename TC, int LANES>
 __global__ __launch_bounds__(PJ_NT) void k_attn_join(AttnPaged p, int chunk, int n_split) {
-    constexpr int LANES = 8, GROUPS = PJ_NT / LANES;
+    constexpr int GROUPS = PJ_NT / LANES;
     __shared__ __align__(16) float part[GROUPS][LANES * 4 + 4];
     __shared__ float gm[GROUPS], gl[GROUPS];
     const int tid = threadIdx.x, d = p.kv.d_head, nq = d / 4, pieces = (nq + LANES - 1) / LANES;
@@ -347,21 +348,22 @@ __global__ __launch_bounds__(PJ_NT) void k_attn_join(AttnPaged p, int chunk, int
         gl[grp] = L;
     }
     __syncthreads();
-    // a wave's half: 32 lanes' groups of one maximum, 4 values each for the
-    // first 8 lanes
-    if (tid >= 32) return;
-    M = gm[tid];
-    const float top = group_max<32>(M), base = top == -INFINITY ? 0.0f : top;
-    const float f = __builtin_amdgcn_exp2f(M - base);
-    L = group_sum<32>(gl[tid] * f);
-    // lane tid: value tid of the piece
-    float y = 0.0f;
+    if (grp != 0 || e >= nq) return;
+    float top = gm[0];
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) y = fmaf(part[g][tid], __shfl(f, g, 32), y);
-    v4f yv;
+    for (int i = 1; i < GROUPS; ++i) top = fmaxf(top, gm[i]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    v4f y = {0, 0, 0, 0};
+    L = 0.0f;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) yv[c] = __shfl(y, (tid & 7) * 4 + c, 32);
-    if (tid < LANES && e < nq) pa_write<TC>(p, s, h, d, e, yv, top, L);
+    for (int i = 0; i < GROUPS; ++i) {
+        const float f = __builtin_amdgcn_exp2f(gm[i] - base);
+        L = fmaf(gl[i], f, L);
+        const v4f z = *reinterpret_cast<const v4f *>(&part[i][tid * 4]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) y[c] = fmaf(z[c], f, y[c]);
+    }
+    pa_write<TC>(p, s, h, d, e, y, top, L);
 }
 
 // Chunk length, number of chunks and waves of a workgroup.  A CU takes some 31
@@ -428,7 +430,13 @@ static hipError_t run_paged_d(const AttnPaged &p, hipStream_t stream) {
                          : d <= 192 ? run_paged<TC, 6, false>(p, P, stream)
                                     : run_paged<TC, 8, false>(p, P, stream);
     if (e != hipSuccess || P.n_split == 1) return e;
-    hipLaunchKernelGGL(k_attn_join<TC>, dim3(p.n_q_head * ((d + 31) / 32), p.n_seq), dim3(PJ_NT), 0, stream, p, P.chunk, P.n_split);
+    // few chunks: whole heads a workgroup (60 sequences of at most 8: 10.9 us
+    // with 32 values each, 5.0 with 128); many: more workgroups (128 chunks
+    // of one sequence: 8.2 us with 128, 4.8 with 32)
+    const bool few = P.n_split <= 16;
+    const int width = few ? 128 : 32;
+    auto join = few ? k_attn_join<TC, 32> : k_attn_join<TC, 8>;
+    hipLaunchKernelGGL(join, dim3(p.n_q_head * ((d + width - 1) / width), p.n_seq), dim3(PJ_NT), 0, stream, p, P.chunk, P.n_split);
     return hipGetLastError();
 }
 hipError_t launch_attn_paged(const AttnPaged &p, hipStream_t stream) {

@@ -12,9 +12,10 @@ namespace s2x {
 //   ceil((len + n) / page) - ceil(len / page)
 // in the free list.  One launch, no workspace: every workgroup sums all
 // lengths itself (8 bytes a sequence out of the L2) into LDS, then finds the
-// sequence of each of its rows and new pages by binary search there.  The
-// launch's latency is what it costs; two launches with the prefix sums in
-// memory would add one.
+// sequence of each of its rows and new pages by binary search there.  Its
+// latencies are what it costs (lengths in, sums, search, table, rows out: 5.1
+// us for 200 sequences with one row each, 6.5 for 700 with 86,000); two
+// launches with the sums in memory would add one.
 // ---------------------------------------------------------------------------
 constexpr int KS_NT = 1024;
 
@@ -27,26 +28,29 @@ __device__ __forceinline__ int ks_upper(const int32_t *first, int n, int32_t t) 
     return lo;
 }
 
+// PER: most sequences of a thread.
+template <int PER>
 __global__ __launch_bounds__(KS_NT) void k_kv_slots(KvSlots p) {
-    __shared__ int32_t tok0[KV_MAX_SEQ], page0[KV_MAX_SEQ];  // saturated starts
-    __shared__ int64_t wsum[2][KS_NT / WAVE], total[2];
+    __shared__ int32_t tok0[PER * KS_NT], page0[PER * KS_NT], held[PER * KS_NT];  // saturated starts, lengths
+    __shared__ int64_t wsum[2][KS_NT / WAVE];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int page_up = (1 << p.page_shift) - 1;
-    auto counts = [&](int b, int64_t &len, int64_t &n, int64_t &have, int64_t &fresh) {
-        len = max(p.kv_len[b], 0);
-        n = max(p.n_new[b], 0);
-        have = (len + page_up) >> p.page_shift;
-        fresh = ((len + n + page_up) >> p.page_shift) - have;
-    };
+    auto pages = [&](int64_t len) { return (len + page_up) >> p.page_shift; };
 
     // prefix sums: each thread a run of sequences, then the waves' sums
-    const int per = (p.n_seq + KS_NT - 1) / KS_NT;
-    const int b0 = min(tid * per, p.n_seq), b1 = min(b0 + per, p.n_seq);
-    int64_t st = 0, sp = 0, len, n, have, fresh;
-    for (int b = b0; b < b1; ++b) {
-        counts(b, len, n, have, fresh);
-        st += n;
-        sp += fresh;
+    const int per = PER == 1 ? 1 : (p.n_seq + KS_NT - 1) / KS_NT, b0 = tid * per;
+    int32_t len[PER], n[PER];
+    int64_t st = 0, sp = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const bool in = i < per && b0 + i < p.n_seq;
+        len[i] = in ? max(p.kv_len[b0 + i], 0) : 0;
+        n[i] = in ? max(p.n_new[b0 + i], 0) : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        st += n[i];
+        sp += pages((int64_t)len[i] + n[i]) - pages(len[i]);
     }
     int64_t it = st, ip = sp;  // inclusive over the wave
 #pragma unroll
@@ -62,38 +66,38 @@ __global__ __launch_bounds__(KS_NT) void k_kv_slots(KvSlots p) {
         wsum[1][wave] = ip;
     }
     __syncthreads();
-    int64_t bt = 0, bp = 0;
+    int64_t t0 = it - st, f0 = ip - sp, n_tok = 0, n_fresh = 0;
 #pragma unroll
     for (int w = 0; w < KS_NT / WAVE; ++w) {
         if (w < wave) {
-            bt += wsum[0][w];
-            bp += wsum[1][w];
+            t0 += wsum[0][w];
+            f0 += wsum[1][w];
+        }
+        n_tok += wsum[0][w];
+        n_fresh += wsum[1][w];
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int b = b0 + i;
+        if (i < per && b < p.n_seq) {
+            // (starts past the last row or page any call can hold: as that)
+            tok0[b] = (int32_t)min(t0, (int64_t)INT32_MAX);
+            page0[b] = (int32_t)min(f0, (int64_t)INT32_MAX);
+            held[b] = len[i];
+            if (blockIdx.x == 0) {
+                p.len_out[b] = (int32_t)min((int64_t)len[i] + n[i], (int64_t)INT32_MAX);
+                p.tok_start[b] = (int32_t)min(t0, p.max_tok);
+            }
+            t0 += n[i];
+            f0 += pages((int64_t)len[i] + n[i]) - pages(len[i]);
         }
     }
-    if (tid == KS_NT - 1) {
-        total[0] = bt + it;
-        total[1] = bp + ip;
-    }
-    int64_t t0 = bt + it - st, f0 = bp + ip - sp;  // of this thread's first sequence
-    for (int b = b0; b < b1; ++b) {
-        counts(b, len, n, have, fresh);
-        // (starts past the last row or page any call can hold: as that)
-        tok0[b] = (int32_t)min(t0, (int64_t)INT32_MAX);
-        page0[b] = (int32_t)min(f0, (int64_t)INT32_MAX);
-        if (blockIdx.x == 0) {
-            p.len_out[b] = (int32_t)min(len + n, (int64_t)INT32_MAX);
-            p.tok_start[b] = (int32_t)min(t0, p.max_tok);
-        }
-        t0 += n;
-        f0 += fresh;
-    }
-    __syncthreads();
-    const int64_t n_tok = total[0], n_fresh = total[1];
     if (blockIdx.x == 0 && tid == 0) {
         p.tok_start[p.n_seq] = (int32_t)min(n_tok, p.max_tok);
         p.used[0] = n_fresh;
         p.used[1] = n_tok;
     }
+    __syncthreads();
 
     const int64_t step = (int64_t)gridDim.x * KS_NT, first = (int64_t)blockIdx.x * KS_NT + tid;
     auto given = [&](int64_t f) {  // the f-th page taken from the free list
@@ -101,21 +105,13 @@ __global__ __launch_bounds__(KS_NT) void k_kv_slots(KvSlots p) {
         const int32_t id = p.free_pages[f];
         return id >= 0 && id < p.n_pages ? id : -1;
     };
-    // the tables' new entries
-    for (int64_t f = first; f < min(n_fresh, (int64_t)INT32_MAX); f += step) {
-        const int b = ks_upper(page0, p.n_seq, (int32_t)f);
-        counts(b, len, n, have, fresh);
-        const int64_t i = have + f - page0[b];
-        if (i < p.ld_table) p.table[b * p.ld_table + i] = given(f);
-    }
     // the rows; entries of the table that this call writes are not read back
     for (int64_t t = first; t < p.max_tok; t += step) {
         int64_t pos = 0, slot = -1;
         if (t < n_tok) {
             const int b = ks_upper(tok0, p.n_seq, (int32_t)t);
-            counts(b, len, n, have, fresh);
-            pos = len + t - tok0[b];
-            const int64_t i = pos >> p.page_shift;
+            pos = (int64_t)held[b] + t - tok0[b];
+            const int64_t i = pos >> p.page_shift, have = pages(held[b]);
             int32_t id = -1;
             if (i < p.ld_table) id = i < have ? p.table[b * p.ld_table + i] : given(page0[b] + i - have);
             if (id >= 0 && id < p.n_pages) slot = ((int64_t)id << p.page_shift) + (pos & page_up);
@@ -123,13 +119,19 @@ __global__ __launch_bounds__(KS_NT) void k_kv_slots(KvSlots p) {
         p.pos[t] = (int32_t)min(pos, (int64_t)INT32_MAX);
         p.slots[t] = slot;
     }
+    // the tables' new entries
+    for (int64_t f = first; f < min(n_fresh, (int64_t)INT32_MAX); f += step) {
+        const int b = ks_upper(page0, p.n_seq, (int32_t)f);
+        const int64_t i = pages(held[b]) + f - page0[b];
+        if (i < p.ld_table) p.table[b * p.ld_table + i] = given(f);
+    }
 }
 
 hipError_t launch_kv_slots(const KvSlots &p, hipStream_t stream) {
     const int64_t rows = p.max_tok > p.n_seq ? p.max_tok : p.n_seq;
     const int64_t wgs = (rows + KS_NT - 1) / KS_NT;
-    hipLaunchKernelGGL(k_kv_slots, dim3((unsigned)(wgs < 1 ? 1 : wgs > 256 ? 256 : wgs)), dim3(KS_NT), 0,
-                       stream, p);
+    auto kern = p.n_seq <= KS_NT ? k_kv_slots<1> : k_kv_slots<KV_MAX_SEQ / KS_NT>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(wgs < 1 ? 1 : wgs > 256 ? 256 : wgs)), dim3(KS_NT), 0, stream, p);
     return hipGetLastError();
 }
 
@@ -145,46 +147,28 @@ hipError_t launch_kv_slots(const KvSlots &p, hipStream_t stream) {
 constexpr int QK_NT = 256;
 
 template <typename T>
-__device__ __forceinline__ void qk_load(const T *p, float (&v)[4]) {
+struct Qk4 {
     typedef T vec __attribute__((ext_vector_type(4)));
-    const vec t = *reinterpret_cast<const vec *>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (float)t[i];
-}
-template <typename T>
-__device__ __forceinline__ void qk_store(T *p, const float (&v)[4]) {
-    typedef T vec __attribute__((ext_vector_type(4)));
-    vec t;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t[i] = (T)f32_materialize(v[i]);
-    *reinterpret_cast<vec *>(p) = t;
-}
+};
 
-// One workgroup: n_t tokens from t0, of each the heads h0, h0 + dh, ...
-template <typename TX, typename TC, int G>
-__global__ __launch_bounds__(QK_NT) void k_qk_norm_rope(QkNormRope p, int n_t) {
-    extern __shared__ float2 turn[];  // [n_t][pairs] cos, sin
+// One workgroup: a token's heads (those of its part, where tokens are few), QK_NT
+// / G at a time.  VEC: d_rot % 8 == 0, so that a lane's values are two whole
+// pieces of four.  cos and sin are evaluated once a token and pair, into LDS; a
+// lane's weights stay in its registers; the next head's values are loaded
+// before the present one's are used.  Bound by its bytes: 8,191 rows of 32 + 2 x
+// 8 heads of 128, bf16 to bf16, 39.5 us = 5.1 TB/s, past a large copy's rate.
+// Several tokens a workgroup were slower (43 us with 2, 47 with 4), the weights
+// as single floats and an IEEE square root and division 55.
+template <typename TX, typename TC, int G, bool VEC>
+__global__ __launch_bounds__(QK_NT) void k_qk_norm_rope(QkNormRope p) {
+    typedef typename Qk4<TX>::vec xvec;
+    typedef typename Qk4<TC>::vec cvec;
+    __shared__ float2 turn[128];  // cos, sin of the token's pairs
     const int tid = threadIdx.x, half = p.d_rot / 2, d = p.kv.d_head;
-    const int64_t t0 = (int64_t)blockIdx.x * n_t;
-    const int nt = (int)min((int64_t)n_t, p.n_tok - t0);
-    for (int i = tid; i < nt * half; i += QK_NT) {
-        const int t = i / half, j = i - t * half;
-        const double a = (double)p.pos[t0 + t] * p.freq[j];
-        // whole turns off: 2 pi as a head and a tail, so that the product
-        // with up to 2^40 turns keeps 2^-50 of a turn
-        const double n = __builtin_rint(a * 0.15915494309189535);
-        const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, a));
-        float s, c;
-        sincosf((float)r, &s, &c);
-        turn[i] = make_float2(c, s);
-    }
-    __syncthreads();
-
+    const int64_t row = blockIdx.x;
     const int lane = tid % G, n_rot = (p.d_rot + 7) / 8;
-    const int heads = p.n_q_head + 2 * p.kv.n_head;
-    const bool vec = p.d_rot % 8 == 0;  // pairs in whole lanes: 16-byte pieces
-    // this lane's values: element e0 + i (i < 4) and e1 + i - 4, those below
-    // their ends
+    const int nq = p.n_q_head, nk = p.kv.n_head, heads = nq + 2 * nk, step = gridDim.y * (QK_NT / G);
+    // this lane's values: element e0 + i and e1 + i (i < 4), those below their ends
     int e0, e1, end0, end1;
     const bool turns = lane < n_rot;
     if (turns && !p.pairs) {
@@ -196,45 +180,100 @@ __global__ __launch_bounds__(QK_NT) void k_qk_norm_rope(QkNormRope p, int n_t) {
         end0 = end1 = turns ? p.d_rot : d;
     }
     const bool live = e0 < end0;
-    for (int i = blockIdx.y * (QK_NT / G) + tid / G; i < nt * heads; i += gridDim.y * (QK_NT / G)) {
-        const int t = i / heads, h = i - t * heads;
-        const int64_t row = t0 + t;
+    const int a0 = live ? e0 : 0, a1 = live ? e1 : 4;  // (idle lanes read, and drop, a live place)
+
+    struct Head {
+        xvec a, b;
+    };
+    auto load = [&](int h) {
         const TX *src = reinterpret_cast<const TX *>(p.x) + row * p.ld_x + (int64_t)h * d;
-        float a[4] = {0, 0, 0, 0}, b[4] = {0, 0, 0, 0};
-        if (live) {
-            if (vec) {
-                qk_load(src + e0, a);
-                qk_load(src + e1, b);
-            } else {
+        Head v;
+        if constexpr (VEC) {
+            v.a = *reinterpret_cast<const xvec *>(src + a0);
+            v.b = *reinterpret_cast<const xvec *>(src + a1);
+        } else {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (e0 + k < end0) a[k] = (float)src[e0 + k];
-                    if (e1 + k < end1) b[k] = (float)src[e1 + k];
-                }
+            for (int k = 0; k < 4; ++k) {
+                v.a[k] = e0 + k < end0 ? src[e0 + k] : (TX)0.0f;
+                v.b[k] = e1 + k < end1 ? src[e1 + k] : (TX)0.0f;
             }
         }
-        const bool value = h >= p.n_q_head + p.kv.n_head;
-        const float *w = h < p.n_q_head ? p.q_norm : value ? nullptr : p.k_norm;
-        if (w) {  // (uniform over the group of lanes)
+        return v;
+    };
+    int h = blockIdx.y * (QK_NT / G) + tid / G;
+    Head next = {};
+    if (h < heads) next = load(h);
+    // the weights of this lane's values (a kind of head without a norm takes no
+    // factor at all)
+    typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+    float wq[8], wk[8];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const float *w = c ? p.k_norm : p.q_norm;
+        float *to = c ? wk : wq;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) to[k] = 0.0f;
+        if (!w) continue;
+        if constexpr (VEC) {
+            const f4 u = *reinterpret_cast<const f4 *>(w + a0), v = *reinterpret_cast<const f4 *>(w + a1);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                to[k] = u[k];
+                to[4 + k] = v[k];
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                to[k] = e0 + k < end0 ? w[e0 + k] : 0.0f;
+                to[4 + k] = e1 + k < end1 ? w[e1 + k] : 0.0f;
+            }
+        }
+    }
+    const int64_t slot = p.slots[row], page = slot >> p.kv.page_shift;
+    const bool cached = slot >= 0 && page < p.kv.n_pages;
+    const int64_t place = page * p.kv.ld_page + (slot & ((1 << p.kv.page_shift) - 1)) * p.kv.ld_tok;
+    if (tid < half) {
+        const double a = (double)p.pos[row] * p.freq[tid];
+        // whole turns off: 2 pi as a head and a tail, so that the product
+        // with up to 2^40 turns keeps 2^-50 of a turn
+        const double n = __builtin_rint(a * 0.15915494309189535);
+        const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, a));
+        float s, c;
+        sincosf((float)r, &s, &c);
+        turn[tid] = make_float2(c, s);
+    }
+    __syncthreads();
+
+    const float inv_d = 1.0f / (float)d;
+    for (; h < heads; h += step) {
+        const Head cur = next;
+        if (h + step < heads) next = load(h + step);
+        float a[4], b[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            a[k] = live ? (float)cur.a[k] : 0.0f;
+            b[k] = live ? (float)cur.b[k] : 0.0f;
+        }
+        const bool query = h < nq, value = h >= nq + nk;
+        if (query ? p.q_norm != nullptr : !value && p.k_norm != nullptr) {  // (uniform over the group of lanes)
             float ss = 0.0f;
 #pragma unroll
             for (int k = 0; k < 4; ++k) ss = fmaf(b[k], b[k], fmaf(a[k], a[k], ss));
-            const float inv = 1.0f / sqrtf(group_sum<G>(ss) / (float)d + p.eps);
-            if (live) {
+            // v_rsq_f32 (1 ulp) where its argument is a normal number
+            const float var = fmaf(group_sum<G>(ss), inv_d, p.eps);
+            const float inv = var >= 0x1p-126f ? __builtin_amdgcn_rsqf(var) : 1.0f / sqrtf(var);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    a[k] = a[k] * inv * (e0 + k < end0 ? w[e0 + k] : 0.0f);
-                    b[k] = b[k] * inv * (e1 + k < end1 ? w[e1 + k] : 0.0f);
-                }
+            for (int k = 0; k < 4; ++k) {
+                a[k] = a[k] * inv * (query ? wq[k] : wk[k]);
+                b[k] = b[k] * inv * (query ? wq[4 + k] : wk[4 + k]);
             }
         }
         if (!value && turns) {
             // (a lane's last pairs may be past the rotated part: theirs are
             // zeros, turned by some other pair's angle)
-            const float2 *ct = turn + t * half;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float2 cs = ct[min(4 * lane + k, half - 1)];
+                const float2 cs = turn[VEC ? 4 * lane + k : min(4 * lane + k, half - 1)];
                 if (p.pairs) {
                     float &u = k < 2 ? a[2 * k] : b[2 * k - 4], &v = k < 2 ? a[2 * k + 1] : b[2 * k - 3];
                     const float u0 = u;
@@ -247,20 +286,20 @@ __global__ __launch_bounds__(QK_NT) void k_qk_norm_rope(QkNormRope p, int n_t) {
                 }
             }
         }
+        if (!live || (!query && !cached)) continue;
         TC *dst;
-        if (h < p.n_q_head) {
-            dst = reinterpret_cast<TC *>(p.q) + row * p.ld_q + (int64_t)h * d;
-        } else {
-            const int64_t slot = p.slots[row], page = slot >> p.kv.page_shift;
-            if (slot < 0 || page >= p.kv.n_pages) continue;
-            const int hk = value ? h - p.n_q_head - p.kv.n_head : h - p.n_q_head;
-            dst = reinterpret_cast<TC *>(value ? p.kv.v : p.kv.k) + page * p.kv.ld_page + hk * p.kv.ld_head +
-                  (slot & ((1 << p.kv.page_shift) - 1)) * p.kv.ld_tok;
-        }
-        if (!live) continue;
-        if (vec) {
-            qk_store(dst + e0, a);
-            qk_store(dst + e1, b);
+        if (query) dst = reinterpret_cast<TC *>(p.q) + row * p.ld_q + (int64_t)h * d;
+        else if (value) dst = reinterpret_cast<TC *>(p.kv.v) + place + (h - nq - nk) * p.kv.ld_head;
+        else dst = reinterpret_cast<TC *>(p.kv.k) + place + (h - nq) * p.kv.ld_head;
+        if constexpr (VEC) {
+            cvec u, v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                u[k] = (TC)f32_materialize(a[k]);
+                v[k] = (TC)f32_materialize(b[k]);
+            }
+            *reinterpret_cast<cvec *>(dst + e0) = u;
+            *reinterpret_cast<cvec *>(dst + e1) = v;
         } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -273,18 +312,14 @@ __global__ __launch_bounds__(QK_NT) void k_qk_norm_rope(QkNormRope p, int n_t) {
 
 template <typename TX, typename TC, int G>
 static hipError_t run_qk(const QkNormRope &p, hipStream_t stream) {
-    const int heads = p.n_q_head + 2 * p.kv.n_head, per_wg = QK_NT / G;
-    const int half = p.d_rot / 2;
-    int n_t = 1, parts = 1;
-    if (p.n_tok < 1024) {
-        parts = (heads + per_wg - 1) / per_wg;
-    } else {
-        n_t = half ? QK_NT / half : 4;
-        n_t = n_t < 1 ? 1 : n_t > 4 ? 4 : n_t;
-    }
-    const int64_t wgs = (p.n_tok + n_t - 1) / n_t;
-    hipLaunchKernelGGL((k_qk_norm_rope<TX, TC, G>), dim3((unsigned)wgs, (unsigned)parts), dim3(QK_NT),
-                       (unsigned)(sizeof(float2) * n_t * (half ? half : 1)), stream, p, n_t);
+    const int heads = p.n_q_head + 2 * p.kv.n_head, per_wg = QK_NT / G, rounds = (heads + per_wg - 1) / per_wg;
+    // 8 workgroups a CU: fewer tokens than that share a token's heads among
+    // workgroups (64 of 48 heads: 3 parts 3.6 us, 2 parts 4.3; 2,000: one part
+    // 12.8, 2 parts 13.0, 3 parts 14.8)
+    const int64_t most = 2048 / p.n_tok;
+    const int parts = most < 1 ? 1 : most > rounds ? rounds : (int)most;
+    auto kern = p.d_rot % 8 ? k_qk_norm_rope<TX, TC, G, false> : k_qk_norm_rope<TX, TC, G, true>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)p.n_tok, (unsigned)parts), dim3(QK_NT), 0, stream, p);
     return hipGetLastError();
 }
 template <typename TX, typename TC>

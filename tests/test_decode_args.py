@@ -67,7 +67,7 @@ def test_cache_refusals(change, status):
 
 @pytest.mark.parametrize("change,status", [
     (dict(cache=None), INVALID), (dict(x_type=3), INVALID), (dict(style=2), INVALID), (dict(n_tok=-1), INVALID),
-    (dict(n_tok=(1 << 24) + 1), UNSUPPORTED), (dict(n_q_head=0), INVALID), (dict(d_rot=130), INVALID),
+    (dict(n_tok=(1 << 23) + 1), UNSUPPORTED), (dict(n_q_head=0), INVALID), (dict(d_rot=130), INVALID),
     (dict(d_rot=3), INVALID), (dict(d_rot=-2), INVALID), (dict(ld_x=6 * 128 - 8), INVALID),
     (dict(ld_x=6 * 128 + 4), INVALID), (dict(ld_q=2 * 128 - 8), INVALID), (dict(ld_q=2 * 128 + 2), INVALID),
     (dict(x=None), INVALID), (dict(q=None), INVALID), (dict(slots=None), INVALID), (dict(pos=None), INVALID),
