@@ -6,9 +6,9 @@
 // head), far below the matrix pipe's rate: the bytes of the cache bound it.
 //
 // A wave takes tiles of 32 keys, each by itself (no barrier in the loop):
-//  * S^T = K Q^T by v_mfma_f32_16x16x32: K's rows are the A operand, which a
-//    lane loads straight into its registers, 16 bytes of key lane % 16; the
-//    16 query heads (zeros past R) are B, loaded once.
+//  * S^T = K Q^T by v_mfma_f32_16x16x32: K's rows are the A operand, 16 bytes of
+//    key lane % 16 a lane, exchanged between the lanes once loaded; the 16
+//    query heads (zeros past R) are B, loaded once.
 //  * S^T leaves that product with lane l holding head l % 16 and keys 4 g + i
 //    (g = l / 16) -- the layout B wants of P^T in the second product, O^T =
 //    V^T P^T, if its 8 values of k are taken as keys 4 g .. 4 g + 3 of the
@@ -139,41 +139,62 @@ __global__ __launch_bounds__(NW * WAVE) void k_attn_paged(AttnPaged p, int chunk
             q[c] = *reinterpret_cast<const vec *>((const TC *)p.q + s * p.ld_q + (int64_t)(h0 + r) * d + 32 * c + 8 * g);
     }
 
-    // page of key t0 + lane % TILE, -1 unseen
-    auto page_of = [&](int64_t t0) {
-        const int64_t t = t0 + (lane & (TILE - 1));
-        int32_t id = -1;
-        if (t >= kr.first && t < end) {
-            id = row[t >> p.kv.page_shift];
-            if (id >= p.kv.n_pages) id = -1;
-        }
-        return id;
+    // Table entry of key t0 + lane % TILE (the row's last one for keys past it).
+    // Only loaded here: a test of it would wait for all loads before it.
+    auto entry_of = [&](int64_t t0) {
+        return row[min((t0 + (lane & (TILE - 1))) >> p.kv.page_shift, p.ld_table - 1)];
     };
     vec k[KT][DC], v[VT];
     const uint32_t magic = (65536u + nch - 1) / nch;  // f / nch for f < 1,024
     uint32_t seen = 0;
-    auto load = [&](int64_t t0, int32_t id) {
-        seen = (uint32_t)__builtin_amdgcn_ballot_w64(id >= 0);  // (lanes repeat the tile's keys)
-        const bool all = EXACT && seen == ~0u;
+    constexpr uint32_t ALL = ~0u;
+    // Keys: lane / 4 of a 16-key part and a 16-byte piece lane % 4 of 64 (four
+    // lanes a row: with a row a lane, as the MFMA wants them, each would be a
+    // cache access of its own).  Values: piece f of the tile's rows in order.
+    auto load = [&](int64_t t0, int32_t entry) {
+        const int64_t t = t0 + (lane & (TILE - 1));
+        const bool ok = t >= kr.first && t < end && (uint32_t)entry < (uint32_t)p.kv.n_pages;
+        seen = (uint32_t)__builtin_amdgcn_ballot_w64(ok);  // (lanes repeat the tile's keys)
+        const TC *ks[KT], *vs[VT];
+        bool kok[KT], vok[VT];
 #pragma unroll
         for (int j = 0; j < KT; ++j) {
-            const int key = 16 * j + r;
-            const uint32_t pid = (uint32_t)__shfl(id, key);
-            const TC *src = kp + ((uint64_t)pid * ldp + (((uint32_t)t0 + key) & pmask) * (uint64_t)ldt + 8 * g);
-            const bool ok = all || (int32_t)pid >= 0;
-#pragma unroll
-            for (int c = 0; c < DC; ++c) {
-                k[j][c] = vec{};
-                if (ok && (EXACT || 32 * c + 8 * g < d)) k[j][c] = *reinterpret_cast<const vec *>(src + 32 * c);
-            }
+            const int key = 16 * j + (lane >> 2);
+            const uint32_t pid = (uint32_t)__shfl(entry, key);
+            ks[j] = kp + ((uint64_t)pid * ldp + (((uint32_t)t0 + key) & pmask) * (uint64_t)ldt);
+            kok[j] = seen >> key & 1;
         }
 #pragma unroll
         for (int i = 0; i < VT; ++i) {
-            const uint32_t f = i * WAVE + lane, key = EXACT ? f / (DP / 8) : f * magic >> 16;
-            const uint32_t pid = (uint32_t)__shfl(id, (int)(key & (TILE - 1)));
-            const TC *src = vp + ((uint64_t)pid * ldp + (((uint32_t)t0 + key) & pmask) * (uint64_t)ldt + 8 * (f - key * nch));
-            v[i] = vec{};
-            if (all || (key < TILE && (int32_t)pid >= 0)) v[i] = *reinterpret_cast<const vec *>(src);
+            // (past the tile's last piece: that one again, not stored)
+            const uint32_t f = EXACT ? i * WAVE + lane : min(i * WAVE + lane, TILE * nch - 1);
+            const uint32_t key = EXACT ? f / (DP / 8) : f * magic >> 16;
+            const uint32_t pid = (uint32_t)__shfl(entry, (int)key);
+            vs[i] = vp + ((uint64_t)pid * ldp + (((uint32_t)t0 + key) & pmask) * (uint64_t)ldt + 8 * (f - key * nch));
+            vok[i] = seen >> key & 1;
+        }
+        const int e = 8 * (lane & 3);
+        if (seen == ALL) {  // (uniform; no lane masks)
+#pragma unroll
+            for (int j = 0; j < KT; ++j)
+#pragma unroll
+                for (int c = 0; c < DC; ++c)
+                    k[j][c] = *reinterpret_cast<const vec *>(ks[j] + (EXACT || 32 * c + e < d ? 32 * c + e : 0));
+#pragma unroll
+            for (int i = 0; i < VT; ++i) v[i] = *reinterpret_cast<const vec *>(vs[i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < KT; ++j)
+#pragma unroll
+                for (int c = 0; c < DC; ++c) {
+                    k[j][c] = vec{};
+                    if (kok[j]) k[j][c] = *reinterpret_cast<const vec *>(ks[j] + (EXACT || 32 * c + e < d ? 32 * c + e : 0));
+                }
+#pragma unroll
+            for (int i = 0; i < VT; ++i) {
+                v[i] = vec{};
+                if (vok[i]) v[i] = *reinterpret_cast<const vec *>(vs[i]);
+            }
         }
     };
 
@@ -184,10 +205,10 @@ __global__ __launch_bounds__(NW * WAVE) void k_attn_paged(AttnPaged p, int chunk
     const float sc = p.scale * 1.44269504088896341f;  // log2(e)
 
     int64_t t0 = start + wave * TILE;
-    int32_t id_next = -1;
+    int32_t next = -1;
     if (t0 < end) {
-        load(t0, page_of(t0));
-        id_next = page_of(t0 + STEP);
+        load(t0, entry_of(t0));
+        next = entry_of(t0 + STEP);
     }
     for (; t0 < end; t0 += STEP) {
         const uint32_t mask = seen;
@@ -201,11 +222,19 @@ __global__ __launch_bounds__(NW * WAVE) void k_attn_paged(AttnPaged p, int chunk
         for (int j = 0; j < KT; ++j) {
             st[j] = v4f{0, 0, 0, 0};
 #pragma unroll
-            for (int c = 0; c < DC; ++c) st[j] = Pa<TC>::mfma(k[j][c], q[c], st[j]);
+            for (int c = 0; c < DC; ++c) {
+                v4i kk = __builtin_bit_cast(v4i, k[j][c]);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    kk[w] = __shfl(kk[w], 4 * r + g);
+                    if (!EXACT && 32 * c + 8 * g >= d) kk[w] = 0;  // (read from the row's start)
+                }
+                st[j] = Pa<TC>::mfma(__builtin_bit_cast(vec, kk), q[c], st[j]);
+            }
         }
         if (t0 + STEP < end) {  // (k and v are free)
-            load(t0 + STEP, id_next);
-            id_next = page_of(t0 + 2 * STEP);
+            load(t0 + STEP, next);
+            next = entry_of(t0 + 2 * STEP);
         }
         // the softmax of head r over keys 4 g + i, 16 + 4 g + i
         float mt = -INFINITY;
@@ -214,7 +243,7 @@ __global__ __launch_bounds__(NW * WAVE) void k_attn_paged(AttnPaged p, int chunk
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 st[j][i] = st[j][i] * sc;
-                if (mask != ~0u && !(mask >> (16 * j + 4 * g + i) & 1)) st[j][i] = -INFINITY;
+                if (mask != ALL && !(mask >> (16 * j + 4 * g + i) & 1)) st[j][i] = -INFINITY;
                 mt = fmaxf(mt, st[j][i]);
             }
         mt = fmaxf(mt, __shfl_xor(mt, 16));

@@ -109,10 +109,13 @@ hipError_t launch_expand_q4(const Q4View &w, const WeightView &dst, hipStream_t 
 // multiplied on the VALU and loaded as each lane needs them it was 11, and those
 // loads' lanes (64 bytes a clock and CU) bound it: 1 x 1152 x 256000 53 us
 // against 34.6 (4.8 TB/s, a copy's rate), 7 x 4096 x 14336 16 against 9.4.  One
-// group of 16 rows is bound by the weight's bytes, several by their VALU and
-// matrix operations (some 7 us a group at 4096 x 14336).  Loads of the next
-// tiles ahead of a tile's products changed nothing: the waves of the other
-// workgroups on a CU cover each other's.
+// group of 16 rows is bound by the weight's bytes.  Several take some 7 us each
+// at 4096 x 14336, not for their operations: 32 rows a wave on the 32 x 32 MFMAs,
+// half the instructions for the same reads of the activation, took as long (64
+// rows 31 us, with twice the columns a wave 24; 32 x 4096 x 4096 10.9 against
+// 6.6, the waves being half as many).  Loads of
+// the next tiles ahead of a tile's products changed nothing either: the waves of
+// the other workgroups on a CU cover each other's.
 //
 // A wave takes 16 rows and NT groups of 16 columns over a range of K, wk waves
 // of a workgroup share their columns' K and join in LDS in order.  Further rows
@@ -142,8 +145,9 @@ __global__ __launch_bounds__(Q4_NT) void k_mul_mat_q4(const uint8_t *__restrict_
     const int tiles_n = (G.N + 15) / 16, per = (G.tiles_k + G.wk - 1) >> G.lwk;
     const int k0 = wk * per, k1 = min(k0 + per, G.tiles_k);
 
-    const int64_t m = min(m0 + r, G.M - 1);  // (rows past M: computed, not stored)
-    const int8_t *xr = xq + m * G.KB * QK + 16 * (g & 1);
+    // the activation as it is loaded: row lane / 4, piece lane % 4 of 64 bytes
+    const int64_t m = min(m0 + (lane >> 2), G.M - 1);  // (rows past M: computed, not stored)
+    const int8_t *xr = xq + m * G.KB * QK + 16 * (lane & 1);
     const uint32_t *dr = xds + m * G.KB;
     const uint8_t *wp[NT];
     const uint16_t *dp[NT];
@@ -166,10 +170,16 @@ __global__ __launch_bounds__(Q4_NT) void k_mul_mat_q4(const uint8_t *__restrict_
             d[b] = dp[b][(int64_t)t * 64];
         }
         // blocks past K: the last one again, against zero nibbles and scales
-        const int kb = 4 * t + (g >> 1), last = G.KB - 1;
+        const int kb = 4 * t + ((lane & 3) >> 1), last = G.KB - 1;
         x[0] = *reinterpret_cast<const v4u *>(xr + min(kb, last) * QK);
         x[1] = *reinterpret_cast<const v4u *>(xr + min(kb + 2, last) * QK);
-        const v2i dx = {(int)(dr[min(4 * t + g, last)] & 0xffffu), 0};
+        uint32_t dx0 = dr[min(4 * t + (lane & 3), last)] & 0xffffu;
+        // row r, piece g to lane 16 g + r
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[h][c] = __shfl(x[h][c], 4 * r + g);
+        const v2i dx = {(int)__shfl(dx0, 4 * r + g), 0};
         // x[h]: 16 bytes of block 2 h + (g >> 1) -> xb[j]: 8 of block j
         v2i xb[4];
 #pragma unroll
