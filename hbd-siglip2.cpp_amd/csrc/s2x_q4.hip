@@ -105,17 +105,18 @@ hipError_t launch_expand_q4(const Q4View &w, const WeightView &dst, hipStream_t 
 //    block g's d_w and d_x in the first of its four slots of k, and A is zeroed
 //    but for the block wanted: one exact product per output.
 // So acc = fmaf((float)I, d_w d_x, acc) is 8 VALU operations on 4 outputs, and a
-// tile's 1,152 bytes of weight come with 5 load instructions.  With the scales
-// multiplied on the VALU and loaded as each lane needs them it was 11, and those
-// loads' lanes (64 bytes a clock and CU) bound it: 1 x 1152 x 256000 53 us
-// against 34.6 (4.8 TB/s, a copy's rate), 7 x 4096 x 14336 16 against 9.4.  One
-// group of 16 rows is bound by the weight's bytes.  Several take some 7 us each
-// at 4096 x 14336, not for their operations: 32 rows a wave on the 32 x 32 MFMAs,
-// half the instructions for the same reads of the activation, took as long (64
-// rows 31 us, with twice the columns a wave 24; 32 x 4096 x 4096 10.9 against
-// 6.6, the waves being half as many).  Loads of
-// the next tiles ahead of a tile's products changed nothing either: the waves of
-// the other workgroups on a CU cover each other's.
+// tile's 1,152 bytes of weight come with 5 load instructions.  What bounds it:
+//  * one group of 16 rows: the weight's bytes, once the loads' lanes (64 bytes a
+//    clock and CU) are few.  With the scales multiplied on the VALU and loaded
+//    as each lane needs them there were 11 loads a tile, and 1 x 1152 x 256000
+//    took 53 us against 34.5 (4.8 TB/s, a copy's rate).
+//  * more rows: the L1.  Lanes next to each other that load from different rows
+//    are a cache access each (counted: 233 a wave and tile, the L1 busy 70 % of
+//    the time); QUAD has four lanes load 64 bytes of a row and exchanges them
+//    through LDS: 64 x 4096 x 14336 31 -> 25 us.  (32 rows a wave on the 32 x 32
+//    MFMAs, half the instructions, took as long as the form without QUAD.)
+//  * loads of the next tiles ahead of a tile's products: no faster, the waves of
+//    the other workgroups on a CU cover each other's.
 //
 // A wave takes 16 rows and NT groups of 16 columns over a range of K, wk waves
 // of a workgroup share their columns' K and join in LDS in order.  Further rows
@@ -129,7 +130,8 @@ struct Q4Grid {
     int tiles_k, KB, M, N, row_groups;
 };
 
-template <int NT>
+// QUAD: the activation loaded four lanes a row.
+template <int NT, bool QUAD>
 __global__ __launch_bounds__(Q4_NT) void k_mul_mat_q4(const uint8_t *__restrict__ wq, const uint16_t *__restrict__ wd,
                                                       Q4Grid G, const int8_t *__restrict__ xq,
                                                       const uint32_t *__restrict__ xds, float *y, int64_t ldy,
@@ -145,9 +147,10 @@ __global__ __launch_bounds__(Q4_NT) void k_mul_mat_q4(const uint8_t *__restrict_
     const int tiles_n = (G.N + 15) / 16, per = (G.tiles_k + G.wk - 1) >> G.lwk;
     const int k0 = wk * per, k1 = min(k0 + per, G.tiles_k);
 
-    // the activation as it is loaded: row lane / 4, piece lane % 4 of 64 bytes
-    const int64_t m = min(m0 + (lane >> 2), G.M - 1);  // (rows past M: computed, not stored)
-    const int8_t *xr = xq + m * G.KB * QK + 16 * (lane & 1);
+    // the activation as it is loaded: row lr, piece lg of 64 bytes
+    const int lr = QUAD ? lane >> 2 : r, lg = QUAD ? lane & 3 : g;
+    const int64_t m = min(m0 + lr, G.M - 1);  // (rows past M: computed, not stored)
+    const int8_t *xr = xq + m * G.KB * QK + 16 * (lg & 1);
     const uint32_t *dr = xds + m * G.KB;
     const uint8_t *wp[NT];
     const uint16_t *dp[NT];
@@ -170,16 +173,18 @@ __global__ __launch_bounds__(Q4_NT) void k_mul_mat_q4(const uint8_t *__restrict_
             d[b] = dp[b][(int64_t)t * 64];
         }
         // blocks past K: the last one again, against zero nibbles and scales
-        const int kb = 4 * t + ((lane & 3) >> 1), last = G.KB - 1;
+        const int kb = 4 * t + (lg >> 1), last = G.KB - 1;
         x[0] = *reinterpret_cast<const v4u *>(xr + min(kb, last) * QK);
         x[1] = *reinterpret_cast<const v4u *>(xr + min(kb + 2, last) * QK);
-        uint32_t dx0 = dr[min(4 * t + (lane & 3), last)] & 0xffffu;
-        // row r, piece g to lane 16 g + r
+        uint32_t dx0 = dr[min(4 * t + lg, last)] & 0xffffu;
+        if constexpr (QUAD) {  // row r, piece g to lane 16 g + r
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) x[h][c] = __shfl(x[h][c], 4 * r + g);
-        const v2i dx = {(int)__shfl(dx0, 4 * r + g), 0};
+                for (int c = 0; c < 4; ++c) x[h][c] = __shfl(x[h][c], 4 * r + g);
+            dx0 = __shfl(dx0, 4 * r + g);
+        }
+        const v2i dx = {(int)dx0, 0};
         // x[h]: 16 bytes of block 2 h + (g >> 1) -> xb[j]: 8 of block j
         v2i xb[4];
 #pragma unroll
@@ -231,15 +236,18 @@ hipError_t launch_mul_mat_q4(const Q4View &w, const int8_t *xq, const uint32_t *
     int wk = 1, lwk = 0;
     for (; wk < Q4_NW && wk < w.tiles_k() && w.tiles_n() * wk < 3584; ++lwk) wk *= 2;
     const int64_t rg = (M + 15) / 16;
-    // two column groups a wave, one read of the rows for both, where that leaves
-    // a workgroup for half of the CUs: 16 x 4096 x 14336 10.2 us (one group
-    // 14.9), 64 x 4320 x 1152 5.9 (7.3); below, 16 x 4096 x 4096 6.2 (5.7),
-    // 43 x 4320 x 1152 5.8 (4.8)
-    const bool two = w.tiles_n() * rg * wk / Q4_NW > 256;
+    // The rows four lanes a row and exchanged, from 5 rows on: 16 x 4096 x 14336
+    // 9.7 us (a lane a row 15.1), 8 x 4096 x 4096 4.8 (4.9), 4 x 11040 x 1152 7.7
+    // (7.3).  Two column groups a wave where that leaves a workgroup for half of
+    // the CUs, one read of the rows for both: 1 x 1152 x 256000 34.5 us (one group
+    // 36.8), 4 x 4096 x 4096 5.1 (4.0); with the exchange only past two groups of
+    // rows: 64 x 4096 x 4096 8.7 (9.5), 16 x 4096 x 14336 11.5 (9.7).
+    const bool quad = M > 4, two = w.tiles_n() * rg * wk / Q4_NW > 256 && (!quad || M > 32);
     const int nt = two ? 2 : 1;
     const int64_t per_wg = (int64_t)(Q4_NW / wk) * nt;
     const Q4Grid G{wk, lwk, (int)w.tiles_k(), (int)(w.K / QK), (int)M, (int)w.N, (int)rg};
-    auto kern = two ? k_mul_mat_q4<2> : k_mul_mat_q4<1>;
+    auto kern = two ? (quad ? k_mul_mat_q4<2, true> : k_mul_mat_q4<2, false>)
+                    : (quad ? k_mul_mat_q4<1, true> : k_mul_mat_q4<1, false>);
     hipLaunchKernelGGL(kern, dim3((unsigned)((w.tiles_n() + per_wg - 1) / per_wg * rg)), dim3(Q4_NT), 0, stream, w.qs,
                        w.d, G, xq, xds, y, ldy, epi);
     return hipGetLastError();

@@ -450,7 +450,7 @@ def q4_terms(q, dw, qx, dx):
     (1, 32, 1, "host"), (1, 64, 17, "device"), (1, 1152, 3456, "in"), (2, 96, 15, "host"), (3, 4320, 100, "host"),
     (7, 160, 33, "in"), (8, 1152, 64, "host"), (15, 288, 48, "host"), (16, 1024, 130, "device"),
     (17, 416, 19, "host"), (31, 2048, 16, "host"), (33, 4320, 65, "in"), (48, 992, 31, "host"),
-    (64, 1152, 129, "host"), (100, 4096, 70, "host"), (160, 320, 270, "device"), (1, 8192, 40, "host"), (64, 32, 3, "host"), (2, 128, 70000, "device"), (5, 11040, 21, "host")])
+    (64, 1152, 129, "host"), (100, 4096, 70, "host"), (208, 320, 270, "device"), (4, 512, 5000, "device"), (50, 256, 9000, "device"), (1, 8192, 40, "host"), (64, 32, 3, "host"), (2, 128, 70000, "device"), (5, 11040, 21, "host")])
 def test_q4_few_rows(m, k, n, how):
     rng = np.random.default_rng(m * 31 + k + n)
     say(f"q4: {m} x {k} x {n} ({how})")
@@ -485,8 +485,8 @@ def test_q4_few_rows(m, k, n, how):
     within(g, want, (16 + 8 * np.abs(v) * (1 + 0.05 * v * v)) * U * np.abs(want) + 1e-35, "gelu")
 
 
-@pytest.mark.parametrize("m,k,n", [(161, 1152, 200), (200, 4320, 96), (300, 64, 1000), (170, 32, 1),
-                                   (161, 416, 129)])
+@pytest.mark.parametrize("m,k,n", [(209, 1152, 200), (210, 4320, 96), (300, 64, 1000), (220, 32, 1),
+                                   (209, 416, 129)])
 def test_q4_many_rows(m, k, n):
     """Past the few-rows limit: the bits of the Q8_0 product of the same
     weight."""
