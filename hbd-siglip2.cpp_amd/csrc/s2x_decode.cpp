@@ -18,8 +18,10 @@ struct s2x_weight_q4 {
 
 namespace s2x {
 
+// (the last bound keeps the repack's grid within 2^32 threads: 38 GB of weight)
 static bool q4_shape_ok(int64_t K, int64_t N) {
-    return K > 0 && N > 0 && K % QK_ == 0 && K <= (1 << 20) && N <= (1 << 24);
+    return K > 0 && N > 0 && K % QK_ == 0 && K <= (1 << 20) && N <= (1 << 24) &&
+           round_up_i(K, 128) * round_up_i(N, 128) <= (int64_t)1 << 36;
 }
 // planes: tiles of 1,024 bytes, then 128 bytes of scales a tile
 static Q4View q4_view(void *base, int64_t K, int64_t N) {

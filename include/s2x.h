@@ -364,10 +364,10 @@ typedef enum { S2X_TYPE_F32 = 0, S2X_TYPE_F16 = 1, S2X_TYPE_BF16 = 2 } s2x_type;
  * (fp16 d, then 16 bytes of nibbles: value i of the block in the low half of
  * byte i, value 16 + i in its high half; a nibble v stands for (v - 8) * d).
  * The repack is lossless; it reorders the nibbles for the int8 MFMA.
- * K % 32 == 0.  create: new device memory of s2x_weight_q4_0_bytes(), raw in
+ * K % 32 == 0, K <= 2^20, N <= 2^24, K * N <= 2^36.  create: new device memory of s2x_weight_q4_0_bytes(), raw in
  * host or device memory, synchronises `stream`.  create_in: into `dev_buf`
- * (256-byte aligned), raw on the device, asynchronous, no allocation on the
- * device. */
+ * (256-byte aligned), raw on the device and unchanged until the call's work on
+ * `stream` has finished, asynchronous, no allocation on the device. */
 typedef struct s2x_weight_q4 s2x_weight_q4;
 size_t s2x_weight_q4_0_bytes(int64_t K, int64_t N);
 int s2x_weight_q4_0_create(const void *raw, int raw_is_host, int64_t K, int64_t N, void *stream,
@@ -389,7 +389,8 @@ int64_t s2x_weight_q4_0_n(const s2x_weight_q4 *w);
  * s2x_mul_mat_q8_0_q8_1's kernel, with its bits.  The limit is about where the
  * two cost the same (4096 x 14336: 160 rows 49 against 61 us, 208 rows 64
  * either way).  workspace: s2x_mul_mat_q4_0_workspace_size() bytes, 256-byte aligned;
- * 0 bytes, and NULL is taken, up to S2X_Q4_FEW_ROWS. */
+ * the call's own until its work has finished; 0 bytes, and NULL is taken, up
+ * to S2X_Q4_FEW_ROWS. */
 #define S2X_Q4_FEW_ROWS 208
 size_t s2x_mul_mat_q4_0_workspace_size(int64_t K, int64_t N, int64_t M);
 int s2x_mul_mat_q4_0_q8_1(const s2x_weight_q4 *w, const void *qs, const void *ds, int64_t M,

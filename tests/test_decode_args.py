@@ -123,7 +123,8 @@ def test_q4_refusals():
     out = ctypes.c_void_p()
     o = ctypes.byref(out)
     assert lib.s2x_weight_q4_0_bytes(33, 4) == 0 and lib.s2x_weight_q4_0_bytes(32, 0) == 0
-    assert lib.s2x_weight_q4_0_bytes(1 << 21, 4) == 0
+    assert lib.s2x_weight_q4_0_bytes((1 << 20) + 32, 4) == 0 and lib.s2x_weight_q4_0_bytes(32, (1 << 24) + 1) == 0
+    assert lib.s2x_weight_q4_0_bytes(1 << 20, 1 << 17) == 0 and lib.s2x_weight_q4_0_bytes(1 << 19, 1 << 17) > 0
     assert lib.s2x_weight_q4_0_bytes(4096, 4096) == 4096 * 4096 // 32 * 18
     assert lib.s2x_weight_q4_0_create(P, 0, 100, 4, None, o) == INVALID
     assert lib.s2x_weight_q4_0_create(None, 1, 128, 4, None, o) == INVALID

@@ -285,7 +285,13 @@ def check_attn(q, cache, table, lens, max_len, scale, window, out_kind, **kw):
     ([100, 50], 2, 1, 8, "f16", "f32", 16, "head"),
     ([61, 50], 2, 1, 40, "bf16", "f32", 2, "token"),
     ([5000, 3, 2600], 16, 2, 128, "f16", "f16", 16, "head"),
-    ([2000], 4, 4, 128, "bf16", "f32", 2048, "token")])
+    ([2000], 4, 4, 128, "bf16", "f32", 2048, "token"),
+    ([300, 31], 32, 2, 256, "f16", "f16", 16, "head"),           # the most LDS a workgroup takes
+    ([1200], 16, 1, 248, "bf16", "f32", 32, "token"),
+    ([90, 250], 20, 1, 208, "f16", "f32", 16, "head"),
+    ([1021] * 16, 8, 8, 64, "f16", "f16", 16, "head"),           # one launch past 320 tokens
+    ([7000], 1, 1, 72, "f16", "f32", 16, "token"),               # more than 32 chunks
+    (list(range(0, 740, 20)), 2, 1, 64, "bf16", "bf16", 16, "head")])
 def test_attn_paged(lens, hq, hkv, d, kind, out_kind, page, by):
     say(f"attn: lens {lens} {hq}/{hkv} x {d} {kind}->{out_kind} page {page} {by}")
     rng = np.random.default_rng(sum(lens) + d)
@@ -336,6 +342,23 @@ def test_attn_score_range():
     ref = attn_ref(q.float().numpy()[[0, 2]], cache, table[[0, 2]], [600, 600], 600, 0.05, 0)
     within(got[[0, 2]], ref[0], 1e-3 * ref[1], "neighbours of a NaN")
     assert np.isnan(got[1]).any(axis=1).all()  # its own rows say so
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_attn_small_values(kind):
+    """Values below the types' normal range count: keys and values around
+    2^-20 (subnormal in f16), scores made of them."""
+    rng = np.random.default_rng(6)
+    lens = [150, 33]
+    q, cache, table = attn_inputs(rng, lens, 4, 2, 64, kind, 16, "head")
+    cache.k.mul_(2.0 ** -19)
+    cache.v.mul_(2.0 ** -20)
+    got, _ = run_attn(q, cache, table, lens, 150, 2.0 ** 17, 0, "f32")
+    ref, size, _, top, seen = attn_ref(q.float().numpy(), cache, table, lens, 150, 2.0 ** 17, 0)
+    # as in check_attn, without its allowance for the smallest output step
+    prob = {"f16": 2.0 ** -21, "bf16": 2.0 ** -22}[kind]
+    rel = 2 * (64 + 6) * U * top + 4 * U + prob + 2 * (seen[:, None] + 8) * U
+    within(got, ref, rel[:, :, None] * size + U * np.abs(ref), kind)
 
 
 def test_attn_offsets_past_32_bits():
@@ -528,6 +551,57 @@ def test_q4_extremes():
     s2x.call("s2x_mul_mat_q4_0_q8_1", w.h, ptr(qd), ptr(dd), 2, ptr(yr), n, ctypes.byref(e), None, 0, stream())
     assert_same(host(yr), y + np.arange(2 * n, dtype=np.float32).reshape(2, n), "in place")
     s2x.call("s2x_mul_mat_q4_0_q8_1", w.h, None, None, 0, ptr(yr), n, None, None, 0, stream())
+
+
+def test_q4_scales_out_of_the_normal_range():
+    """Subnormal f16 scales on both sides count; a row whose scales are NaN or
+    infinite, a column whose scale is, leave the others alone."""
+    rng = np.random.default_rng(12)
+    m, k, n = 9, 256, 40
+    q, dw = q4_weight(rng, n, k)
+    qx, ds, dx = q8_1_planes(rng, m, k)
+    dw[:] = (rng.integers(1, 900, dw.shape) * 2.0 ** -24).astype(np.float16)
+    dx[:4] = (rng.integers(1, 900, dx[:4].shape) * 2.0 ** -24).astype(np.float16)
+    ref, size = q4_terms(q, dw, qx, dx)
+    word = lambda d: dev(np.ascontiguousarray(d).view(np.uint16).astype(np.uint32))
+    qd = dev(qx)
+    w = Q4(q, dw)
+    y = run_q4(w, qd, word(dx), m)
+    within(y, ref, (k // 32 + 20) * U * size, "subnormal scales")
+    bad = dx.copy()
+    bad[2, 1], bad[5, 0] = np.nan, np.inf
+    keep = [0, 1, 3, 4, 6, 7, 8]
+    z = run_q4(w, qd, word(bad), m)
+    assert_same(z[keep], y[keep], "rows beside NaN and inf")
+    assert np.isnan(z[2]).all() and not np.isfinite(z[5]).any()
+    dw2 = dw.copy()
+    dw2[7, 3] = np.inf
+    z = run_q4(Q4(q, dw2), qd, word(dx), m)
+    cols = [c for c in range(n) if c != 7]
+    assert_same(z[:, cols], y[:, cols], "columns beside inf")
+    assert not np.isfinite(z[:, 7]).any()
+
+
+def test_q4_two_streams_at_once():
+    """Calls on two streams, one weight, buffers of their own; past the
+    few-rows limit each with its workspace."""
+    rng = np.random.default_rng(13)
+    k, n = 1024, 520
+    w = Q4(*q4_weight(rng, n, k))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for m in (3, 20, 230):
+        sets = []
+        for i in range(6):
+            qx, ds, _ = q8_1_planes(rng, m, k)
+            size = s2x.lib.s2x_mul_mat_q4_0_workspace_size(k, n, m)
+            sets.append((dev(qx), dev(ds), empty((m, n), torch.float32), empty((max(size, 1),), torch.uint8), size))
+        torch.cuda.synchronize()
+        for i, (qx, ds, y, ws, size) in enumerate(sets):
+            s2x.call("s2x_mul_mat_q4_0_q8_1", w.h, ptr(qx), ptr(ds), m, ptr(y), n, None, ptr(ws), size,
+                     ctypes.c_void_p(streams[i % 2].cuda_stream))
+        torch.cuda.synchronize()
+        for qx, ds, y, _, _ in sets:
+            assert_same(host(y), run_q4(w, qx, ds, m), f"m={m}")
 
 
 # ---------------------------------------------------------------------------
