@@ -20,8 +20,10 @@
 //    the registers, and the page ids of the one after.
 // A workgroup's waves join in LDS; a sequence's chunks, where there is more than
 // one, in k_attn_join.  Measured (both launches): one sequence of 131,071
-// tokens, 32 / 8 heads of 128, 103 us = 5.2 TB/s of keys and values, what a
-// large copy reaches; 60 sequences up to 8,000 in pages of 16, 133 us = 4.2.
+// tokens, 32 / 8 heads of 128, 101 us = 5.3 TB/s of keys and values, what a
+// large copy reaches; 60 sequences up to 8,000 in pages of 16, 120 us = 4.6.
+#include <type_traits>
+
 #include "s2x_decode.h"
 #include "s2x_device.h"
 
@@ -33,7 +35,6 @@ constexpr int PJ_NT = 256;    // threads of the join
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef short v8s __attribute__((ext_vector_type(8)));
-typedef __bf16 v4bf __attribute__((ext_vector_type(4)));
 
 template <typename T> struct Pa;
 // Terms of the cache's type that a probability enters the second product as:
@@ -395,21 +396,23 @@ __global__ __launch_bounds__(PJ_NT) void k_attn_join(AttnPaged p, int chunk, int
     pa_write<TC>(p, s, h, d, e, y, top, L);
 }
 
-// Chunk length, number of chunks and waves of a workgroup.  A CU takes some 31
-// bytes a ns, whatever its waves have in flight (one step of 128 keys of 128
-// halves 2.1 us), so a launch wants all CUs at work to the end; a second
-// launch, the join, is 3 us and its gap.
+// Chunk length, number of chunks and waves of a workgroup.  A step of a workgroup
+// (128 keys of 128 halves and their values) takes 1.4 us however few are at
+// work, some 45 bytes a ns and CU, so a launch wants all CUs at work to the end;
+// a second launch, the join, is 3 us and its gap.
 //  * no split, 8 waves a workgroup, for what a split does not speed up: up to
-//    320 tokens (3 sequences up to 300, 16 heads of 72: 7.3 us, in two chunks
-//    8.4) and, from 128 workgroups on, up to 1,024 (32 x 1,000, 8 key heads of
-//    128: 16.0 us, in chunks of 256 18.9).
+//    320 tokens (3 sequences up to 300, 16 heads of 72: 7.5 us, in chunks of 128
+//    8.1; one of 500: 9.0 against 8.1) and, from 128 workgroups on, up to 1,024
+//    (8 key heads of 128: 32 up to 500 10.2 us, in chunks of 128 12.3, 64 up to
+//    700 16.3 against 20.4, 32 up to 1,000 16.1 against 15.6; 32 up to 2,000
+//    26.9 against 23.4).
 //  * one sequence: two workgroups a CU (131,071 tokens, 8 key heads: chunks of
-//    2,048 103 us, of 1,024 105, of 512 108, of 4,096 110; 2,000 tokens: of
-//    128 8.9 us, of 256 10.6), a batch, whose lengths differ: up to 16 a CU,
-//    chunks of 256 to 1,024 (60 up to 8,000: 1,024 133 us, 2,048 155; 16 up
-//    to 8,000: 256 36.7, 512 40, 1,024 43; 8 up to 4,000: 256 17.5, 128 20).
-//  * more waves a workgroup, loads of the next tile before the first product:
-//    no faster; the bytes a CU can take bound it.
+//    2,048 101.5 us, of 1,024 104, of 512 108; 2,000 tokens: of 128 8.7 us, of
+//    256 10.2); a batch, whose lengths differ: 6 a CU, chunks of 256 to 768 (60
+//    up to 8,000: 768 125 us, 1,024 124, 2,048 141, 384 138; 16 up to 8,000:
+//    768 34.2, 512 36.5, 1,024 37.9; 8 up to 4,000: 256 17.3, 512 19.5, 128 21).
+//  * more waves a workgroup in a split, loads of the next tile before the first
+//    product: no faster.
 struct PaPlan {
     int chunk, n_split, nw;
 };
@@ -418,8 +421,8 @@ static PaPlan pa_plan(int64_t n_seq, int64_t max_len, int64_t n_q_head, int64_t 
     const int64_t span = max_len + PA_ALIGN;  // (the first tile may begin before a window)
     if (max_len <= 320 || (units >= 128 && max_len <= 1024))
         return PaPlan{(int)((span + 127) / 128 * 128), 1, 8};
-    const int64_t wgs = 512 * (n_seq < 8 ? n_seq : 8);
-    const int64_t least = span * units < 65536 ? 128 : 256, most = n_seq == 1 ? 2048 : 1024;
+    const int64_t wgs = 512 * (n_seq < 3 ? n_seq : 3);
+    const int64_t least = span * units < 65536 ? 128 : 256, most = n_seq == 1 ? 2048 : 768;
     int64_t c = span * units / wgs;
     c = c < least ? least : c > most ? most : c;
     if (c < span * units >> 22) c = span * units >> 22;  // (a grid of at most 2^23)
@@ -437,8 +440,9 @@ static hipError_t run_paged_w(const AttnPaged &p, const PaPlan &P, hipStream_t s
     const int group = p.n_q_head / p.kv.n_head, R = group < 16 ? group : 16;
     const int64_t wgs = (int64_t)P.n_split * p.kv.n_head * ((group + 15) / 16) * p.n_seq;
     const int v = NW * KT * 16 * p.kv.d_head * 2 + 64, o = NW * R * (DC * 32 + 4) * 4, lds = v > o ? v : o;
-    constexpr bool BF = sizeof(TC) == 2 && Pa<TC>::up == 1.0f;
-    auto kern = BF && p.out_f32 ? k_attn_paged<TC, DC, EXACT, BF ? 3 : 2, KT, NW> : k_attn_paged<TC, DC, EXACT, 2, KT, NW>;
+    // (a bf16 cache's third term only where the output would show it)
+    constexpr int MOST = std::is_same<TC, __bf16>::value ? 3 : 2;
+    auto kern = p.out_f32 ? k_attn_paged<TC, DC, EXACT, MOST, KT, NW> : k_attn_paged<TC, DC, EXACT, 2, KT, NW>;
     hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(NW * WAVE), lds, stream, p, P.chunk, P.n_split);
     return hipGetLastError();
 }
