@@ -110,18 +110,18 @@ hipError_t launch_expand_q4(const Q4View &w, const WeightView &dst, hipStream_t 
 //    clock and CU) are few.  With the scales multiplied on the VALU and loaded
 //    as each lane needs them there were 11 loads a tile, and 1 x 1152 x 256000
 //    took 53 us against 34.5 (4.8 TB/s, a copy's rate).
-//  * more rows: the L1.  Lanes next to each other that load from different rows
-//    are a cache access each (counted: 233 a wave and tile, the L1 busy 70 % of
-//    the time); QUAD has four lanes load 64 bytes of a row and exchanges them
-//    through LDS: 64 x 4096 x 14336 31 -> 25 us.  (32 rows a wave on the 32 x 32
-//    MFMAs, half the instructions, took as long as the form without QUAD.)
+//  * more rows: the L1, then the operations.  Lanes next to each other that load
+//    from different rows are a cache access each (counted: 233 a wave and tile,
+//    the L1 busy 70 % of the time); QUAD has four lanes load 64 bytes of a row
+//    and exchanges them through LDS: 64 x 4096 x 14336 31 -> 24.6 us, and with 32
+//    rows a wave (below) 19.6.
 //  * loads of the next tiles ahead of a tile's products: no faster, the waves of
 //    the other workgroups on a CU cover each other's.
 //
 // A wave takes 16 rows and NT groups of 16 columns over a range of K, wk waves
 // of a workgroup share their columns' K and join in LDS in order.  Further rows
 // are further workgroups, next to each other on one XCD, so that the weight
-// comes out of its L2 again (more rows a wave: slower at every size up to 64).
+// comes out of its L2 again.
 // ---------------------------------------------------------------------------
 constexpr int Q4_NW = 8, Q4_NT = Q4_NW * WAVE;
 
@@ -129,6 +129,26 @@ struct Q4Grid {
     int wk, lwk;  // waves along K (a power of two) and its logarithm
     int tiles_k, KB, M, N, row_groups;
 };
+
+// The waves' sums [wave][ROWS][P] joined in the order of K, the epilogue, and out.
+template <int COLS, int P, int ROWS>
+__device__ __forceinline__ void q4_join(const float *part, const Q4Grid &G, int col, int m0, int groups, float *y,
+                                        int64_t ldy, const EpiParams &epi) {
+    const int cols = COLS * groups, rows = min(ROWS, G.M - m0);
+    for (int i = threadIdx.x; i < rows * cols; i += Q4_NT) {
+        const int row = i / cols, c = i - row * cols, grp = c / COLS;
+        const int64_t mr = m0 + row, n = (int64_t)col * cols + c;
+        if (n >= G.N) continue;
+        const float *p = part + ((grp << G.lwk) * ROWS + row) * P + c % COLS;
+        float v = p[0];
+        for (int k = 1; k < G.wk; ++k) v = v + p[k * ROWS * P];
+        if (epi.kind != EPI_NONE) v = v + epi.bias[n];
+        if (epi.kind == EPI_BIAS_GELU) v = gelu_tanh(v);
+        if (epi.kind == EPI_BIAS_RESID)
+            v = v + epi.resid[(epi.resid_rows > 0 ? mr % epi.resid_rows : mr) * epi.ld_resid + n];
+        y[mr * ldy + n] = v;
+    }
+}
 
 // QUAD: the activation loaded four lanes a row.
 template <int NT, bool QUAD>
@@ -213,19 +233,127 @@ __global__ __launch_bounds__(Q4_NT) void k_mul_mat_q4(const uint8_t *__restrict_
 #pragma unroll
     for (int b = 0; b < NT; ++b) *reinterpret_cast<v4f *>(&part[wave][r][16 * b + 4 * g]) = acc[b] * 0.0625f;
     __syncthreads();
-    const int cols = COLS * groups, rows = min(16, G.M - m0);
-    for (int i = tid; i < rows * cols; i += Q4_NT) {
-        const int row = i / cols, c = i - row * cols, grp = c / COLS;
-        const int64_t mr = m0 + row, n = (int64_t)col * cols + c;
-        if (n >= G.N) continue;
-        float v = part[grp << G.lwk][row][c % COLS];
-        for (int k = 1; k < G.wk; ++k) v = v + part[(grp << G.lwk) + k][row][c % COLS];
-        if (epi.kind != EPI_NONE) v = v + epi.bias[n];
-        if (epi.kind == EPI_BIAS_GELU) v = gelu_tanh(v);
-        if (epi.kind == EPI_BIAS_RESID)
-            v = v + epi.resid[(epi.resid_rows > 0 ? mr % epi.resid_rows : mr) * epi.ld_resid + n];
-        y[mr * ldy + n] = v;
+    q4_join<COLS, P, 16>(&part[0][0][0], G, col, m0, groups, y, ldy, epi);
+}
+
+// The same for 32 rows and 32 columns a wave, on the 32 x 32 MFMAs: half the
+// instructions an output of the 16 x 16 ones, and the conversion of the block
+// dots on the matrix pipe too.  A 32-value block is one
+// v_mfma_i32_32x32x32_i8 whose accumulator begins at the bits of c0 = 1/2pi, a
+// float whose ulp is 2^-26: its result read as a float is c0 + 16 I 2^-26 exactly
+// (|16 I| <= 32 * 128 * 128 = 2^19 stays in c0's binade); one f16 product adds
+// -c0 as three exact terms, another makes the scales d_w d_x, and the VALU is left
+// with one fma an output.  The sums are those of the 16-row form times 2^-22, a
+// power of two: the same bits (no term is below 2^-74 of that scale).  A tile's
+// rows, 128 bytes each, go through a part of LDS that is the wave's own: loaded
+// four lanes to 64 bytes of a row, read 16 bytes of a block a lane.  (64 columns a
+// wave: 64 x 4096 x 14336 18.6 us against 19.6, 64 x 4096 x 4096 10.8 against 8.1.)
+constexpr int Q4_XROW = 32 * 128, Q4_XW = Q4_XROW + 32 * 16;  // a wave's quants and scale words in LDS
+
+__global__ __launch_bounds__(Q4_NT) void k_mul_mat_q4_32(const uint8_t *__restrict__ wq,
+                                                         const uint16_t *__restrict__ wd, Q4Grid G,
+                                                         const int8_t *__restrict__ xq,
+                                                         const uint32_t *__restrict__ xds, float *y, int64_t ldy,
+                                                         EpiParams epi) {
+    constexpr int COLS = 32, P = COLS + 4;
+    // rows of the waves, then their sums [wave][32][P]
+    constexpr int ROWS = Q4_NW * Q4_XW, SUMS = Q4_NW * 32 * P * 4;
+    __shared__ __align__(16) uint8_t lds32[ROWS > SUMS ? ROWS : SUMS];
+    const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wk = wave & (G.wk - 1), wn = wave >> G.lwk;
+    const int groups = Q4_NW >> G.lwk;
+    const int id = xcd_linear(blockIdx.x, gridDim.x), col = id / G.row_groups;
+    const int m0 = (id - col * G.row_groups) * 32, tn0 = (col * groups + wn) * 2;
+    const int tiles_n = (G.N + 15) / 16, per = (G.tiles_k + G.wk - 1) >> G.lwk;
+    const int k0 = wk * per, k1 = min(k0 + per, G.tiles_k);
+
+    // as loaded: rows 16 a + lane / 4, piece lane % 4 of 64 bytes
+    const int8_t *xr[2];
+    const uint32_t *dr[2];
+    uint8_t *xl = lds32 + wave * Q4_XW;
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+        const int64_t m = min(m0 + 16 * a + (lane >> 2), G.M - 1);  // (rows past M: computed, not stored)
+        xr[a] = xq + m * G.KB * QK + 16 * (lane & 1);
+        dr[a] = xds + m * G.KB;
     }
+    // piece c of row w at place c ^ (w & 7) of the row's 8: 8 lanes' reads of one
+    // piece lie in 8 bank groups
+    uint8_t *xs[2][2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int w = 16 * a + (lane >> 2), c = 4 * q + (lane & 3);
+            xs[a][q] = xl + w * 128 + 16 * (c ^ (w & 7));
+        }
+    const int64_t tile = (int64_t)min(tn0 + (r >> 4), tiles_n - 1) * G.tiles_k;
+    const uint8_t *wp = wq + tile * 1024 + (16 * h + (r & 15)) * 16;  // values 16 h .. + 7 of its 4 blocks; + 512: the next 8
+    const uint16_t *dp = wd + tile * 64 + 16 * h + (r & 15);          // block h; + 32: block 2 + h
+    v16f acc = {};
+    // f16 (-0.125, -1119/256, -387/8192, 0) x (1, 2^-7, 2^-13, 0) = -c0, lanes
+    // 32 .. 63 zero
+    const v2i cA = {h ? 0 : (int)0xC45FB000u, h ? 0 : 0xAA0C};
+    const v2i cB = {h ? 0 : 0x20003C00, h ? 0 : 0x0800};
+
+    for (int t = k0; t < k1; ++t) {
+        v4u w[2], xg[2][2];
+        uint32_t d[2], dg[2];
+        const int kb = 4 * t + ((lane & 3) >> 1), last = G.KB - 1;  // (blocks past K: the last, against zeros)
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            xg[a][0] = *reinterpret_cast<const v4u *>(xr[a] + min(kb, last) * QK);
+            xg[a][1] = *reinterpret_cast<const v4u *>(xr[a] + min(kb + 2, last) * QK);
+            dg[a] = dr[a][min(4 * t + (lane & 3), last)] & 0xffffu;
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            w[j] = *reinterpret_cast<const v4u *>(wp + (int64_t)t * 1024 + 512 * j);
+            d[j] = dp[(int64_t)t * 64 + 32 * j];
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            *reinterpret_cast<v4u *>(xs[a][0]) = xg[a][0];
+            *reinterpret_cast<v4u *>(xs[a][1]) = xg[a][1];
+            reinterpret_cast<uint32_t *>(xl + Q4_XROW)[64 * a + lane] = dg[a];  // [row][block]
+        }
+        __builtin_amdgcn_wave_barrier();
+        v4i x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            x[j] = *reinterpret_cast<const v4i *>(xl + r * 128 + 16 * ((2 * j + h) ^ (r & 7)));
+        v2i dx[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            dx[j] = v2i{(int)reinterpret_cast<const uint32_t *>(xl + Q4_XROW)[4 * r + 2 * j + h], 0};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            __builtin_amdgcn_sched_barrier(0);  // (blocks apart: 121 registers, 4 waves a SIMD; mixed 134)
+            const v4i wv = {(int)((w[0][j] << 4) & 0xf0f0f0f0u), (int)(w[0][j] & 0xf0f0f0f0u),
+                            (int)((w[1][j] << 4) & 0xf0f0f0f0u), (int)(w[1][j] & 0xf0f0f0f0u)};
+            const v2i dw = {h == (j & 1) ? (int)d[j / 2] : 0, 0};
+            const v16i magic = 0x3E22F983;
+            v16f I = __builtin_bit_cast(v16f, __builtin_amdgcn_mfma_i32_32x32x32_i8(wv, x[j], magic, 0, 0, 0));
+            I = __builtin_amdgcn_mfma_f32_32x32x8f16(__builtin_bit_cast(v4h, cA), __builtin_bit_cast(v4h, cB), I, 0, 0, 0);
+            const v16f s = __builtin_amdgcn_mfma_f32_32x32x8f16(__builtin_bit_cast(v4h, dw), __builtin_bit_cast(v4h, dx[j / 2]),
+                                                                v16f{}, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[i] = fmaf(I[i], s[i], acc[i]);
+        }
+    }
+
+    // acc[4 q + i]: column 8 q + 4 h + i of row r
+    float *part = reinterpret_cast<float *>(lds32);
+    float *mine = part + (wave * 32 + r) * P + 4 * h;
+    __syncthreads();  // (the sums lie over the waves' rows)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<v4f *>(mine + 8 * q) =
+            v4f{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]} * 0x1p22f;
+    __syncthreads();
+    q4_join<COLS, P, 32>(part, G, col, m0, groups, y, ldy, epi);
 }
 
 hipError_t launch_mul_mat_q4(const Q4View &w, const int8_t *xq, const uint32_t *xds, int64_t M, float *y,
@@ -235,22 +363,29 @@ hipError_t launch_mul_mat_q4(const Q4View &w, const int8_t *xq, const uint32_t *
     // shape alone, so that a row's sums are grouped the same whatever M is.
     int wk = 1, lwk = 0;
     for (; wk < Q4_NW && wk < w.tiles_k() && w.tiles_n() * wk < 3584; ++lwk) wk *= 2;
-    const int64_t rg = (M + 15) / 16;
+    Q4Grid G{wk, lwk, (int)w.tiles_k(), (int)(w.K / QK), (int)M, (int)w.N, (int)((M + 31) / 32)};
+    const int groups = Q4_NW / wk;
+    const auto launch = [&](auto kern, int tiles) {  // column tiles of a wave
+        const int64_t per_wg = (int64_t)groups * tiles;
+        hipLaunchKernelGGL(kern, dim3((unsigned)((w.tiles_n() + per_wg - 1) / per_wg * G.row_groups)), dim3(Q4_NT), 0,
+                           stream, w.qs, w.d, G, xq, xds, y, ldy, epi);
+        return hipGetLastError();
+    };
+    // 32 rows a wave past 16, where that makes 160 workgroups: 24 x 4096 x 14336
+    // (224) 12.3 us, 16 rows a wave 14.7, 64 x 4096 x 14336 (448) 19.6 (24.6), 160
+    // x 4320 x 1152 (180) 8.5 (9.3); 32 x 4096 x 4096 (128) 8.0 (6.1), 43 x 4320 x
+    // 1152 (72) 7.3 (4.6)
+    if (M > 16 && (w.tiles_n() + 1) / 2 * G.row_groups * wk / Q4_NW >= 160) return launch(k_mul_mat_q4_32, 2);
+    G.row_groups = (int)((M + 15) / 16);
     // The rows four lanes a row and exchanged, from 5 rows on: 16 x 4096 x 14336
     // 9.7 us (a lane a row 15.1), 8 x 4096 x 4096 4.8 (4.9), 4 x 11040 x 1152 7.7
-    // (7.3).  Two column groups a wave where that leaves a workgroup for half of
-    // the CUs, one read of the rows for both: 1 x 1152 x 256000 34.5 us (one group
-    // 36.8), 4 x 4096 x 4096 5.1 (4.0); with the exchange only past two groups of
-    // rows: 64 x 4096 x 4096 8.7 (9.5), 16 x 4096 x 14336 11.5 (9.7).
-    const bool quad = M > 4, two = w.tiles_n() * rg * wk / Q4_NW > 256 && (!quad || M > 32);
-    const int nt = two ? 2 : 1;
-    const int64_t per_wg = (int64_t)(Q4_NW / wk) * nt;
-    const Q4Grid G{wk, lwk, (int)w.tiles_k(), (int)(w.K / QK), (int)M, (int)w.N, (int)rg};
-    auto kern = two ? (quad ? k_mul_mat_q4<2, true> : k_mul_mat_q4<2, false>)
-                    : (quad ? k_mul_mat_q4<1, true> : k_mul_mat_q4<1, false>);
-    hipLaunchKernelGGL(kern, dim3((unsigned)((w.tiles_n() + per_wg - 1) / per_wg * rg)), dim3(Q4_NT), 0, stream, w.qs,
-                       w.d, G, xq, xds, y, ldy, epi);
-    return hipGetLastError();
+    // (7.3).  Below, two column groups a wave where that leaves a workgroup for
+    // half of the CUs, one read of the rows for both: 1 x 1152 x 256000 34.5 us
+    // (one group 36.8), 4 x 4096 x 4096 5.1 (4.0); with the exchange one group
+    // is as fast or faster: 16 x 4096 x 14336 9.7 (two 11.5).
+    if (M > 4) return launch(k_mul_mat_q4<1, true>, 1);
+    if (w.tiles_n() * wk / Q4_NW > 256) return launch(k_mul_mat_q4<2, false>, 2);
+    return launch(k_mul_mat_q4<1, false>, 1);
 }
 
 }  // namespace s2x

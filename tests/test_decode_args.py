@@ -135,6 +135,6 @@ def test_q4_refusals():
     lib.s2x_weight_q4_0_destroy(None)
     assert lib.s2x_weight_q4_0_k(None) == 0 and lib.s2x_weight_q4_0_n(None) == 0
     assert lib.s2x_mul_mat_q4_0_q8_1(None, P, P, 1, P, 4, None, None, 0, None) == INVALID
-    assert lib.s2x_mul_mat_q4_0_workspace_size(1152, 64, 208) == 0
-    assert lib.s2x_mul_mat_q4_0_workspace_size(1152, 64, 209) >= 1152 * 64
-    assert lib.s2x_mul_mat_q4_0_workspace_size(1150, 64, 209) == 0
+    assert lib.s2x_mul_mat_q4_0_workspace_size(1152, 64, 256) == 0
+    assert lib.s2x_mul_mat_q4_0_workspace_size(1152, 64, 257) >= 1152 * 64
+    assert lib.s2x_mul_mat_q4_0_workspace_size(1150, 64, 257) == 0
