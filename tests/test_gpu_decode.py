@@ -530,27 +530,27 @@ def test_q4_many_rows(m, k, n):
     s2x.lib.s2x_weight_destroy(h)
 
 
-def test_q4_extremes():
+@pytest.mark.parametrize("m,k,n", [(2, 128, 20), (7, 256, 20), (40, 1024, 6000)])
+def test_q4_extremes(m, k, n):
     """Largest quants against largest nibbles (|I| = 32 * 8 * 128), zero and
     negative scales, residual in place, no rows."""
-    k, n = 128, 20
     q = np.zeros((n, k), np.uint8)  # -8
     q[1] = 15
     dw = np.ones((n, k // 32), np.float16)
     dw[2], dw[3] = 0, -1
-    qx = np.full((2, k), -128, np.int8)
+    qx = np.full((m, k), -128, np.int8)
     qx[1] = 127
-    dx = np.ones((2, k // 32), np.float16)
+    dx = np.ones((m, k // 32), np.float16)
     ds = dx.view(np.uint16).astype(np.uint32)
     w, qd, dd = Q4(q, dw), dev(qx), dev(ds)
-    y = run_q4(w, qd, dd, 2)
+    y = run_q4(w, qd, dd, m)
     ref, _ = q4_terms(q, dw, qx, dx)
     assert_same(y, ref.astype(np.float32), "exact in f32")
-    yr = dev(np.arange(2 * n, dtype=np.float32).reshape(2, n))
+    yr = dev(np.arange(m * n, dtype=np.float32).reshape(m, n))
     zero = dev(np.zeros(n, np.float32))
     e = s2x.Epilogue(kind=s2x.EPI_BIAS_RESID, bias=zero.data_ptr(), resid=yr.data_ptr(), ld_resid=n)
-    s2x.call("s2x_mul_mat_q4_0_q8_1", w.h, ptr(qd), ptr(dd), 2, ptr(yr), n, ctypes.byref(e), None, 0, stream())
-    assert_same(host(yr), y + np.arange(2 * n, dtype=np.float32).reshape(2, n), "in place")
+    s2x.call("s2x_mul_mat_q4_0_q8_1", w.h, ptr(qd), ptr(dd), m, ptr(yr), n, ctypes.byref(e), None, 0, stream())
+    assert_same(host(yr), y + np.arange(m * n, dtype=np.float32).reshape(m, n), "in place")
     s2x.call("s2x_mul_mat_q4_0_q8_1", w.h, None, None, 0, ptr(yr), n, None, None, 0, stream())
 
 
@@ -697,11 +697,12 @@ def test_step_from_empty_caches():
     assert host(s.len).tolist() == lens.tolist()
 
 
-def test_step_captured():
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_step_captured(kind):
     """The step in a graph, replayed over new inputs and lengths with eager
     work between the replays: every replay's outputs and cache equal those of
     eager calls on buffers of their own."""
-    a, b = Step(5, 8, 2, 128, 1152, 16, 400), Step(5, 8, 2, 128, 1152, 16, 400)
+    a, b = (Step(5, 8, 2, 128, 1152, 16, 400, kind) for _ in range(2))
     for s in (a, b):
         s.cache.mem[0].zero_()
         s.cache.mem[1].zero_()
