@@ -400,12 +400,18 @@ __global__ __launch_bounds__(PJ_NT) void k_attn_join(AttnPaged p, int chunk, int
 // (128 keys of 128 halves and their values) takes 1.4 us however few are at
 // work, some 45 bytes a ns and CU, so a launch wants all CUs at work to the end;
 // a second launch, the join, is 3 us and its gap.
-//  * no split, 8 waves a workgroup, for what a split does not speed up: up to
-//    320 tokens (3 sequences up to 300, 16 heads of 72: 7.5 us, in chunks of 128
-//    8.1; one of 500: 9.0 against 8.1) and, from 128 workgroups on, up to 1,024
-//    (8 key heads of 128: 32 up to 500 10.2 us, in chunks of 128 12.3, 64 up to
-//    700 16.3 against 20.4, 32 up to 1,000 16.1 against 15.6; 32 up to 2,000
-//    26.9 against 23.4).
+//  * no split for what it does not speed up: up to 320 tokens (3 sequences up
+//    to 300, 16 heads of 72: 7.5 us, in chunks of 128 8.1; one of 500: 9.0
+//    against 8.1) and, from 128 workgroups on, up to 1,024 (8 key heads of 128:
+//    32 up to 500 10.2 us, in chunks of 128 12.3, 64 up to 700 16.3 against
+//    20.4, 32 up to 1,000 16.1 against 15.6; 32 up to 2,000 26.9 against 23.4).
+//    8 waves a workgroup, one of which fits a CU, where they have keys and the
+//    launch is one round of them or the rounds few for the length (16 of 16
+//    heads up to 200: 6.6 us, 4 waves 7.2; 64 of 8 heads up to 700: 16.5
+//    against 19.3); 4 otherwise (64 of 8 heads up to 100: 6.3 us, 8 waves 9.8;
+//    200 of 16 heads up to 300: 33 against 58, 200 of 8 up to 1,000: 55
+//    against 62).
+//  * with a window, as for sequences of its length.
 //  * one sequence: two workgroups a CU (131,071 tokens, 8 key heads: chunks of
 //    2,048 101.5 us, of 1,024 104, of 512 108; 2,000 tokens: of 128 8.7 us, of
 //    256 10.2); a batch, whose lengths differ: 6 a CU, chunks of 256 to 768 (60
@@ -416,11 +422,13 @@ __global__ __launch_bounds__(PJ_NT) void k_attn_join(AttnPaged p, int chunk, int
 struct PaPlan {
     int chunk, n_split, nw;
 };
-static PaPlan pa_plan(int64_t n_seq, int64_t max_len, int64_t n_q_head, int64_t n_kv_head) {
+static PaPlan pa_plan_len(int64_t n_seq, int64_t max_len, int64_t n_q_head, int64_t n_kv_head) {
     const int64_t units = n_seq * n_kv_head * ((n_q_head / n_kv_head + 15) / 16);
     const int64_t span = max_len + PA_ALIGN;  // (the first tile may begin before a window)
-    if (max_len <= 320 || (units >= 128 && max_len <= 1024))
-        return PaPlan{(int)((span + 127) / 128 * 128), 1, 8};
+    if (max_len <= 320 || (units >= 128 && max_len <= 1024)) {
+        const bool wide = max_len > 128 && (units <= 256 || (max_len > 512 && units <= 1024));
+        return PaPlan{(int)((span + 127) / 128 * 128), 1, wide ? 8 : 4};
+    }
     const int64_t wgs = 512 * (n_seq < 3 ? n_seq : 3);
     const int64_t least = span * units < 65536 ? 128 : 256, most = n_seq == 1 ? 2048 : 768;
     int64_t c = span * units / wgs;
@@ -429,9 +437,20 @@ static PaPlan pa_plan(int64_t n_seq, int64_t max_len, int64_t n_q_head, int64_t 
     c = (c + 127) / 128 * 128;
     return PaPlan{(int)c, (int)((span + c - 1) / c), 4};
 }
+static PaPlan pa_plan(int64_t n_seq, int64_t max_len, int64_t window, int64_t n_q_head, int64_t n_kv_head) {
+    const PaPlan P = pa_plan_len(n_seq, max_len, n_q_head, n_kv_head);
+    if (window <= 0 || window >= max_len) return P;
+    PaPlan W = pa_plan_len(n_seq, window, n_q_head, n_kv_head);
+    if (W.n_split > P.n_split) {  // (no more chunks than the workspace, sized without a window, has room for)
+        const int64_t span = window + PA_ALIGN;
+        W.chunk = (int)(((span + P.n_split - 1) / P.n_split + 127) / 128 * 128);
+        W.n_split = (int)((span + W.chunk - 1) / W.chunk);
+    }
+    return W;
+}
 
 size_t attn_paged_workspace(int64_t n_seq, int64_t max_len, int64_t n_q_head, int64_t n_kv_head, int64_t d_head) {
-    const int n = pa_plan(n_seq, max_len, n_q_head, n_kv_head).n_split;
+    const int n = pa_plan(n_seq, max_len, 0, n_q_head, n_kv_head).n_split;
     return n > 1 ? (size_t)(n_seq * n_q_head) * n * (d_head + 2) * 4 : 0;
 }
 
@@ -453,7 +472,7 @@ static hipError_t run_paged(const AttnPaged &p, const PaPlan &P, hipStream_t str
 }
 template <typename TC>
 static hipError_t run_paged_d(const AttnPaged &p, hipStream_t stream) {
-    const PaPlan P = pa_plan(p.n_seq, p.max_len, p.n_q_head, p.kv.n_head);
+    const PaPlan P = pa_plan(p.n_seq, p.max_len, p.window, p.n_q_head, p.kv.n_head);
     const int d = p.kv.d_head;
     const hipError_t e = d == 64   ? run_paged<TC, 2, true>(p, P, stream)
                          : d == 128 ? run_paged<TC, 4, true>(p, P, stream)

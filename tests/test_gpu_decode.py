@@ -290,6 +290,8 @@ def check_attn(q, cache, table, lens, max_len, scale, window, out_kind, **kw):
     ([1200], 16, 1, 248, "bf16", "f32", 32, "token"),
     ([90, 250], 20, 1, 208, "f16", "f32", 16, "head"),
     ([1021] * 16, 8, 8, 64, "f16", "f16", 16, "head"),           # one launch past 320 tokens
+    ([3, 0, 12] * 30, 5, 5, 256, "bf16", "f32", 16, "head"),     # many short ones
+    (list(range(300, 380)), 4, 4, 72, "f16", "f16", 16, "head"),
     ([7000], 1, 1, 72, "f16", "f32", 16, "token"),               # more than 32 chunks
     (list(range(0, 740, 20)), 2, 1, 64, "bf16", "bf16", 16, "head")])
 def test_attn_paged(lens, hq, hkv, d, kind, out_kind, page, by):
@@ -305,6 +307,20 @@ def test_attn_window(window):
     lens = [0, 1, 90, 128, 1000, 2049]
     q, cache, table = attn_inputs(rng, lens, 6, 2, 128, "f16", 16, "head")
     check_attn(q, cache, table, lens, 2049, 128 ** -0.5, window, "f32")
+
+
+@pytest.mark.parametrize("n,length,window,hq,hkv", [
+    (2, 9000, 300, 4, 2), (2, 9000, 2000, 4, 2), (1, 40000, 5000, 2, 1), (40, 1500, 700, 4, 4), (130, 1030, 1000, 1, 1),
+    (6, 3000, 2990, 8, 8)])
+def test_attn_window_of_long_sequences(n, length, window, hq, hkv):
+    """Chunks laid for the window, in the workspace sized without it; tokens
+    before the window in pages that are gone from the table."""
+    rng = np.random.default_rng(window)
+    lens = [length - 7 * i for i in range(n)]
+    q, cache, table = attn_inputs(rng, lens, hq, hkv, 64, "f16", 16, "head")
+    for i, x in enumerate(lens):
+        table[i, :max(0, (x - window) // 16)] = -1
+    check_attn(q, cache, table, lens, length, 0.125, window, "f32")
 
 
 def test_attn_bounds_and_strides():
