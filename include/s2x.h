@@ -364,10 +364,11 @@ typedef enum { S2X_TYPE_F32 = 0, S2X_TYPE_F16 = 1, S2X_TYPE_BF16 = 2 } s2x_type;
  * (fp16 d, then 16 bytes of nibbles: value i of the block in the low half of
  * byte i, value 16 + i in its high half; a nibble v stands for (v - 8) * d).
  * The repack is lossless; it reorders the nibbles for the int8 MFMA.
- * K % 32 == 0, K <= 2^20, N <= 2^24, K * N <= 2^36.  create: new device memory of s2x_weight_q4_0_bytes(), raw in
- * host or device memory, synchronises `stream`.  create_in: into `dev_buf`
- * (256-byte aligned), raw on the device and unchanged until the call's work on
- * `stream` has finished, asynchronous, no allocation on the device. */
+ * K % 32 == 0, K <= 2^20, N <= 2^24, K * N <= 2^36 (K and N to whole 128).
+ * create: new device memory of s2x_weight_q4_0_bytes(), raw in host or device
+ * memory, synchronises `stream`.  create_in: into `dev_buf` (256-byte aligned),
+ * raw on the device and unchanged until the call's work on `stream` has
+ * finished, asynchronous, no allocation on the device. */
 typedef struct s2x_weight_q4 s2x_weight_q4;
 size_t s2x_weight_q4_0_bytes(int64_t K, int64_t N);
 int s2x_weight_q4_0_create(const void *raw, int raw_is_host, int64_t K, int64_t N, void *stream,
@@ -388,9 +389,9 @@ int64_t s2x_weight_q4_0_n(const s2x_weight_q4 *w);
  * into `workspace` as Q8_0 (exact: same blocks, same scales) and run
  * s2x_mul_mat_q8_0_q8_1's kernel, with its bits.  The limit is about where the
  * two cost the same (4096 x 14336: 208 rows 53 against 64 us, 256 56 against 65,
- * 288 65 either way).  workspace: s2x_mul_mat_q4_0_workspace_size() bytes, 256-byte aligned;
- * the call's own until its work has finished; 0 bytes, and NULL is taken, up
- * to S2X_Q4_FEW_ROWS. */
+ * 288 65 either way).  workspace: s2x_mul_mat_q4_0_workspace_size() bytes,
+ * 256-byte aligned; the call's own until its work has finished; 0 bytes, and
+ * NULL is taken, up to S2X_Q4_FEW_ROWS. */
 #define S2X_Q4_FEW_ROWS 256
 size_t s2x_mul_mat_q4_0_workspace_size(int64_t K, int64_t N, int64_t M);
 int s2x_mul_mat_q4_0_q8_1(const s2x_weight_q4 *w, const void *qs, const void *ds, int64_t M,
@@ -468,7 +469,9 @@ int s2x_qk_norm_rope_kv(const void *x, int32_t x_type, int64_t ld_x, int64_t n_t
  * rounding stays below the output's.  Lengths above max_len or beyond the
  * table's row count as that; pages outside 0 .. n_pages - 1 are not seen; a
  * sequence that sees nothing gets zeros and lse = -inf.  Keys and values of
- * unseen places are never read.  q and out 16-byte aligned, ld_q and ld_out
+ * unseen places are never read; an infinite value among the seen ones makes
+ * its output an infinity or a NaN (a probability's second term may have either
+ * sign or be 0), the others stay.  q and out 16-byte aligned, ld_q and ld_out
  * multiples of 8.  n_seq <= 65,535, n_seq * n_head of the cache <= 2^22;
  * workspace (256-byte aligned, the call's own until it has finished) of
  * s2x_attn_paged_workspace_size() bytes; NULL where that is 0. */

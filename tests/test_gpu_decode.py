@@ -372,6 +372,28 @@ def test_attn_score_range():
 
 
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_attn_infinite_value(kind):
+    """An infinite value that is seen makes its own element infinite or a NaN, for
+    the heads on its key head; every other element keeps its bits.  One that a
+    window leaves out changes nothing.  (The first term of a probability is
+    positive: inf (0, where it underflows: NaN).  The second is the first's rounding error: positive, and
+    the sum is inf; negative, inf - inf; 0, inf + 0 * inf.  Never finite, never
+    -inf.)"""
+    rng = np.random.default_rng(7)
+    lens = [90, 700]  # one chunk and several
+    q, cache, table = attn_inputs(rng, lens, 4, 2, 72, kind, 16, "head")
+    before, lse0 = run_attn(q, cache, table, lens, 700, 0.1, 0, "f32")
+    apart, _ = run_attn(q, cache, table, lens, 700, 0.1, 40, "f32")
+    for s in (0, 1):
+        cache.v[int(table[s, 1]), 1, 3, 37] = float("inf")  # token 19
+    got, lse = run_attn(q, cache, table, lens, 700, 0.1, 0, "f32")
+    hit = np.zeros(got.shape, bool)
+    hit[:, 2:, 37] = True
+    assert (np.isnan(got[hit]) | (got[hit] == np.inf)).all() and (got[~hit] == before[~hit]).all() and (lse == lse0).all()
+    assert (run_attn(q, cache, table, lens, 700, 0.1, 40, "f32")[0] == apart).all()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
 def test_attn_small_values(kind):
     """Values below the types' normal range count: keys and values around
     2^-20 (subnormal in f16), scores made of them."""
