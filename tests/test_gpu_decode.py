@@ -376,9 +376,9 @@ def test_attn_infinite_value(kind):
     """An infinite value that is seen makes its own element infinite or a NaN, for
     the heads on its key head; every other element keeps its bits.  One that a
     window leaves out changes nothing.  (The first term of a probability is
-    positive: inf (0, where it underflows: NaN).  The second is the first's rounding error: positive, and
-    the sum is inf; negative, inf - inf; 0, inf + 0 * inf.  Never finite, never
-    -inf.)"""
+    positive: inf; or 0, where it underflows: NaN.  The second is the first's
+    rounding error: positive, and the sum is inf; negative, inf - inf; 0, inf +
+    0 * inf.  Never finite, never -inf.)"""
     rng = np.random.default_rng(7)
     lens = [90, 700]  # one chunk and several
     q, cache, table = attn_inputs(rng, lens, 4, 2, 72, kind, 16, "head")
