@@ -144,33 +144,30 @@ hipError_t launch_kv_slots(const KvSlots &p, hipStream_t stream) {
 // whole in one lane: lanes 0 .. ceil(d_rot / 8) - 1 hold 4 pairs, the lanes
 // behind them 8 values that stay.
 // ---------------------------------------------------------------------------
-constexpr int QK_NT = 256;  // most threads of a workgroup
 
 template <typename T>
 struct Qk4 {
     typedef T vec __attribute__((ext_vector_type(4)));
 };
 
-// One workgroup: the heads of NTOK tokens (of one, or a part of its heads,
-// where tokens are few), a group of G lanes one at a time.  VEC: d_rot % 8 == 0,
-// so that a lane's values are two whole pieces of four.  cos and sin are
-// evaluated once a token and pair, into LDS; a lane's weights stay in its
-// registers; the next head's values are loaded before the present one's are
-// used.  Bound by its bytes: 8,191 rows of 32 + 2 x 8 heads of 128, bf16 to bf16,
-// 39.5 us = 5.1 TB/s, past a large copy's rate (the weights as single floats and
-// an IEEE square root and division: 55).
-template <typename TX, typename TC, int G, bool VEC, int NTOK>
-__global__ __launch_bounds__(QK_NT) void k_qk_norm_rope(QkNormRope p) {
+// One workgroup: a token's heads (those of its part, where tokens are few), NT / G
+// at a time.  VEC: d_rot % 8 == 0, so that a lane's values are two whole
+// pieces of four.  cos and sin are evaluated once a token and pair, into LDS; a
+// lane's weights stay in its registers; the next head's values are loaded
+// before the present one's are used.  Bound by its bytes: 8,191 rows of 32 + 2 x
+// 8 heads of 128, bf16 to bf16, 39.5 us = 5.1 TB/s, past a large copy's rate.
+// Several tokens a workgroup were slower (43 us with 2, 47 with 4), NT and the
+// loop left to run time 42, the weights
+// as single floats and an IEEE square root and division 55.
+template <typename TX, typename TC, int G, bool VEC, int NT>
+__global__ __launch_bounds__(NT) void k_qk_norm_rope(QkNormRope p) {
     typedef typename Qk4<TX>::vec xvec;
     typedef typename Qk4<TC>::vec cvec;
-    __shared__ float2 turn[NTOK * 128];  // cos, sin of the tokens' pairs
-    __shared__ int64_t place_of[NTOK];    // of their keys and values in the cache, -1 none
+    __shared__ float2 turn[128];  // cos, sin of the token's pairs
     const int tid = threadIdx.x, half = p.d_rot / 2, d = p.kv.d_head;
-    const int64_t row0 = (int64_t)blockIdx.x * NTOK;
-    const int nt = NTOK == 1 ? 1 : (int)min((int64_t)NTOK, p.n_tok - row0);
+    const int64_t row = blockIdx.x;
     const int lane = tid % G, n_rot = (p.d_rot + 7) / 8;
-    const int nq = p.n_q_head, nk = p.kv.n_head, heads = nq + 2 * nk;
-    const int per_wg = blockDim.x / G, step = gridDim.y * per_wg;
+    const int nq = p.n_q_head, nk = p.kv.n_head, heads = nq + 2 * nk, step = gridDim.y * (NT / G);
     // this lane's values: element e0 + i and e1 + i (i < 4), those below their ends
     int e0, e1, end0, end1;
     const bool turns = lane < n_rot;
@@ -188,8 +185,8 @@ __global__ __launch_bounds__(QK_NT) void k_qk_norm_rope(QkNormRope p) {
     struct Head {
         xvec a, b;
     };
-    auto load = [&](int t, int h) {
-        const TX *src = reinterpret_cast<const TX *>(p.x) + (row0 + t) * p.ld_x + (int64_t)h * d;
+    auto load = [&](int h) {
+        const TX *src = reinterpret_cast<const TX *>(p.x) + row * p.ld_x + (int64_t)h * d;
         Head v;
         if constexpr (VEC) {
             v.a = *reinterpret_cast<const xvec *>(src + a0);
@@ -203,10 +200,9 @@ __global__ __launch_bounds__(QK_NT) void k_qk_norm_rope(QkNormRope p) {
         }
         return v;
     };
-    const int first = blockIdx.y * per_wg + tid / G;
-    int t = 0, h = first;
+    int h = blockIdx.y * (NT / G) + tid / G;
     Head next = {};
-    if (h < heads) next = load(0, h);
+    if (h < heads) next = load(h);
     // the weights of this lane's values (a kind of head without a norm takes no
     // factor at all)
     typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -233,41 +229,32 @@ __global__ __launch_bounds__(QK_NT) void k_qk_norm_rope(QkNormRope p) {
             }
         }
     }
-    if (tid < nt) {
-        const int64_t slot = p.slots[row0 + tid], page = slot >> p.kv.page_shift;
-        place_of[tid] = slot >= 0 && page < p.kv.n_pages
-                            ? page * p.kv.ld_page + (slot & ((1 << p.kv.page_shift) - 1)) * p.kv.ld_tok : -1;
-    }
-    for (int j = tid; j < nt * half; j += blockDim.x) {
-        const int tt = NTOK > 1 && j >= half;
-        const double a = (double)p.pos[row0 + tt] * p.freq[j - tt * half];
+    const int64_t slot = p.slots[row], page = slot >> p.kv.page_shift;
+    const bool cached = slot >= 0 && page < p.kv.n_pages;
+    const int64_t place = page * p.kv.ld_page + (slot & ((1 << p.kv.page_shift) - 1)) * p.kv.ld_tok;
+    if (tid < half) {  // (half <= NT: 3 heads or more of G lanes, half <= 4 G)
+        const double a = (double)p.pos[row] * p.freq[tid];
         // whole turns off: 2 pi as a head and a tail, so that the product
         // with up to 2^40 turns keeps 2^-50 of a turn
         const double n = __builtin_rint(a * 0.15915494309189535);
         const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, a));
         float s, c;
         sincosf((float)r, &s, &c);
-        turn[j] = make_float2(c, s);
+        turn[tid] = make_float2(c, s);
     }
     __syncthreads();
 
     const float inv_d = 1.0f / (float)d;
-    while (t < nt && h < heads) {
+    for (; h < heads; h += step) {
         const Head cur = next;
-        const int tc = t, hc = h;
-        h += step;
-        if (h >= heads) {
-            h = first;
-            ++t;
-        }
-        if (t < nt) next = load(t, h);
+        if (h + step < heads) next = load(h + step);
         float a[4], b[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             a[k] = live ? (float)cur.a[k] : 0.0f;
             b[k] = live ? (float)cur.b[k] : 0.0f;
         }
-        const bool query = hc < nq, value = hc >= nq + nk;
+        const bool query = h < nq, value = h >= nq + nk;
         if (query ? p.q_norm != nullptr : !value && p.k_norm != nullptr) {  // (uniform over the group of lanes)
             float ss = 0.0f;
 #pragma unroll
@@ -284,10 +271,9 @@ __global__ __launch_bounds__(QK_NT) void k_qk_norm_rope(QkNormRope p) {
         if (!value && turns) {
             // (a lane's last pairs may be past the rotated part: theirs are
             // zeros, turned by some other pair's angle)
-            const float2 *ct = turn + tc * half;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float2 cs = ct[VEC ? 4 * lane + k : min(4 * lane + k, half - 1)];
+                const float2 cs = turn[VEC ? 4 * lane + k : min(4 * lane + k, half - 1)];
                 if (p.pairs) {
                     float &u = k < 2 ? a[2 * k] : b[2 * k - 4], &v = k < 2 ? a[2 * k + 1] : b[2 * k - 3];
                     const float u0 = u;
@@ -300,12 +286,11 @@ __global__ __launch_bounds__(QK_NT) void k_qk_norm_rope(QkNormRope p) {
                 }
             }
         }
-        const int64_t place = place_of[tc];
-        if (!live || (!query && place < 0)) continue;
+        if (!live || (!query && !cached)) continue;
         TC *dst;
-        if (query) dst = reinterpret_cast<TC *>(p.q) + (row0 + tc) * p.ld_q + (int64_t)hc * d;
-        else if (value) dst = reinterpret_cast<TC *>(p.kv.v) + place + (hc - nq - nk) * p.kv.ld_head;
-        else dst = reinterpret_cast<TC *>(p.kv.k) + place + (hc - nq) * p.kv.ld_head;
+        if (query) dst = reinterpret_cast<TC *>(p.q) + row * p.ld_q + (int64_t)h * d;
+        else if (value) dst = reinterpret_cast<TC *>(p.kv.v) + place + (h - nq - nk) * p.kv.ld_head;
+        else dst = reinterpret_cast<TC *>(p.kv.k) + place + (h - nq) * p.kv.ld_head;
         if constexpr (VEC) {
             cvec u, v;
 #pragma unroll
@@ -325,29 +310,28 @@ __global__ __launch_bounds__(QK_NT) void k_qk_norm_rope(QkNormRope p) {
     }
 }
 
-template <typename TX, typename TC, int G>
-static hipError_t run_qk(const QkNormRope &p, hipStream_t stream) {
-    const int heads = p.n_q_head + 2 * p.kv.n_head;
-    // no more waves than a token's heads fill: 21,445 rows of 1 + 2 heads of 96
-    // 13.3 us, in 256 threads 21.6
-    int threads = (heads * G + 63) / 64 * 64;
-    threads = threads > QK_NT ? QK_NT : threads;
-    const int per_wg = threads / G, rounds = (heads + per_wg - 1) / per_wg;
+template <typename TX, typename TC, int G, int NT>
+static hipError_t run_qk_nt(const QkNormRope &p, hipStream_t stream) {
+    const int heads = p.n_q_head + 2 * p.kv.n_head, per_wg = NT / G, rounds = (heads + per_wg - 1) / per_wg;
     // 8 workgroups a CU: fewer tokens than that share a token's heads among
     // workgroups (64 of 48 heads: 3 parts 3.6 us, 2 parts 4.3; 2,000: one part
     // 12.8, 2 parts 13.0, 3 parts 14.8)
     const int64_t most = 2048 / p.n_tok;
     const int parts = most < 1 ? 1 : most > rounds ? rounds : (int)most;
-    // two tokens a workgroup where a token is done in a few rounds and the card
-    // stays full: 20,000 rows of 8 + 2 heads of 128 28.6 us, one token 32.4; of 4 +
-    // 2 x 4 heads of 64 16.8, 19.8; 8,191 rows of 48 heads in 6 rounds 43.6, 40.0;
-    // 2,500 rows of 8 + 2 heads 6.6, 6.2
-    const bool two = rounds <= 3 && p.n_tok >= 4096;
-    const int64_t wgs = two ? (p.n_tok + 1) / 2 : p.n_tok;
-    auto kern = two ? (p.d_rot % 8 ? k_qk_norm_rope<TX, TC, G, false, 2> : k_qk_norm_rope<TX, TC, G, true, 2>)
-                    : (p.d_rot % 8 ? k_qk_norm_rope<TX, TC, G, false, 1> : k_qk_norm_rope<TX, TC, G, true, 1>);
-    hipLaunchKernelGGL(kern, dim3((unsigned)wgs, (unsigned)parts), dim3(threads), 0, stream, p);
+    auto kern = p.d_rot % 8 ? k_qk_norm_rope<TX, TC, G, false, NT> : k_qk_norm_rope<TX, TC, G, true, NT>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)p.n_tok, (unsigned)parts), dim3(NT), 0, stream, p);
     return hipGetLastError();
+}
+template <typename TX, typename TC, int G>
+static hipError_t run_qk(const QkNormRope &p, hipStream_t stream) {
+    // no more waves than a token's heads fill: 21,445 rows of 1 + 2 heads of 96
+    // 12.9 us, in 256 threads 21.4
+    const int want = (p.n_q_head + 2 * p.kv.n_head) * G;
+    if constexpr (3 * G <= 64)
+        if (want <= 64) return run_qk_nt<TX, TC, G, 64>(p, stream);
+    if constexpr (3 * G <= 128)
+        if (want <= 128) return run_qk_nt<TX, TC, G, 128>(p, stream);
+    return run_qk_nt<TX, TC, G, 256>(p, stream);
 }
 template <typename TX, typename TC>
 static hipError_t run_qk_g(const QkNormRope &p, hipStream_t stream) {

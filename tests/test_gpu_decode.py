@@ -185,12 +185,12 @@ def test_qk_norm_rope(t, hq, hkv, d, d_rot, style, norm, x_kind, kind, page, by)
 
 
 @pytest.mark.parametrize("t,hq,hkv,d,d_rot,style,norm,x_kind,kind,page,by", [
-    (4097, 1, 1, 96, 48, "half", True, "f32", "bf16", 16, "head"),   # a token past whole pairs of them
+    (4097, 1, 1, 96, 48, "half", True, "f32", "bf16", 16, "head"),   # workgroups of one and two waves
     (4096, 9, 3, 128, 128, "pairs", True, "bf16", "f16", 64, "token"),
     (4099, 2, 1, 72, 36, "half", False, "f16", "bf16", 16, "head"),
     (4097, 1, 2, 256, 256, "half", True, "f16", "f16", 8, "head"),
     (4097, 1, 1, 64, 0, "half", True, "f32", "f16", 16, "head")])
-def test_qk_two_tokens_a_workgroup(t, hq, hkv, d, d_rot, style, norm, x_kind, kind, page, by):
+def test_qk_few_heads_many_rows(t, hq, hkv, d, d_rot, style, norm, x_kind, kind, page, by):
     say(f"qk: {t} rows {hq}/{hkv} x {d} rot {d_rot} {style} {x_kind}->{kind}")
     qk_case(t + d, t, hq, hkv, d, d_rot, style, norm, x_kind, kind, page, by)
 
