@@ -1595,6 +1595,14 @@ static hipError_t run_tiled(const WeightView &w, const int8_t *xq, int64_t ldx, 
                             int64_t ld_ds, int64_t M, float *y, int64_t ldy, const EpiParams &epi,
                             hipStream_t stream);
 
+// A tile's offsets into the scales, y and the residual are 31-bit bytes.
+bool gemm_in_reach(const WeightView &w, int64_t ldy, const EpiParams &epi) {
+    constexpr int64_t BM = Wide::BM, most = 0x7fffffff;
+    return w.ldT * (w.K_pad / QK) <= most / 2 && ldy <= most / 4 / BM &&
+           (epi.kind != EPI_BIAS_RESID ||
+            (epi.ld_resid > 0 && (epi.resid_rows > 0 ? epi.resid_rows : BM) <= most / 4 / epi.ld_resid));
+}
+
 hipError_t launch_gemm(const WeightView &w, const int8_t *xq, const uint32_t *xds, int64_t ld_ds,
                        int64_t M, float *y, int64_t ldy, const EpiParams &epi_in,
                        hipStream_t stream, int64_t ldx) {
@@ -1608,8 +1616,8 @@ hipError_t launch_gemm(const WeightView &w, const int8_t *xq, const uint32_t *xd
         M > (1 << 30) || w.N > (1 << 30) || ((uintptr_t)xq & 15) || ((uintptr_t)w.qs & 15) ||
         ((uintptr_t)xds & 3) || (epi.kind != EPI_DUMP_I && (!xds || ld_ds < KB)) ||
         ldx < w.K_pad || ldx % 16 || w.ld_qs < w.K_pad || w.ld_qs % 16 || (int64_t)C::BM * ldx > 0x7fffffff ||
-        (int64_t)gemm::BN_MAX * w.ld_qs > 0x7fffffff || w.ldT * KB * 2 > 0x7fffffff ||
-        C::BM * ld_ds * 4 > 0x7fffffff || C::BM * ldy * 4 > 0x7fffffff ||
+        (int64_t)gemm::BN_MAX * w.ld_qs > 0x7fffffff || C::BM * ld_ds * 4 > 0x7fffffff ||
+        !gemm_in_reach(w, ldy, epi) ||
         (epi.kb_split != 0 && (epi.kind != EPI_NONE || epi.kb_split < 0 || epi.y_split < M * ldy)))
         return hipErrorInvalidValue;
 #define S2X_RUN(E)                                                                     \
@@ -1620,9 +1628,7 @@ hipError_t launch_gemm(const WeightView &w, const int8_t *xq, const uint32_t *xd
     case EPI_BIAS: return S2X_RUN(EPI_BIAS);
     case EPI_BIAS_GELU: return S2X_RUN(EPI_BIAS_GELU);
     case EPI_BIAS_RESID:
-        if (!epi.resid || epi.ld_resid < w.N || epi.resid_rows < 0 ||
-            (epi.resid_rows > 0 ? epi.resid_rows : C::BM) * epi.ld_resid * 4 > 0x7fffffff)
-            return hipErrorInvalidValue;
+        if (!epi.resid || epi.ld_resid < w.N || epi.resid_rows < 0) return hipErrorInvalidValue;
         return S2X_RUN(EPI_BIAS_RESID);
     case EPI_DUMP_I:
         if (epi.dump_kb < 0 || epi.dump_kb >= KB) return hipErrorInvalidValue;

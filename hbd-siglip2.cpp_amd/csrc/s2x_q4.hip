@@ -128,6 +128,7 @@ constexpr int Q4_NW = 8, Q4_NT = Q4_NW * WAVE;
 struct Q4Grid {
     int wk, lwk;  // waves along K (a power of two) and its logarithm
     int tiles_k, KB, M, N, row_groups;
+    int64_t resid0;  // the residual's row of row 0 (before resid_rows wraps it)
 };
 
 // The waves' sums [wave][ROWS][P] joined in the order of K, the epilogue, and out.
@@ -137,7 +138,7 @@ __device__ __forceinline__ void q4_join(const float *part, const Q4Grid &G, int 
     const int cols = COLS * groups, rows = min(ROWS, G.M - m0);
     for (int i = threadIdx.x; i < rows * cols; i += Q4_NT) {
         const int row = i / cols, c = i - row * cols, grp = c / COLS;
-        const int64_t mr = m0 + row, n = (int64_t)col * cols + c;
+        const int64_t mr = m0 + row, rr = G.resid0 + mr, n = (int64_t)col * cols + c;
         if (n >= G.N) continue;
         const float *p = part + ((grp << G.lwk) * ROWS + row) * P + c % COLS;
         float v = p[0];
@@ -145,7 +146,7 @@ __device__ __forceinline__ void q4_join(const float *part, const Q4Grid &G, int 
         if (epi.kind != EPI_NONE) v = v + epi.bias[n];
         if (epi.kind == EPI_BIAS_GELU) v = gelu_tanh(v);
         if (epi.kind == EPI_BIAS_RESID)
-            v = v + epi.resid[(epi.resid_rows > 0 ? mr % epi.resid_rows : mr) * epi.ld_resid + n];
+            v = v + epi.resid[(epi.resid_rows > 0 ? rr % epi.resid_rows : rr) * epi.ld_resid + n];
         y[mr * ldy + n] = v;
     }
 }
@@ -356,14 +357,14 @@ __global__ __launch_bounds__(Q4_NT) void k_mul_mat_q4_32(const uint8_t *__restri
     q4_join<COLS, P, 32>(part, G, col, m0, groups, y, ldy, epi);
 }
 
-hipError_t launch_mul_mat_q4(const Q4View &w, const int8_t *xq, const uint32_t *xds, int64_t M, float *y,
-                             int64_t ldy, const EpiParams &epi, hipStream_t stream) {
+static hipError_t run_q4(const Q4View &w, const int8_t *xq, const uint32_t *xds, int64_t M, float *y, int64_t ldy,
+                         const EpiParams &epi, int64_t resid0, hipStream_t stream) {
     // Parts of K: until the column groups' waves are 14 a CU (4096 x 14336, one
     // row: 10.5 us in 8 parts, 10.1 in 4, 10.4 in 2, 17 in 1).  From the weight's
     // shape alone, so that a row's sums are grouped the same whatever M is.
     int wk = 1, lwk = 0;
     for (; wk < Q4_NW && wk < w.tiles_k() && w.tiles_n() * wk < 3584; ++lwk) wk *= 2;
-    Q4Grid G{wk, lwk, (int)w.tiles_k(), (int)(w.K / QK), (int)M, (int)w.N, (int)((M + 31) / 32)};
+    Q4Grid G{wk, lwk, (int)w.tiles_k(), (int)(w.K / QK), (int)M, (int)w.N, (int)((M + 31) / 32), resid0};
     const int groups = Q4_NW / wk;
     const auto launch = [&](auto kern, int tiles) {  // column tiles of a wave
         const int64_t per_wg = (int64_t)groups * tiles;
@@ -386,6 +387,16 @@ hipError_t launch_mul_mat_q4(const Q4View &w, const int8_t *xq, const uint32_t *
     if (M > 4) return launch(k_mul_mat_q4<1, true>, 1);
     if (w.tiles_n() * wk / Q4_NW > 256) return launch(k_mul_mat_q4<2, false>, 2);
     return launch(k_mul_mat_q4<1, false>, 1);
+}
+
+// Any M.  2,048 rows a launch: at the widest weight (2^24 columns, 2^16
+// workgroups a row group of 32) that is 2^22 workgroups, 2^31 threads.
+hipError_t launch_mul_mat_q4(const Q4View &w, const int8_t *xq, const uint32_t *xds, int64_t M, float *y,
+                             int64_t ldy, const EpiParams &epi, hipStream_t stream) {
+    hipError_t e = hipSuccess;
+    for (int64_t m = 0; m < M && e == hipSuccess; m += 2048)
+        e = run_q4(w, xq + m * w.K, xds + m * (w.K / QK), M - m < 2048 ? M - m : 2048, y + m * ldy, ldy, epi, m, stream);
+    return e;
 }
 
 }  // namespace s2x

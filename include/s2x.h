@@ -389,9 +389,14 @@ int64_t s2x_weight_q4_0_n(const s2x_weight_q4 *w);
  * into `workspace` as Q8_0 (exact: same blocks, same scales) and run
  * s2x_mul_mat_q8_0_q8_1's kernel, with its bits.  The limit is about where the
  * two cost the same (4096 x 14336: 208 rows 53 against 64 us, 256 56 against 65,
- * 288 65 either way).  workspace: s2x_mul_mat_q4_0_workspace_size() bytes,
- * 256-byte aligned; the call's own until its work has finished; 0 bytes, and
- * NULL is taken, up to S2X_Q4_FEW_ROWS. */
+ * 288 65 either way).  That kernel's offsets have 31 bits: a weight of K * N >=
+ * 2^35 (N to whole 128), rows of y 2^22 floats or more apart and a residual
+ * of 2 GiB (resid_rows, or 128 rows where that is 0) are read as they lie
+ * whatever M is, with the bits of few rows.
+ * workspace: s2x_mul_mat_q4_0_workspace_size() bytes, 256-byte aligned; the
+ * call's own until its work has finished; 0 bytes, and NULL is taken, up to
+ * S2X_Q4_FEW_ROWS and for weights past that reach (and for shapes that are
+ * refused). */
 #define S2X_Q4_FEW_ROWS 256
 size_t s2x_mul_mat_q4_0_workspace_size(int64_t K, int64_t N, int64_t M);
 int s2x_mul_mat_q4_0_q8_1(const s2x_weight_q4 *w, const void *qs, const void *ds, int64_t M,
