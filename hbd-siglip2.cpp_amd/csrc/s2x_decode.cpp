@@ -270,9 +270,8 @@ int s2x_qk_norm_rope_kv(const void *x, int32_t x_type, int64_t ld_x, int64_t n_t
     return e == hipSuccess ? S2X_OK : hip_fail(e, "qk_norm_rope_kv launch");
 }
 
-static int check_paged_shape(int64_t n_seq, int64_t max_len, int64_t n_q_head, int64_t n_kv_head,
-                             int64_t d_head) {
-    const char *who = "attn_paged";
+static int check_paged_shape(const char *who, int64_t n_seq, int64_t max_len, int64_t n_q_head,
+                             int64_t n_kv_head, int64_t d_head) {
     if (n_seq < 0 || max_len < 0 || n_q_head <= 0 || n_kv_head <= 0 || n_q_head % n_kv_head || d_head <= 0)
         return fail(S2X_ERR_INVALID_ARG, "%s: n_seq=%lld max_len=%lld, %lld query heads on %lld", who,
                     (long long)n_seq, (long long)max_len, (long long)n_q_head, (long long)n_kv_head);
@@ -286,19 +285,20 @@ static int check_paged_shape(int64_t n_seq, int64_t max_len, int64_t n_q_head, i
 
 size_t s2x_attn_paged_workspace_size(int64_t n_seq, int64_t max_len, int64_t n_q_head, int64_t n_kv_head,
                                      int64_t d_head) {
-    if (check_paged_shape(n_seq, max_len, n_q_head, n_kv_head, d_head) != S2X_OK) return 0;
+    if (check_paged_shape("attn_paged", n_seq, max_len, n_q_head, n_kv_head, d_head) != S2X_OK) return 0;
     return attn_paged_workspace(n_seq, max_len, n_q_head, n_kv_head, d_head);
 }
 
-int s2x_attn_paged(const void *q, int64_t ld_q, const s2x_kv_cache *cache, const int32_t *block_table,
-                   int64_t ld_table, const int32_t *kv_len, int64_t n_seq, int64_t max_len,
-                   int64_t n_q_head, float scale, int64_t window, void *out, int32_t out_type,
-                   int64_t ld_out, float *lse, void *workspace, size_t ws_bytes, void *stream) {
-    const char *who = "attn_paged";
+// (tok_start null: row s of q is sequence s's)
+static int attn_paged(const char *who, const void *q, int64_t ld_q, int64_t n_row, const int32_t *tok_start,
+                      const s2x_kv_cache *cache, const int32_t *block_table, int64_t ld_table,
+                      const int32_t *kv_len, int64_t n_seq, int64_t max_len, int64_t n_q_head, float scale,
+                      int64_t window, void *out, int32_t out_type, int64_t ld_out, float *lse,
+                      void *workspace, size_t ws_bytes, void *stream) {
     KvView v;
     int st = check_cache(cache, v, who);
     if (st != S2X_OK) return st;
-    st = check_paged_shape(n_seq, max_len, n_q_head, v.n_head, v.d_head);
+    st = check_paged_shape(who, n_seq, max_len, n_q_head, v.n_head, v.d_head);
     if (st != S2X_OK) return st;
     if (out_type != S2X_TYPE_F32 && out_type != v.type)
         return fail(S2X_ERR_UNSUPPORTED, "%s: out_type %d (F32 or the cache's type)", who, (int)out_type);
@@ -309,11 +309,11 @@ int s2x_attn_paged(const void *q, int64_t ld_q, const s2x_kv_cache *cache, const
     if (ld_q < H || ld_q % 8 || ld_out < H || ld_out % 8)
         return fail(S2X_ERR_INVALID_ARG, "%s: ld_q=%lld / ld_out=%lld below the row or no multiple of 8", who,
                     (long long)ld_q, (long long)ld_out);
-    if (n_seq == 0) return S2X_OK;
+    if (n_seq == 0 || n_row == 0) return S2X_OK;
     if (!q || !kv_len || !out || (ld_table && max_len && !block_table))
         return fail(S2X_ERR_INVALID_ARG, "%s: null pointer", who);
     if (!aligned(q, 16) || !aligned(out, 16) || !aligned(block_table, 4) || !aligned(kv_len, 4) ||
-        !aligned(lse, 4))
+        !aligned(lse, 4) || !aligned(tok_start, 4))
         return fail(S2X_ERR_INVALID_ARG, "%s: misaligned pointer", who);
     const size_t need = attn_paged_workspace(n_seq, max_len, n_q_head, v.n_head, v.d_head);
     if (need && (!workspace || !aligned(workspace, 256)))
@@ -321,9 +321,28 @@ int s2x_attn_paged(const void *q, int64_t ld_q, const s2x_kv_cache *cache, const
     if (ws_bytes < need) return fail(S2X_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", who, ws_bytes, need);
     const AttnPaged p{q, ld_q, v, block_table, ld_table, kv_len, (int)n_seq, (int)max_len, (int)n_q_head,
                       (int)(window > INT32_MAX ? 0 : window), scale, out, out_type == S2X_TYPE_F32, ld_out,
-                      lse, workspace};
+                      lse, workspace, tok_start, n_row};
     const hipError_t e = launch_attn_paged(p, (hipStream_t)stream);
     return e == hipSuccess ? S2X_OK : hip_fail(e, "attn_paged launch");
+}
+
+int s2x_attn_paged(const void *q, int64_t ld_q, const s2x_kv_cache *cache, const int32_t *block_table,
+                   int64_t ld_table, const int32_t *kv_len, int64_t n_seq, int64_t max_len,
+                   int64_t n_q_head, float scale, int64_t window, void *out, int32_t out_type,
+                   int64_t ld_out, float *lse, void *workspace, size_t ws_bytes, void *stream) {
+    return attn_paged("attn_paged", q, ld_q, n_seq, nullptr, cache, block_table, ld_table, kv_len, n_seq, max_len,
+                      n_q_head, scale, window, out, out_type, ld_out, lse, workspace, ws_bytes, stream);
+}
+
+int s2x_attn_paged_rows(const void *q, int64_t ld_q, int64_t n_row, const int32_t *tok_start,
+                        const s2x_kv_cache *cache, const int32_t *block_table, int64_t ld_table,
+                        const int32_t *kv_len, int64_t n_seq, int64_t max_len, int64_t n_q_head, float scale,
+                        int64_t window, void *out, int32_t out_type, int64_t ld_out, float *lse,
+                        void *workspace, size_t ws_bytes, void *stream) {
+    if (n_row < 0) return fail(S2X_ERR_INVALID_ARG, "attn_paged_rows: n_row=%lld", (long long)n_row);
+    if (!tok_start && n_seq > 0 && n_row > 0) return fail(S2X_ERR_INVALID_ARG, "attn_paged_rows: tok_start is null");
+    return attn_paged("attn_paged_rows", q, ld_q, n_row, tok_start, cache, block_table, ld_table, kv_len, n_seq,
+                      max_len, n_q_head, scale, window, out, out_type, ld_out, lse, workspace, ws_bytes, stream);
 }
 
 }  // extern "C"

@@ -74,6 +74,8 @@ struct AttnPaged {
     int64_t        ld_out;
     float         *lse;      // may be null
     void          *ws;
+    const int32_t *tok_start;  // null: row s of q is sequence s's
+    int64_t        n_row;      // rows of q, with tok_start
 };
 size_t attn_paged_workspace(int64_t n_seq, int64_t max_len, int64_t n_q_head, int64_t n_kv_head,
                             int64_t d_head);

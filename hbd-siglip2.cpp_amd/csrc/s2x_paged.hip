@@ -73,12 +73,23 @@ __device__ __forceinline__ PaRange pa_range(const AttnPaged &p, int s) {
     return r;
 }
 
+// Row of q, out and lse that is sequence s's: s itself, or of packed rows the last
+// that s brings; -1: it brings none, or none that the call has.  (PACKED at
+// compile time: a test of the pointer in every workgroup, with or without a
+// branch, was 0.1 to 0.4 us of 10 to 17.)
+template <bool PACKED>
+__device__ __forceinline__ int64_t pa_row(const AttnPaged &p, int s) {
+    if constexpr (!PACKED) return s;
+    const int32_t from = p.tok_start[s], to = p.tok_start[s + 1];
+    return from >= 0 && to > from && to <= p.n_row ? to - 1 : -1;
+}
+
 // Values 4 e .. 4 e + 3 of head h: the sums over its keys by the sum of the
 // exponentials (nothing seen: zeros, and lse = -inf by itself).
 template <typename TC>
-__device__ __forceinline__ void pa_write(const AttnPaged &p, int s, int h, int d, int e, v4f a, float M, float L) {
+__device__ __forceinline__ void pa_write(const AttnPaged &p, int64_t row, int h, int d, int e, v4f a, float M, float L) {
     typedef TC vec4 __attribute__((ext_vector_type(4)));
-    const int64_t at = s * p.ld_out + (int64_t)h * d + 4 * e;
+    const int64_t at = row * p.ld_out + (int64_t)h * d + 4 * e;
     v4f y;
     vec4 t;
 #pragma unroll
@@ -88,12 +99,12 @@ __device__ __forceinline__ void pa_write(const AttnPaged &p, int s, int h, int d
     }
     if (p.out_f32) *reinterpret_cast<v4f *>((float *)p.out + at) = y;
     else *reinterpret_cast<vec4 *>((TC *)p.out + at) = t;
-    if (e == 0 && p.lse) p.lse[(int64_t)s * p.n_q_head + h] = (M + log2f(L)) * 0.693147180559945309f;
+    if (e == 0 && p.lse) p.lse[row * p.n_q_head + h] = (M + log2f(L)) * 0.693147180559945309f;
 }
 
 // DC: 32-value chunks of a head; EXACT: d_head = 32 DC; NP: terms of P; KT: 16-key
-// parts of a tile; NW: waves of a workgroup.
-template <typename TC, int DC, bool EXACT, int NP, int KT, int NW>
+// parts of a tile; NW: waves of a workgroup; PACKED: rows by tok_start.
+template <typename TC, int DC, bool EXACT, int NP, int KT, int NW, bool PACKED>
 __global__ __launch_bounds__(NW * WAVE) void k_attn_paged(AttnPaged p, int chunk, int n_split) {
     typedef typename Pa<TC>::vec vec;
     constexpr int DP = 32 * DC, DT = 2 * DC, VT = DC * KT;  // values padded, 16-value parts, V loads of a tile
@@ -126,6 +137,8 @@ __global__ __launch_bounds__(NW * WAVE) void k_attn_paged(AttnPaged p, int chunk
     const PaRange kr = pa_range(p, s);
     const int64_t start = kr.begin + (int64_t)split * chunk, end = min(start + chunk, kr.len);
     if (start >= end && n_split > 1) return;  // (uniform; an only chunk writes zeros)
+    const int64_t qrow = pa_row<PACKED>(p, s);
+    if (PACKED && qrow < 0) return;  // (uniform)
 
     const TC *kp = (const TC *)p.kv.k + hk * p.kv.ld_head, *vp = (const TC *)p.kv.v + hk * p.kv.ld_head;
     const int32_t *row = p.table + s * p.ld_table;
@@ -137,7 +150,7 @@ __global__ __launch_bounds__(NW * WAVE) void k_attn_paged(AttnPaged p, int chunk
     for (int c = 0; c < DC; ++c) {
         q[c] = vec{};
         if (r < R && (EXACT || 32 * c + 8 * g < d))
-            q[c] = *reinterpret_cast<const vec *>((const TC *)p.q + s * p.ld_q + (int64_t)(h0 + r) * d + 32 * c + 8 * g);
+            q[c] = *reinterpret_cast<const vec *>((const TC *)p.q + qrow * p.ld_q + (int64_t)(h0 + r) * d + 32 * c + 8 * g);
     }
 
     // Table entry of key t0 + lane % TILE (the row's last one for keys past it).
@@ -332,7 +345,7 @@ __global__ __launch_bounds__(NW * WAVE) void k_attn_paged(AttnPaged p, int chunk
             if (e == 0)
                 reinterpret_cast<float2 *>(ws + (int64_t)p.n_seq * p.n_q_head * n_split * d)[at] = make_float2(M, L);
         } else {
-            pa_write<TC>(p, s, h0 + h, d, e, a, M, L);
+            pa_write<TC>(p, qrow, h0 + h, d, e, a, M, L);
         }
     }
 }
@@ -342,7 +355,7 @@ __global__ __launch_bounds__(NW * WAVE) void k_attn_paged(AttnPaged p, int chunk
 // own running maximum.  The first loads are of chunks that the launch has room
 // for, whether the sequence has them or not, so that they do not wait for its
 // length.
-template <typename TC, int LANES>
+template <typename TC, int LANES, bool PACKED>
 __global__ __launch_bounds__(PJ_NT) void k_attn_join(AttnPaged p, int chunk, int n_split) {
     constexpr int GROUPS = PJ_NT / LANES;
     __shared__ __align__(16) float part[GROUPS][LANES * 4 + 4];
@@ -356,6 +369,8 @@ __global__ __launch_bounds__(PJ_NT) void k_attn_join(AttnPaged p, int chunk, int
     float2 t = mlp[min(grp, n_split - 1)];
     v4f x = ov[(int64_t)min(grp, n_split - 1) * nq];
     const PaRange kr = pa_range(p, s);
+    const int64_t qrow = pa_row<PACKED>(p, s);
+    if (PACKED && qrow < 0) return;  // (uniform)
     const int n = kr.len > kr.begin ? (int)((kr.len - kr.begin + chunk - 1) / chunk) : 0;
     v4f a = {0, 0, 0, 0};
     float M = -INFINITY, L = 0.0f;
@@ -393,7 +408,7 @@ __global__ __launch_bounds__(PJ_NT) void k_attn_join(AttnPaged p, int chunk, int
 #pragma unroll
         for (int c = 0; c < 4; ++c) y[c] = fmaf(z[c], f, y[c]);
     }
-    pa_write<TC>(p, s, h, d, e, y, top, L);
+    pa_write<TC>(p, qrow, h, d, e, y, top, L);
 }
 
 // Chunk length, number of chunks and waves of a workgroup.  A step of a workgroup
@@ -454,45 +469,48 @@ size_t attn_paged_workspace(int64_t n_seq, int64_t max_len, int64_t n_q_head, in
     return n > 1 ? (size_t)(n_seq * n_q_head) * n * (d_head + 2) * 4 : 0;
 }
 
-template <typename TC, int DC, bool EXACT, int KT, int NW>
+template <typename TC, int DC, bool EXACT, int KT, int NW, bool PACKED>
 static hipError_t run_paged_w(const AttnPaged &p, const PaPlan &P, hipStream_t stream) {
     const int group = p.n_q_head / p.kv.n_head, R = group < 16 ? group : 16;
     const int64_t wgs = (int64_t)P.n_split * p.kv.n_head * ((group + 15) / 16) * p.n_seq;
     const int v = NW * KT * 16 * p.kv.d_head * 2 + 64, o = NW * R * (DC * 32 + 4) * 4, lds = v > o ? v : o;
     // (a bf16 cache's third term only where the output would show it)
     constexpr int MOST = std::is_same<TC, __bf16>::value ? 3 : 2;
-    auto kern = p.out_f32 ? k_attn_paged<TC, DC, EXACT, MOST, KT, NW> : k_attn_paged<TC, DC, EXACT, 2, KT, NW>;
+    auto kern = p.out_f32 ? k_attn_paged<TC, DC, EXACT, MOST, KT, NW, PACKED> : k_attn_paged<TC, DC, EXACT, 2, KT, NW, PACKED>;
     hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(NW * WAVE), lds, stream, p, P.chunk, P.n_split);
     return hipGetLastError();
 }
-template <typename TC, int DC, bool EXACT>
+template <typename TC, int DC, bool EXACT, bool PACKED>
 static hipError_t run_paged(const AttnPaged &p, const PaPlan &P, hipStream_t stream) {
     constexpr int KT = DC > 4 ? 1 : 2;
-    return P.nw == 8 ? run_paged_w<TC, DC, EXACT, KT, 8>(p, P, stream) : run_paged_w<TC, DC, EXACT, KT, 4>(p, P, stream);
+    return P.nw == 8 ? run_paged_w<TC, DC, EXACT, KT, 8, PACKED>(p, P, stream)
+                     : run_paged_w<TC, DC, EXACT, KT, 4, PACKED>(p, P, stream);
 }
-template <typename TC>
+template <typename TC, bool PACKED>
 static hipError_t run_paged_d(const AttnPaged &p, hipStream_t stream) {
     const PaPlan P = pa_plan(p.n_seq, p.max_len, p.window, p.n_q_head, p.kv.n_head);
     const int d = p.kv.d_head;
-    const hipError_t e = d == 64   ? run_paged<TC, 2, true>(p, P, stream)
-                         : d == 128 ? run_paged<TC, 4, true>(p, P, stream)
-                         : d == 256 ? run_paged<TC, 8, true>(p, P, stream)
-                         : d < 64   ? run_paged<TC, 2, false>(p, P, stream)
-                         : d <= 96  ? run_paged<TC, 3, false>(p, P, stream)
-                         : d <= 192 ? run_paged<TC, 6, false>(p, P, stream)
-                                    : run_paged<TC, 8, false>(p, P, stream);
+    const hipError_t e = d == 64   ? run_paged<TC, 2, true, PACKED>(p, P, stream)
+                         : d == 128 ? run_paged<TC, 4, true, PACKED>(p, P, stream)
+                         : d == 256 ? run_paged<TC, 8, true, PACKED>(p, P, stream)
+                         : d < 64   ? run_paged<TC, 2, false, PACKED>(p, P, stream)
+                         : d <= 96  ? run_paged<TC, 3, false, PACKED>(p, P, stream)
+                         : d <= 192 ? run_paged<TC, 6, false, PACKED>(p, P, stream)
+                                    : run_paged<TC, 8, false, PACKED>(p, P, stream);
     if (e != hipSuccess || P.n_split == 1) return e;
     // few chunks: whole heads a workgroup (60 sequences of at most 8: 10.9 us
     // with 32 values each, 5.0 with 128); many: more workgroups (128 chunks
     // of one sequence: 8.2 us with 128, 4.8 with 32)
     const bool few = P.n_split <= 16;
     const int width = few ? 128 : 32;
-    auto join = few ? k_attn_join<TC, 32> : k_attn_join<TC, 8>;
+    auto join = few ? k_attn_join<TC, 32, PACKED> : k_attn_join<TC, 8, PACKED>;
     hipLaunchKernelGGL(join, dim3(p.n_q_head * ((d + width - 1) / width), p.n_seq), dim3(PJ_NT), 0, stream, p, P.chunk, P.n_split);
     return hipGetLastError();
 }
 hipError_t launch_attn_paged(const AttnPaged &p, hipStream_t stream) {
-    return p.kv.type == TY_F16 ? run_paged_d<_Float16>(p, stream) : run_paged_d<__bf16>(p, stream);
+    if (p.tok_start)
+        return p.kv.type == TY_F16 ? run_paged_d<_Float16, true>(p, stream) : run_paged_d<__bf16, true>(p, stream);
+    return p.kv.type == TY_F16 ? run_paged_d<_Float16, false>(p, stream) : run_paged_d<__bf16, false>(p, stream);
 }
 
 }  // namespace s2x

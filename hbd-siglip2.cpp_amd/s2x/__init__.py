@@ -168,6 +168,8 @@ _sig("s2x_qk_norm_rope_kv", [_p, _i32, _i64, _i64, _i64, _p, _p, _f32, _p, _i64,
 _sig("s2x_attn_paged_workspace_size", [_i64, _i64, _i64, _i64, _i64], _sz)
 _sig("s2x_attn_paged", [_p, _i64, ctypes.POINTER(KVCache), _p, _i64, _p, _i64, _i64, _i64, _f32,
                         _i64, _p, _i32, _i64, _p, _p, _sz, _p])
+_sig("s2x_attn_paged_rows", [_p, _i64, _i64, _p, ctypes.POINTER(KVCache), _p, _i64, _p, _i64, _i64, _i64, _f32,
+                             _i64, _p, _i32, _i64, _p, _p, _sz, _p])
 _sig("s2x_vision_create", [ctypes.POINTER(VisionWeights), ctypes.POINTER(_p)])
 _sig("s2x_vision_destroy", [_p], None)
 _sig("s2x_vision_set_stream", [_p, _p])

@@ -351,7 +351,8 @@ int s2x_get_rows_q8_0(const void *table_raw, int64_t K, int64_t n_rows_table,
 /* encoders.  No counterpart in the reference.  The step's calls, in order:    */
 /* s2x_kv_slots (where the new tokens' keys and values go), a projection       */
 /* (s2x_mul_mat_q4_0_q8_1 or any other product), s2x_qk_norm_rope_kv (norms,   */
-/* position rotation, write into the cache), s2x_attn_paged.                   */
+/* position rotation, write into the cache), s2x_attn_paged_rows (or, where    */
+/* every sequence brings one token, s2x_attn_paged).                           */
 /* All run on the current device, allocate nothing and may be captured into a  */
 /* graph.  Values that only the device knows (lengths, page ids, slots,        */
 /* positions) are checked there: none makes a kernel read or write outside the */
@@ -467,7 +468,8 @@ int s2x_qk_norm_rope_kv(const void *x, int32_t x_type, int64_t ld_x, int64_t n_t
  * (with window > 0 the last `window` of them), q in cache->type (n_seq rows of
  * n_q_head*d_head, ld_q apart), out in out_type (F32 or cache->type, rows
  * ld_out apart), lse (optional, n_seq x n_q_head floats) = log sum_t
- * exp(q . k_t * scale).  kv_len counts the new token where
+ * exp(q . k_t * scale).  Row s of q is sequence s's: rows packed by
+ * s2x_kv_slots are that only where every n_new is 1.  kv_len counts the new token where
  * s2x_qk_norm_rope_kv has written it.  Scores, softmax and sums are in f32;
  * the probabilities enter the second product as a sum of two terms of the
  * cache's type (three where out is f32 and the cache bf16), so that their
@@ -487,6 +489,18 @@ int s2x_attn_paged(const void *q, int64_t ld_q, const s2x_kv_cache *cache,
                    int64_t n_seq, int64_t max_len, int64_t n_q_head, float scale, int64_t window,
                    void *out, int32_t out_type, int64_t ld_out, float *lse, void *workspace,
                    size_t ws_bytes, void *stream);
+/* The same where a sequence may bring no token in this call, or several: q has
+ * n_row rows packed as s2x_kv_slots packs them, those of sequence s from
+ * tok_start[s] to tok_start[s + 1] - 1 (n_seq + 1 entries on the device).  The
+ * last of them is its query (it sees kv_len[s] tokens as above), and the same
+ * row of out (ld_out apart) and of lse (n_row x n_q_head) gets the result.  A
+ * sequence without a row, or with one outside 0 .. n_row - 1, is left out;
+ * other rows of out and lse keep what they held.  Workspace as above. */
+int s2x_attn_paged_rows(const void *q, int64_t ld_q, int64_t n_row, const int32_t *tok_start,
+                        const s2x_kv_cache *cache, const int32_t *block_table, int64_t ld_table,
+                        const int32_t *kv_len, int64_t n_seq, int64_t max_len, int64_t n_q_head,
+                        float scale, int64_t window, void *out, int32_t out_type, int64_t ld_out,
+                        float *lse, void *workspace, size_t ws_bytes, void *stream);
 
 /* ------------------------------------------------------------------------ */
 /* a10  encoders (replace siglip2::VisionEncoder / TextEncoder,               */

@@ -8,9 +8,9 @@ import pytest
 import torch
 
 import s2x
-from decode_util import q8_1_planes
+from decode_util import CODES, TYPES, attn_ref, q8_1_planes
 from gpu_util import assert_same, dev, empty, host, ptr, say, stream
-from test_gpu_decode import NAN, U, Q4, q4_terms, q4_weight, run_q4, within
+from test_gpu_decode import NAN, U, Q4, Step, attn_inputs, q4_terms, q4_weight, run_attn, run_q4, within
 
 pytestmark = pytest.mark.gpu
 
@@ -82,3 +82,159 @@ def test_q4_residual_past_two_gib():
                             for a in range(0, m, 256)])
     e = s2x.Epilogue(kind=s2x.EPI_BIAS_RESID, bias=bd.data_ptr(), resid=rd.data_ptr(), ld_resid=ld, resid_rows=rows)
     assert_same(run_q4(w, qd, dd, m, e), (parts + bias) + resid[np.arange(m) % rows], "y")
+
+
+# ---------------------------------------------------------------------------
+# attention over packed rows
+# ---------------------------------------------------------------------------
+def run_rows(q, starts, cache, table, lens, max_len, scale, window, out_kind, lse=True):
+    """q (rows, hq, d) packed; rows of out and lse start as NaNs."""
+    n_row, hq, d = q.shape
+    n = len(lens)
+    out = torch.full((n_row, hq, d), NAN, dtype=TYPES[out_kind], device="cuda:0")
+    ls = torch.full((n_row, hq), NAN, device="cuda:0") if lse else None
+    qd, td, ld, sd = q.to("cuda:0"), dev(table), dev(np.asarray(lens, np.int32)), dev(np.asarray(starts, np.int32))
+    assert len(starts) == n + 1
+    size = s2x.lib.s2x_attn_paged_workspace_size(n, max_len, hq, cache.n_head, d)
+    ws = torch.full((max(size, 1),), 0xff, dtype=torch.uint8, device="cuda:0")
+    s2x.call("s2x_attn_paged_rows", ptr(qd), hq * d, n_row, ptr(sd), cache.ref(), ptr(td), table.shape[1], ptr(ld), n,
+             max_len, hq, scale, window, ptr(out), CODES[out_kind], hq * d, ptr(ls), ptr(ws), size, stream())
+    torch.cuda.synchronize()
+    return out.double().cpu().numpy(), None if ls is None else host(ls)
+
+
+@pytest.mark.parametrize("lens,news,hq,hkv,d,kind,out_kind,window,pad", [
+    ([40, 7, 12], [1, 0, 1], 4, 2, 64, "f16", "f16", 0, 1),
+    ([0, 7, 0, 300], [0, 0, 0, 0], 4, 2, 64, "f16", "f32", 0, 3),
+    ([300, 0, 129, 5, 200], [0, 0, 1, 5, 90], 16, 16, 72, "f16", "f32", 0, 0),
+    ([3000, 17, 2999, 64], [1, 17, 0, 1], 8, 2, 128, "bf16", "bf16", 0, 2),      # several chunks
+    ([9000, 4000], [0, 33], 4, 1, 128, "f16", "f32", 700, 5),
+    ([513, 64, 65, 1], [2, 0, 1, 0], 34, 2, 80, "bf16", "f32", 0, 0),
+    ([1021] * 16, [1, 0] * 8, 8, 8, 64, "f16", "f16", 100, 8)])
+def test_attn_rows(lens, news, hq, hkv, d, kind, out_kind, window, pad):
+    """Packed rows: each sequence's last row has the bits that its query has
+    where row s is sequence s's; all other rows stay."""
+    say(f"attn rows: lens {lens} new {news} {hq}/{hkv} x {d} {kind}->{out_kind}")
+    rng = np.random.default_rng(sum(lens) + 3)
+    _, cache, table = attn_inputs(rng, lens, hq, hkv, d, kind, 16, "head")
+    starts = np.concatenate([[0], np.cumsum(news)])
+    n_row = int(starts[-1]) + pad
+    q = torch.from_numpy(rng.standard_normal((n_row, hq, d)).astype(np.float32)).to(TYPES[kind])
+    got, lse = run_rows(q, starts, cache, table, lens, max(lens), d ** -0.5, window, out_kind)
+    last = np.maximum(starts[1:] - 1, 0)
+    want, wlse = run_attn(q[last], cache, table, lens, max(lens), d ** -0.5, window, out_kind)
+    brings = np.flatnonzero(news)
+    assert_same(got[last[brings]], want[brings], "out")
+    assert_same(lse[last[brings]], wlse[brings], "lse")
+    others = np.setdiff1d(np.arange(n_row), last[brings])
+    assert np.isnan(got[others]).all() and np.isnan(lse[others]).all()
+    again, _ = run_rows(q, starts, cache, table, lens, max(lens), d ** -0.5, window, out_kind, lse=False)
+    assert_same(again[last[brings]], want[brings], "without lse")
+
+
+@pytest.mark.parametrize("length", [200, 5000])
+def test_attn_rows_bad_starts(length):
+    """Starts that are no rows of q (negative, falling, past its end): those
+    sequences are left out, the others are not."""
+    rng = np.random.default_rng(length)
+    lens = [length, 30, 20, length, 8, 9]
+    _, cache, table = attn_inputs(rng, lens, 4, 2, 64, "f16", 16, "head")
+    q = torch.from_numpy(rng.standard_normal((6, 4, 64)).astype(np.float32)).half()
+    starts = [-2 ** 31, -3, 2, 1, 5, 7, 2 ** 31 - 1]  # (only sequence 3, row 4, is whole and inside)
+    got, lse = run_rows(q, starts, cache, table, lens, length, 0.125, 0, "f32")
+    want, _ = run_attn(q[[4] * 6], cache, table, lens, length, 0.125, 0, "f32")
+    assert_same(got[4], want[3], "row 4")
+    assert np.isnan(np.delete(got, 4, 0)).all() and np.isnan(np.delete(lse, 4, 0)).all()
+    starts = [0, 1, 1, 2, 2 ** 31 - 1, -1, 4]
+    got, _ = run_rows(q, starts, cache, table, lens, length, 0.125, 0, "f32")
+    want, _ = run_attn(q[[0, 0, 1, 1, 1, 1]], cache, table, lens, length, 0.125, 0, "f32")
+    assert_same(got[:2], want[[0, 2]], "rows 0 and 1")
+    assert np.isnan(got[2:]).all()
+
+
+class PackedStep(Step):
+    """The step as documented, for batches in which a sequence may be idle."""
+
+    def run(self):
+        st, n = stream(), self.n_seq
+        (q0, d0), (q1, d1) = self.planes
+        h = self.hq * self.d
+        s2x.call("s2x_kv_slots", ptr(self.len), ptr(self.new), n, ptr(self.free), self.free.numel(), self.page,
+                 self.cache.n_pages, ptr(self.table), self.table.shape[1], n, ptr(self.len_out), ptr(self.start),
+                 ptr(self.pos), ptr(self.slots), ptr(self.used), st)
+        s2x.call("s2x_quantize_q8_1", ptr(self.x), self.hidden, n, self.hidden, self.hidden, ptr(q0), ptr(d0), st)
+        s2x.call("s2x_mul_mat_q4_0_q8_1", self.qkv.h, ptr(q0), ptr(d0), n, ptr(self.y), self.wide, None, None, 0, st)
+        s2x.call("s2x_qk_norm_rope_kv", ptr(self.y), 0, self.wide, n, self.hq, ptr(self.wq), ptr(self.wk), 1e-6,
+                 ptr(self.freq), self.d, 0, ptr(self.pos), ptr(self.slots), ptr(self.q), h, self.cache.ref(), st)
+        s2x.call("s2x_attn_paged_rows", ptr(self.q), h, n, ptr(self.start), self.cache.ref(), ptr(self.table),
+                 self.table.shape[1], ptr(self.len_out), n, self.max_len, self.hq, self.d ** -0.5, 0, ptr(self.ctx), 0, h,
+                 None, ptr(self.ws), self.ws_size, st)
+        s2x.call("s2x_quantize_q8_1", ptr(self.ctx), h, n, h, h, ptr(q1), ptr(d1), st)
+        s2x.call("s2x_mul_mat_q4_0_q8_1", self.o.h, ptr(q1), ptr(d1), n, ptr(self.out), self.hidden, None, None, 0, st)
+
+
+def check_context(s, lens, new, kind, what):
+    """The context of every sequence that brought a token, against 64 bits; rows
+    behind the last token as they were."""
+    rows = np.flatnonzero(new)
+    hq, d = s.hq, s.d
+    q = np.zeros((s.n_seq, hq, d), np.float32)
+    q[rows] = host(s.q.float()).reshape(-1, hq, d)[:len(rows)]
+    ref, size, _, top, _ = attn_ref(q, s.cache, host(s.table), lens, s.max_len, d ** -0.5, 0)
+    # a score's d products and two scalings, a probability's terms of the
+    # cache's type, the two sums
+    tol = (2 * (d + 6) * U * top + {"f16": 2.0 ** -20, "bf16": 2.0 ** -21}[kind] + 2 * (lens.max() + 8) * U)[:, :, None] * size
+    ctx = host(s.ctx).reshape(-1, hq, d)
+    within(ctx[:len(rows)], ref[rows], tol[rows], what)
+    assert (ctx[len(rows):] == 7.0).all(), what
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_step_with_idle_sequences(kind):
+    """Thirty steps of four sequences, each idle now and then, all of them
+    once: every active sequence's context is that of its own query."""
+    s = PackedStep(4, 8, 2, 64, 288, 16, 64, kind)
+    rng = np.random.default_rng(14)
+    lens = np.zeros(4, np.int64)
+    for i in range(30):
+        new = np.zeros(4, int) if i == 11 else (rng.random(4) < 0.6).astype(int)
+        s.x.copy_(dev(rng.standard_normal((4, 288)).astype(np.float32)))
+        s.new.copy_(dev(new.astype(np.int32)))
+        s.ctx.fill_(7.0)
+        s.run()
+        lens = lens + new
+        check_context(s, lens, new, kind, f"step {i}, new {new}")
+        s.advance()
+    assert host(s.len).tolist() == lens.tolist()
+
+
+def test_captured_step_with_idle_sequences():
+    """The same step in a graph: which sequences are idle is read anew at each
+    replay."""
+    s = PackedStep(5, 8, 2, 128, 1152, 16, 400)
+    rng = np.random.default_rng(15)
+    for m in s.cache.mem:
+        m.zero_()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        s.run()
+    torch.cuda.current_stream().wait_stream(st)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        s.run()
+    s.table.fill_(-1)
+    lens, free = np.zeros(5, np.int64), s.free
+    for i in range(25):
+        new = (rng.random(5) < 0.7).astype(int)
+        s.x.copy_(dev(rng.standard_normal((5, 1152)).astype(np.float32)))
+        s.new.copy_(dev(new.astype(np.int32)))
+        s.ctx.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        lens = lens + new
+        check_context(s, lens, new, "f16", f"replay {i}, new {new}")
+        free.copy_(torch.roll(free, -int(s.used[0])))
+        s.len.copy_(s.len_out)
+        torch.randn(1000, 1000, device="cuda:0").sum()  # eager work between replays
