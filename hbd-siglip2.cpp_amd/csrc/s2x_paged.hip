@@ -22,8 +22,6 @@
 // one, in k_attn_join.  Measured (both launches): one sequence of 131,071
 // tokens, 32 / 8 heads of 128, 101 us = 5.3 TB/s of keys and values, what a
 // large copy reaches; 60 sequences up to 8,000 in pages of 16, 120 us = 4.6.
-#include <type_traits>
-
 #include "s2x_decode.h"
 #include "s2x_device.h"
 
@@ -37,10 +35,15 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 typedef short v8s __attribute__((ext_vector_type(8)));
 
 template <typename T> struct Pa;
-// Terms of the cache's type that a probability enters the second product as:
-// f16 11 bits each, bf16 8.  f16 takes p * 2^15 (p <= 1), which keeps the
-// second term's 2^-25 of the largest above the subnormal range.
+// A probability enters the second product as a sum of terms of the cache's type:
+// three of bf16, 8 bits each, hold an f32's 24; two of f16, 11 bits and a
+// sign each, hold 23 (off by 2^-23 at most, twice f32's half step), and a third
+// would change little where the sums round in f32.  bf16 with two, 17 bits, was
+// 0.1 us of 10 to 16 faster, and where values cancel showed in a bf16 output too.
+// f16 takes p * 2^15 (p <= 1), which keeps the second term's
+// 2^-25 of the largest above the subnormal range.
 template <> struct Pa<_Float16> {
+    static constexpr int terms = 2;
     typedef v8h vec;
     static constexpr float up = 32768.0f, down = 1.0f / 32768.0f;
     static __device__ __forceinline__ v4f mfma(vec a, vec b, v4f c) {
@@ -51,6 +54,7 @@ template <> struct Pa<_Float16> {
     }
 };
 template <> struct Pa<__bf16> {
+    static constexpr int terms = 3;
     typedef v8bf vec;
     static constexpr float up = 1.0f, down = 1.0f;
     static __device__ __forceinline__ v4f mfma(vec a, vec b, v4f c) {
@@ -102,13 +106,13 @@ __device__ __forceinline__ void pa_write(const AttnPaged &p, int64_t row, int h,
     if (e == 0 && p.lse) p.lse[row * p.n_q_head + h] = (M + log2f(L)) * 0.693147180559945309f;
 }
 
-// DC: 32-value chunks of a head; EXACT: d_head = 32 DC; NP: terms of P; KT: 16-key
-// parts of a tile; NW: waves of a workgroup; PACKED: rows by tok_start.
-template <typename TC, int DC, bool EXACT, int NP, int KT, int NW, bool PACKED>
+// DC: 32-value chunks of a head; EXACT: d_head = 32 DC; KT: 16-key parts of a
+// tile; NW: waves of a workgroup; PACKED: rows by tok_start.
+template <typename TC, int DC, bool EXACT, int KT, int NW, bool PACKED>
 __global__ __launch_bounds__(NW * WAVE) void k_attn_paged(AttnPaged p, int chunk, int n_split) {
     typedef typename Pa<TC>::vec vec;
     constexpr int DP = 32 * DC, DT = 2 * DC, VT = DC * KT;  // values padded, 16-value parts, V loads of a tile
-    constexpr int TILE = 16 * KT, STEP = NW * TILE, NT = NW * WAVE;
+    constexpr int TILE = 16 * KT, STEP = NW * TILE, NT = NW * WAVE, NP = Pa<TC>::terms;
     extern __shared__ __align__(16) uint8_t lds[];  // V tiles of the waves, then their sums
     __shared__ float ml[NW][2][16];
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
@@ -474,9 +478,7 @@ static hipError_t run_paged_w(const AttnPaged &p, const PaPlan &P, hipStream_t s
     const int group = p.n_q_head / p.kv.n_head, R = group < 16 ? group : 16;
     const int64_t wgs = (int64_t)P.n_split * p.kv.n_head * ((group + 15) / 16) * p.n_seq;
     const int v = NW * KT * 16 * p.kv.d_head * 2 + 64, o = NW * R * (DC * 32 + 4) * 4, lds = v > o ? v : o;
-    // (a bf16 cache's third term only where the output would show it)
-    constexpr int MOST = std::is_same<TC, __bf16>::value ? 3 : 2;
-    auto kern = p.out_f32 ? k_attn_paged<TC, DC, EXACT, MOST, KT, NW, PACKED> : k_attn_paged<TC, DC, EXACT, 2, KT, NW, PACKED>;
+    auto kern = k_attn_paged<TC, DC, EXACT, KT, NW, PACKED>;
     hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(NW * WAVE), lds, stream, p, P.chunk, P.n_split);
     return hipGetLastError();
 }

@@ -471,9 +471,9 @@ int s2x_qk_norm_rope_kv(const void *x, int32_t x_type, int64_t ld_x, int64_t n_t
  * exp(q . k_t * scale).  Row s of q is sequence s's: rows packed by
  * s2x_kv_slots are that only where every n_new is 1.  kv_len counts the new token where
  * s2x_qk_norm_rope_kv has written it.  Scores, softmax and sums are in f32;
- * the probabilities enter the second product as a sum of two terms of the
- * cache's type (three where out is f32 and the cache bf16), so that their
- * rounding stays below the output's.  Lengths above max_len or beyond the
+ * the probabilities enter the second product as a sum of terms of the cache's
+ * type: three of bf16, which hold an f32 whole, two of f16, off by at most 2^-23
+ * of a probability (and 2^-40 of the largest).  Lengths above max_len or beyond the
  * table's row count as that; pages outside 0 .. n_pages - 1 are not seen; a
  * sequence that sees nothing gets zeros and lse = -inf.  Keys and values of
  * unseen places are never read; an infinite value among the seen ones makes

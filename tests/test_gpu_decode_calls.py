@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import s2x
-from decode_util import CODES, TYPES, attn_ref, q8_1_planes
+from decode_util import CODES, HALF_STEP, TYPES, Cache, attn_ref, q8_1_planes
 from gpu_util import assert_same, dev, empty, host, ptr, say, stream
 from test_gpu_decode import NAN, U, Q4, Step, attn_inputs, q4_terms, q4_weight, run_attn, run_q4, within
 
@@ -238,3 +238,46 @@ def test_captured_step_with_idle_sequences():
         free.copy_(torch.roll(free, -int(s.used[0])))
         s.len.copy_(s.len_out)
         torch.randn(1000, 1000, device="cuda:0").sum()  # eager work between replays
+
+
+# ---------------------------------------------------------------------------
+# bits of the probabilities
+# ---------------------------------------------------------------------------
+def split_bf16(x, terms):
+    """x (f64) as a sum of bf16 terms, each the nearest to what is left."""
+    left, total = x.copy(), np.zeros_like(x)
+    for _ in range(terms):
+        t = torch.from_numpy(left.astype(np.float32)).bfloat16().double().numpy()
+        total, left = total + t, left - t
+    return total
+
+
+@pytest.mark.parametrize("out_kind", ["bf16", "f32"])
+@pytest.mark.parametrize("max_len", [3, 4000])
+def test_attn_bf16_probabilities(out_kind, max_len):
+    """A bf16 cache holds its probabilities in 24 bits whatever the output's
+    type: three keys, two of score 0 with the first two bf16 terms of e as
+    values, one of score ln e with -1, so that the sum is what two terms leave of
+    e.  U of `size`, the sum of the terms' sizes: e is off by 2 of exp2 and 1.2 of
+    its argument, half of the size; five sums of at most the size's half, 2 each
+    where the matrix pipe cuts off.  10 in all, then the output's rounding."""
+    rng = np.random.default_rng(41)
+    n, d = 64, 64
+    x = torch.from_numpy(rng.uniform(0.1, 0.6, n).astype(np.float32)).bfloat16().double().numpy()
+    e = np.exp(-x)
+    hi = split_bf16(e, 1)
+    lo = split_bf16(e - hi, 1)
+    cache = Cache(n, 1, 16, d, "bf16", fill=lambda s: torch.zeros(s, device="cuda:0"))
+    sign = np.where(np.arange(d) % 3 == 1, -1.0, 1.0)
+    cache.k[:, 0, 2, 0] = torch.from_numpy(-x).to("cuda:0", torch.bfloat16)
+    for t, v in enumerate((hi, lo, -np.ones(n))):
+        cache.v[:, 0, t] = torch.from_numpy(v[:, None] * sign).to("cuda:0", torch.bfloat16)
+    q = torch.zeros(n, 1, d, dtype=torch.bfloat16)
+    q[:, 0, 0] = 1
+    table = np.zeros((n, max_len // 16 + 1), np.int32)
+    table[:, 0] = np.arange(n)
+    ref, size = (hi + lo - e) / (2 + e), (hi + np.abs(lo) + e) / (2 + e)
+    tol = 10 * U * size + HALF_STEP[out_kind] * np.abs(ref) + 4 * U * np.abs(ref)
+    assert (np.abs((hi + lo - split_bf16(e, 2)) / (2 + e) - ref) > tol).sum() >= 10  # two terms would not do
+    got, _ = run_attn(q, cache, table, [3] * n, max_len, 1.0, 0, out_kind)
+    within(got[:, 0], ref[:, None] * sign, tol[:, None] + np.zeros(d), f"{out_kind} max_len {max_len}")
