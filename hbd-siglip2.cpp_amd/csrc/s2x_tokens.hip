@@ -119,11 +119,18 @@ __global__ __launch_bounds__(KS_NT) void k_kv_slots(KvSlots p) {
         p.pos[t] = (int32_t)min(pos, (int64_t)INT32_MAX);
         p.slots[t] = slot;
     }
-    // the tables' new entries
+    // the tables' new entries; past a row's end on to the next sequence's pages, so
+    // that the rounds are the table's, not those of lengths that no table holds
+    // (up to 2^31 pages)
     for (int64_t f = first; f < min(n_fresh, (int64_t)INT32_MAX); f += step) {
         const int b = ks_upper(page0, p.n_seq, (int32_t)f);
         const int64_t i = pages(held[b]) + f - page0[b];
-        if (i < p.ld_table) p.table[b * p.ld_table + i] = given(f);
+        if (i < p.ld_table) {
+            p.table[b * p.ld_table + i] = given(f);
+        } else {
+            if (b + 1 >= p.n_seq) break;
+            f += (uint32_t)(page0[b + 1] - (int32_t)f - 1) / (uint32_t)step * step;  // (page0[b + 1] > f)
+        }
     }
 }
 

@@ -10,7 +10,8 @@ import torch
 import s2x
 from decode_util import CODES, HALF_STEP, TYPES, Cache, attn_ref, q8_1_planes
 from gpu_util import assert_same, dev, empty, host, ptr, say, stream
-from test_gpu_decode import NAN, U, Q4, Step, attn_inputs, q4_terms, q4_weight, run_attn, run_q4, within
+from test_gpu_decode import (NAN, U, Q4, Step, attn_inputs, check_slots, q4_terms, q4_weight, run_attn, run_q4,
+                             run_slots, slots_case, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -281,3 +282,39 @@ def test_attn_bf16_probabilities(out_kind, max_len):
     assert (np.abs((hi + lo - split_bf16(e, 2)) / (2 + e) - ref) > tol).sum() >= 10  # two terms would not do
     got, _ = run_attn(q, cache, table, [3] * n, max_len, 1.0, 0, out_kind)
     within(got[:, 0], ref[:, None] * sign, tol[:, None] + np.zeros(d), f"{out_kind} max_len {max_len}")
+
+
+# ---------------------------------------------------------------------------
+# slots
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("n_seq,new,cached,ld", [
+    (1000, 2 ** 31 - 1, 0, 2), (1, 2 ** 31 - 1, 5, 3), (1000, 2 ** 20, 1, 2), (8192, 2 ** 17, 0, 1), (1500, 2 ** 20, 3, 0)])
+def test_slots_lengths_past_the_table(n_seq, new, cached, ld):
+    """More new pages than the table or the free list hold, up to 2^31 of one token: the
+    rows' entries within the table, and no time for those behind it (a thread a
+    page would be 2 million rounds of a search)."""
+    rng = np.random.default_rng(n_seq)
+    table = np.full((n_seq, ld), -1, np.int32)
+    if ld:
+        table[:, :min(cached, ld)] = 7
+    free = rng.permutation(3 * n_seq + 10)
+    a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    run_slots([1], [1], [0], 1, 1, np.zeros((1, 1)), 1)
+    torch.cuda.synchronize()
+    say(f"slots: {n_seq} of {new} new tokens, table of {ld}")
+    a.record()
+    got = run_slots([cached] * n_seq, [new] * n_seq, free, 1, 3 * n_seq + 10, table, 50)
+    b.record()
+    torch.cuda.synchronize()
+    assert a.elapsed_time(b) < 100, "milliseconds"
+    want = table.copy()
+    for s in range(n_seq):
+        for i in range(cached, ld):
+            f = s * new + i - cached
+            if f < 2 ** 31 - 1:
+                want[s, i] = free[f] if f < len(free) else -1
+    assert_same(got[0], want, "table")
+    assert got[1].tolist() == [min(cached + new, 2 ** 31 - 1)] * n_seq and got[5].tolist() == [n_seq * new] * 2
+    assert got[2].tolist() == [0] + [50] * n_seq and got[3].tolist() == list(range(cached, cached + 50))
+    slots = [int(want[0, i]) if i < ld else -1 for i in range(cached, cached + 50)]
+    assert got[4].tolist() == slots
