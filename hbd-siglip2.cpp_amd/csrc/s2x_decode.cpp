@@ -221,17 +221,22 @@ int s2x_kv_slots(const int32_t *kv_len, const int32_t *n_new, int64_t n_seq, con
         !aligned(len_out, 4) || !aligned(tok_start, 4) || !aligned(pos, 4) || !aligned(slots, 8) ||
         !aligned(used, 8))
         return fail(S2X_ERR_INVALID_ARG, "kv_slots: misaligned pointer");
-    // the workgroups read the lengths while others write: no output over them
+    // the workgroups read the lengths, and the table, while others write: no
+    // output over them
     struct Range { const void *p; int64_t bytes; };
     const Range in[] = {{kv_len, 4 * n_seq}, {n_new, 4 * n_seq}, {free_pages, 4 * n_free}};
     const Range out[] = {{block_table, 4 * n_seq * ld_table}, {len_out, 4 * n_seq}, {tok_start, 4 * n_seq + 4},
                          {pos, 4 * max_tok}, {slots, 8 * max_tok}, {used, 16}};
-    for (const Range &a : in)
-        for (const Range &b : out) {
-            const uintptr_t x = (uintptr_t)a.p, z = (uintptr_t)b.p;
-            if (a.bytes && b.bytes && x < z + (uintptr_t)b.bytes && z < x + (uintptr_t)a.bytes)
-                return fail(S2X_ERR_INVALID_ARG, "kv_slots: an output overlaps an input");
-        }
+    const auto meet = [](const Range &a, const Range &b) {
+        const uintptr_t x = (uintptr_t)a.p, z = (uintptr_t)b.p;
+        return a.bytes && b.bytes && x < z + (uintptr_t)b.bytes && z < x + (uintptr_t)a.bytes;
+    };
+    for (const Range &b : out) {
+        for (const Range &a : in)
+            if (meet(a, b)) return fail(S2X_ERR_INVALID_ARG, "kv_slots: an output overlaps an input");
+        for (const Range *a = out; a != &b; ++a)
+            if (meet(*a, b)) return fail(S2X_ERR_INVALID_ARG, "kv_slots: two outputs overlap");
+    }
     const KvSlots p{kv_len, n_new, (int)n_seq, free_pages, n_free, shift, n_pages, block_table, ld_table,
                     max_tok, len_out, tok_start, pos, slots, used};
     const hipError_t e = launch_kv_slots(p, (hipStream_t)stream);

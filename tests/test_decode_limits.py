@@ -5,7 +5,7 @@ import ctypes
 import pytest
 
 import s2x
-from test_decode_args import INVALID, ODD, OK, UNSUPPORTED, WORKSPACE, P, cache
+from test_decode_args import INVALID, ODD, OK, UNSUPPORTED, WORKSPACE, P, cache, slots
 
 
 def test_q4_workspace_past_the_int8_gemm():
@@ -45,3 +45,12 @@ def test_attn_rows_refusals(change, status):
 def test_attn_rows_without_rows():
     assert attn_rows(n_row=0, q=None, out=None, tok_start=None, kv_len=None) == OK
     assert attn_rows(n_seq=0, q=None, out=None, tok_start=None, kv_len=None) == OK
+
+
+@pytest.mark.parametrize("change", [
+    dict(pos=4 << 20), dict(slots=(4 << 20) + 72), dict(len_out=(4 << 20) - 8), dict(used=6 << 20),
+    dict(start=(8 << 20) + 8), dict(pos=(5 << 20) + 12)])
+def test_slots_outputs_apart(change):
+    """The table (80 bytes from 4 << 20 on) is read while the others are
+    written; no two outputs share a byte."""
+    assert slots(**change) == INVALID, s2x.lib.s2x_last_error()
