@@ -435,7 +435,15 @@ typedef struct {
  * A page that free_pages does not have (used[0] > n_free) is entered as -1, so
  * is an id of free_pages outside 0 .. n_pages - 1; a token whose page is
  * missing, outside 0 .. n_pages - 1 or behind the row's end gets slot -1.
- * Tokens past max_tok get no row (tok_start stops there).  n_seq <= 8,192. */
+ * Tokens past max_tok get no row (tok_start stops there).
+ * len_out counts every token, those without a page or a row too.  So where
+ * used[0] > n_free or used[1] > max_tok do not carry len_out on: an attention
+ * over it would read places of tokens without a row, which hold what was there
+ * before, and a later call counts a missing page as held (it stays -1, its
+ * tokens' slots too).  The same call once more, with kv_len and n_new as they
+ * were and more pages behind those of free_pages (or more rows), gives the
+ * tables, positions and slots of a call that had them from the start.
+ * No two outputs overlap, nor an output an input.  n_seq <= 8,192. */
 int s2x_kv_slots(const int32_t *kv_len, const int32_t *n_new, int64_t n_seq,
                  const int32_t *free_pages, int64_t n_free, int64_t page_size, int64_t n_pages,
                  int32_t *block_table, int64_t ld_table, int64_t max_tok, int32_t *len_out,

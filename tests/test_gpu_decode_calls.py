@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import s2x
-from decode_util import CODES, HALF_STEP, TYPES, Cache, attn_ref, q8_1_planes
+from decode_util import CODES, HALF_STEP, TYPES, Cache, attn_ref, q8_1_planes, slots_ref
 from gpu_util import assert_same, dev, empty, host, ptr, say, stream
 from test_gpu_decode import (NAN, U, Q4, Step, attn_inputs, check_slots, q4_terms, q4_weight, run_attn, run_q4,
                              run_slots, slots_case, within)
@@ -318,3 +318,36 @@ def test_slots_lengths_past_the_table(n_seq, new, cached, ld):
     assert got[2].tolist() == [0] + [50] * n_seq and got[3].tolist() == list(range(cached, cached + 50))
     slots = [int(want[0, i]) if i < ld else -1 for i in range(cached, cached + 50)]
     assert got[4].tolist() == slots
+
+
+@pytest.mark.parametrize("short,lost", [(7, 0), (10 ** 6, 0), (0, 40), (9, 30)])
+def test_slots_shortage_and_again(short, lost):
+    """A call with too few pages or rows, then the same lengths again with
+    enough, over the tables that the first one left: all outputs of a call that
+    had enough from the start."""
+    rng = np.random.default_rng(short % 97 + lost)
+    kv_len, n_new, free, page, n_pages, table, rows = slots_case(rng, 20, 100, 50, 16)
+    few = free[:max(0, len(free) - short)]
+    first = run_slots(kv_len, n_new, few, page, n_pages, table, rows - 9 - lost if lost else rows)
+    used = first[5].tolist()
+    assert (used[0] > len(few)) == (short > 0) and used[1] == rows - 9
+    again = run_slots(kv_len, n_new, free, page, n_pages, first[0], rows)
+    whole = run_slots(kv_len, n_new, free, page, n_pages, table, rows)
+    ref = slots_ref(kv_len, n_new, free, page, n_pages, table, rows)
+    for name, a, w, r in zip(("table", "len", "start", "pos", "slots", "used"), again, whole, ref):
+        assert_same(a, w, name)
+        assert_same(a, r, name)
+    assert (again[4][:used[1]] >= 0).all()
+
+
+def test_slots_shortage_carried_on():
+    """Carried on all the same, a missing page stays missing: its tokens have no
+    slot, the pages behind it are given as ever."""
+    table = np.array([[3, -1, -1], [5, -1, -1]], np.int32)
+    got = run_slots([16, 16], [1, 1], [9], 16, 20, table, 2)  # one page for two
+    assert got[0].tolist() == [[3, 9, -1], [5, -1, -1]] and got[4].tolist() == [9 * 16, -1]
+    assert got[5].tolist() == [2, 2]
+    check_slots(got[1], [1, 1], [8, 7], 16, 20, got[0], 2, "the next step")
+    got = run_slots(got[1], [1, 16], [8, 7], 16, 20, got[0], 17)
+    assert got[0].tolist() == [[3, 9, -1], [5, -1, 8]]
+    assert got[4].tolist() == [9 * 16 + 1] + [-1] * 15 + [8 * 16]
