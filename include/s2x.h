@@ -410,9 +410,9 @@ int s2x_mul_mat_q4_0_q8_1(const s2x_weight_q4 *w, const void *qs, const void *ds
  * d_head values at k + page*ld_page + h*ld_head + place*ld_tok (elements; v
  * alike), so a page may hold its tokens by head (ld_head = page_size*d_head,
  * ld_tok = d_head) or by token (ld_tok = n_head*d_head, ld_head = d_head).
- * page_size: a power of two up to 65,536; d_head: a multiple of 8 up to 256;
- * k and v 16-byte aligned, strides multiples of 8 below 2^31 that keep all
- * rows apart. */
+ * page_size: a power of two up to 65,536; d_head: a multiple of 8 up to 256; at
+ * most 1,024 heads and 2^31 - 1 pages; k and v 16-byte aligned, strides
+ * multiples of 8 below 2^31 that keep all rows apart. */
 typedef struct {
     void   *k, *v;
     int32_t type;       /* S2X_TYPE_F16 or S2X_TYPE_BF16 */
@@ -443,7 +443,8 @@ typedef struct {
  * tokens' slots too).  The same call once more, with kv_len and n_new as they
  * were and more pages behind those of free_pages (or more rows), gives the
  * tables, positions and slots of a call that had them from the start.
- * No two outputs overlap, nor an output an input.  n_seq <= 8,192. */
+ * No two outputs overlap, nor an output an input.  n_seq <= 8,192, max_tok <
+ * 2^31 - 1, n_free, n_pages and ld_table < 2^31. */
 int s2x_kv_slots(const int32_t *kv_len, const int32_t *n_new, int64_t n_seq,
                  const int32_t *free_pages, int64_t n_free, int64_t page_size, int64_t n_pages,
                  int32_t *block_table, int64_t ld_table, int64_t max_tok, int32_t *len_out,
@@ -461,8 +462,9 @@ int s2x_kv_slots(const int32_t *kv_len, const int32_t *n_new, int64_t n_seq,
  * to cache->type: queries to q (n_tok rows, ld_q apart), keys and values to
  * slot slots[row] of the cache.  A slot outside the cache (-1) leaves the
  * cache alone; its row of q is written all the same.  Two rows with one slot
- * leave either's values there.  x and q 16-byte aligned, ld_x and ld_q
- * multiples of 8; d_rot even, 0 <= d_rot <= d_head. */
+ * leave values of either there, not all of one row.  x and q 16-byte aligned,
+ * ld_x and ld_q multiples of 8; d_rot even, 0 <= d_rot <= d_head; n_tok <= 2^23,
+ * n_q_head <= 1,024. */
 typedef enum { S2X_ROPE_HALVES = 0, S2X_ROPE_PAIRS = 1 } s2x_rope_style;
 int s2x_qk_norm_rope_kv(const void *x, int32_t x_type, int64_t ld_x, int64_t n_tok,
                         int64_t n_q_head, const float *q_norm, const float *k_norm, float eps,
@@ -477,19 +479,22 @@ int s2x_qk_norm_rope_kv(const void *x, int32_t x_type, int64_t ld_x, int64_t n_t
  * n_q_head*d_head, ld_q apart), out in out_type (F32 or cache->type, rows
  * ld_out apart), lse (optional, n_seq x n_q_head floats) = log sum_t
  * exp(q . k_t * scale).  Row s of q is sequence s's: rows packed by
- * s2x_kv_slots are that only where every n_new is 1.  kv_len counts the new token where
- * s2x_qk_norm_rope_kv has written it.  Scores, softmax and sums are in f32;
- * the probabilities enter the second product as a sum of terms of the cache's
- * type: three of bf16, which hold an f32 whole, two of f16, off by at most 2^-23
- * of a probability (and 2^-40 of the largest).  Lengths above max_len or beyond the
- * table's row count as that; pages outside 0 .. n_pages - 1 are not seen; a
- * sequence that sees nothing gets zeros and lse = -inf.  Keys and values of
- * unseen places are never read; an infinite value among the seen ones makes
- * its output an infinity or a NaN (a probability's second term may have either
- * sign or be 0), the others stay.  q and out 16-byte aligned, ld_q and ld_out
- * multiples of 8.  n_seq <= 65,535, n_seq * n_head of the cache <= 2^22;
+ * s2x_kv_slots are that only where every n_new is 1.  kv_len counts the new
+ * token where s2x_qk_norm_rope_kv has written it.  Scores, softmax and sums
+ * are in f32; the probabilities enter the second product as a sum of terms of
+ * the cache's type: three of bf16, which hold an f32 whole, two of f16, off by
+ * at most 2^-23 of a probability (and 2^-40 of the largest).  Lengths above
+ * max_len or beyond the table's row count as that; pages outside
+ * 0 .. n_pages - 1 are not seen; a sequence that sees nothing gets zeros and
+ * lse = -inf.  Keys and values of unseen places are never read; an infinite
+ * value among the seen ones makes its output an infinity or a NaN (a
+ * probability's later terms may have either sign or be 0), the others stay.  q
+ * and out 16-byte aligned, ld_q and ld_out multiples of 8.  n_seq <= 65,535,
+ * max_len <= 2^30, n_q_head <= 1,024, ld_table < 2^31, and n_seq * n_head of the
+ * cache <= 2^22, a key head counted once for each 16 query heads on it.
  * workspace (256-byte aligned, the call's own until it has finished) of
- * s2x_attn_paged_workspace_size() bytes; NULL where that is 0. */
+ * s2x_attn_paged_workspace_size() bytes; NULL where that is 0, which it also is
+ * for shapes that the call refuses. */
 size_t s2x_attn_paged_workspace_size(int64_t n_seq, int64_t max_len, int64_t n_q_head,
                                      int64_t n_kv_head, int64_t d_head);
 int s2x_attn_paged(const void *q, int64_t ld_q, const s2x_kv_cache *cache,

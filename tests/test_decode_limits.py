@@ -5,7 +5,7 @@ import ctypes
 import pytest
 
 import s2x
-from test_decode_args import INVALID, ODD, OK, UNSUPPORTED, WORKSPACE, P, cache, slots
+from test_decode_args import INVALID, ODD, OK, UNSUPPORTED, WORKSPACE, P, attn, cache, qk, slots
 
 
 def test_q4_workspace_past_the_int8_gemm():
@@ -54,3 +54,37 @@ def test_slots_outputs_apart(change):
     """The table (80 bytes from 4 << 20 on) is read while the others are
     written; no two outputs share a byte."""
     assert slots(**change) == INVALID, s2x.lib.s2x_last_error()
+
+
+def test_attn_limits():
+    """Sequences x key heads, a key head once for each 16 query heads on it; the
+    largest lengths and head counts; refused shapes want no workspace."""
+    size = s2x.lib.s2x_attn_paged_workspace_size
+    assert size(1, 1 << 30, 1024, 1, 64) > 0 and size(1, (1 << 30) + 1, 1024, 1, 64) == 0
+    assert size(1, 5000, 1024, 1, 64) > 0 and size(1, 5000, 1025, 1, 64) == 0
+    # 18 query heads a key head count as two, 16 as one; the null pointer is refused behind the shape
+    for n_q, n_kv, most in ((1008, 56, (1 << 22) // 112), (896, 56, 65535), (1024, 64, 65535), (1024, 1, 65535),
+                            (128, 128, (1 << 22) // 128)):
+        kw = dict(n_q_head=n_q, ld_q=n_q * 128, ld_out=n_q * 128, q=None)
+        c = lambda: cache(n_head=n_kv, ld_page=n_kv * 16 * 128)
+        assert attn(n_seq=most, cache=c(), **kw) == INVALID, (n_q, n_kv)
+        assert attn(n_seq=most + 1, cache=c(), **kw) == UNSUPPORTED, (n_q, n_kv)
+    assert attn(n_seq=0, max_len=1 << 30) == OK
+    big = dict(ld_q=1026 * 128, ld_out=1026 * 128)
+    assert attn(n_seq=0, n_q_head=1024, **big) == OK and attn(n_seq=0, n_q_head=1026, **big) == UNSUPPORTED
+    assert attn(ld_table=1 << 31) == INVALID
+
+
+def test_qk_limits():
+    wide = dict(n_tok=0, ld_x=1100 * 128, ld_q=1100 * 128)
+    assert qk(n_q_head=1024, **wide) == OK and qk(n_q_head=1025, **wide) == UNSUPPORTED
+    most = dict(n_tok=0, ld_x=(2 + 2 * 1025) * 128)
+    assert qk(cache=cache(n_head=1024, ld_page=1024 * 16 * 128), **most) == OK
+    assert qk(cache=cache(n_head=1025, ld_page=1025 * 16 * 128), **most) == UNSUPPORTED
+    assert qk(cache=cache(n_pages=2 ** 31 - 1), n_tok=0) == OK
+
+
+@pytest.mark.parametrize("change", [dict(n_free=2 ** 31), dict(ld_table=2 ** 31), dict(n_pages=2 ** 31),
+                                    dict(max_tok=2 ** 31 - 1), dict(n_seq=8193)])
+def test_slots_limits(change):
+    assert slots(**change) == UNSUPPORTED, s2x.lib.s2x_last_error()
