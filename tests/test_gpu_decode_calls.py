@@ -351,3 +351,42 @@ def test_slots_shortage_carried_on():
     got = run_slots(got[1], [1, 16], [8, 7], 16, 20, got[0], 17)
     assert got[0].tolist() == [[3, 9, -1], [5, -1, 8]]
     assert got[4].tolist() == [9 * 16 + 1] + [-1] * 15 + [8 * 16]
+
+
+# ---------------------------------------------------------------------------
+# Q4_0 products past the few-rows limit
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("m,k,n", [(257, 1152, 200), (300, 416, 1027), (1000, 96, 129), (263, 4320, 33)])
+def test_q4_many_rows_epilogues(m, k, n):
+    """The expanded weight's product against f64 and every epilogue on its bits:
+    bias, GELU, residual (strided, wrapped, in place), rows of y with a gap."""
+    rng = np.random.default_rng(m + n)
+    say(f"q4: {m} x {k} x {n}")
+    q, dw = q4_weight(rng, n, k)
+    qx, ds, dx = q8_1_planes(rng, m, k)
+    w, qd, dd = Q4(q, dw), dev(qx), dev(ds)
+    ref, terms = q4_terms(q, dw, qx, dx)
+    y = run_q4(w, qd, dd, m, ldy=n + 7)
+    # a block's term is rounded twice and added once
+    within(y, ref, (k // 32 + 4) * U * terms + 1e-30, "y")
+    bias, resid = rng.standard_normal(n).astype(np.float32), rng.standard_normal((m, n + 3)).astype(np.float32)
+    bd, rd = dev(bias), dev(resid)
+    e = s2x.Epilogue(kind=s2x.EPI_BIAS, bias=bd.data_ptr())
+    assert_same(run_q4(w, qd, dd, m, e, ldy=n + 1), y + bias, "bias")
+    e = s2x.Epilogue(kind=s2x.EPI_BIAS_RESID, bias=bd.data_ptr(), resid=rd.data_ptr(), ld_resid=n + 3)
+    assert_same(run_q4(w, qd, dd, m, e, ldy=n + 5), (y + bias) + resid[:, :n], "residual")
+    for rows in (1, 100):
+        e.resid_rows = rows
+        assert_same(run_q4(w, qd, dd, m, e), (y + bias) + resid[np.arange(m) % rows, :n], f"residual of {rows} rows")
+    e = s2x.Epilogue(kind=s2x.EPI_BIAS_GELU, bias=bd.data_ptr())
+    g = run_q4(w, qd, dd, m, e, ldy=n + 2)
+    v = (y + bias).astype(np.float64)
+    want = v / (1 + np.exp(-2 * np.sqrt(2 / np.pi) * (v + 0.044715 * v ** 3)))
+    # (the exponent's 4 roundings grow with it)
+    within(g, want, (16 + 8 * np.abs(v) * (1 + 0.05 * v * v)) * U * np.abs(want) + 1e-35, "gelu")
+    yr = dev(np.ascontiguousarray(resid[:, :n]))
+    e = s2x.Epilogue(kind=s2x.EPI_BIAS_RESID, bias=bd.data_ptr(), resid=yr.data_ptr(), ld_resid=n)
+    size = s2x.lib.s2x_mul_mat_q4_0_workspace_size(k, n, m)
+    ws = empty((size,), torch.uint8)
+    s2x.call("s2x_mul_mat_q4_0_q8_1", w.h, ptr(qd), ptr(dd), m, ptr(yr), n, ctypes.byref(e), ptr(ws), size, stream())
+    assert_same(host(yr), (y + bias) + resid[:, :n], "in place")
