@@ -23,6 +23,9 @@ int fail(int status, const char *fmt, ...) {
     vsnprintf(buf, sizeof(buf), fmt, ap);
     va_end(ap);
     g_last_error = buf;
+    // the runtime keeps a failed call's error until it is asked for, and the next
+    // launch, the caller's own too, would be told it
+    if (status == S2X_ERR_HIP || status == S2X_ERR_OOM) (void)hipGetLastError();
     return status;
 }
 

@@ -390,3 +390,28 @@ def test_q4_many_rows_epilogues(m, k, n):
     ws = empty((size,), torch.uint8)
     s2x.call("s2x_mul_mat_q4_0_q8_1", w.h, ptr(qd), ptr(dd), m, ptr(yr), n, ctypes.byref(e), ptr(ws), size, stream())
     assert_same(host(yr), (y + bias) + resid[:, :n], "in place")
+
+
+@pytest.mark.parametrize("from_host", [False, True])
+def test_q4_weight_without_memory(from_host):
+    """A weight that does not fit says so, and the calls after it are as ever: the
+    refused allocation's error is not reported by the next launch."""
+    k, n = 1 << 15, 1 << 18  # 4.8 GB of blocks, as much of planes
+    rng = np.random.default_rng(3)
+    small = Q4(*q4_weight(rng, 40, 64))
+    qx, ds, _ = q8_1_planes(rng, 3, 64)
+    qd, dd = dev(qx), dev(ds)
+    before = run_q4(small, qd, dd, 3)
+    raw = torch.zeros(n * k // 32 * 18, dtype=torch.uint8, device="cpu" if from_host else "cuda:0")
+    torch.cuda.empty_cache()
+    free, _ = torch.cuda.mem_get_info()
+    say(f"free {free >> 20} MiB, all but 1 GiB taken")
+    rest = torch.empty(free - (1 << 30), dtype=torch.uint8, device="cuda:0")
+    h, y = ctypes.c_void_p(), empty((3, 40), torch.float32)
+    status = s2x.lib.s2x_weight_q4_0_create(ptr(raw), int(from_host), k, n, stream(), ctypes.byref(h))
+    after = s2x.lib.s2x_mul_mat_q4_0_q8_1(small.h, ptr(qd), ptr(dd), 3, ptr(y), 40, None, None, 0, stream())
+    del rest
+    torch.cuda.empty_cache()
+    assert status == 5 and h.value is None, (status, s2x.lib.s2x_last_error())
+    assert after == 0, s2x.lib.s2x_last_error()
+    assert_same(host(y), before, "the next product")
