@@ -96,7 +96,8 @@ struct Q4View {
     int64_t tiles_n() const { return (N + 15) / 16; }
 };
 hipError_t launch_repack_q4_0(const void *raw, const Q4View &w, hipStream_t stream);
-// y = epilogue (NONE, BIAS, BIAS_GELU, BIAS_RESID), xq [M][K], xds [M][K / 32]
+// y = epilogue (NONE, BIAS, BIAS_GELU, BIAS_RESID), xq [M][K], xds [M][K / 32];
+// any M, made for few rows
 hipError_t launch_mul_mat_q4(const Q4View &w, const int8_t *xq, const uint32_t *xds, int64_t M, float *y,
                              int64_t ldy, const EpiParams &epi, hipStream_t stream);
 // the same weight as Q8_0 planes (rows of dst.ld_qs bytes, transposed scales)

@@ -162,10 +162,15 @@ struct Qk4 {
 // pieces of four.  cos and sin are evaluated once a token and pair, into LDS; a
 // lane's weights stay in its registers; the next head's values are loaded
 // before the present one's are used.  Bound by its bytes: 8,191 rows of 32 + 2 x
-// 8 heads of 128, bf16 to bf16, 39.5 us = 5.1 TB/s, past a large copy's rate.
-// Several tokens a workgroup were slower (43 us with 2, 47 with 4), NT and the
-// loop left to run time 42, the weights
-// as single floats and an IEEE square root and division 55.
+// 8 heads of 128, bf16 to bf16, 39.5 us = 5.1 TB/s, a large copy's rate (4.9 to
+// 5.3).  Several tokens a workgroup, their number at run time, were slower there
+// (43 us with 2, 47 with 4); two were faster where heads are few, since threads
+// idle there and a token's weights, angles and barrier are paid for few bytes
+// (20,000 rows of 8 + 2 heads of 128 28.6 us against 32.4, of 4 + 8 heads of 64
+// 16.8 against 19.8): given up for the wide rows, not tried at compile time.  NT
+// and the loop left to run time were 42, the weights as single floats and an IEEE
+// square root and division 55.  Not VEC: single elements, 8,191 rows of 16 + 32
+// heads of 72 in bf16, 36 turned, 89 us, with 72 turned 34.
 template <typename TX, typename TC, int G, bool VEC, int NT>
 __global__ __launch_bounds__(NT) void k_qk_norm_rope(QkNormRope p) {
     typedef typename Qk4<TX>::vec xvec;
