@@ -159,7 +159,7 @@ int64_t s2x_weight_q4_0_n(const s2x_weight_q4 *w) { return w ? w->view.N : 0; }
 
 size_t s2x_mul_mat_q4_0_workspace_size(int64_t K, int64_t N, int64_t M) {
     if (!q4_shape_ok(K, N) || M <= S2X_Q4_FEW_ROWS) return 0;
-    if (!gemm_in_reach(planes_view(nullptr, K, N, gemm_ld_q(K)), N, EpiParams{})) return 0;
+    if (!gemm_in_reach(K, gemm_ld_dw(N), N, EpiParams{})) return 0;
     return weight_planes_bytes(K, N, gemm_ld_q(K));
 }
 
@@ -186,11 +186,11 @@ int s2x_mul_mat_q4_0_q8_1(const s2x_weight_q4 *w, const void *qs, const void *ds
     if (M == 0) return S2X_OK;
     hipStream_t s = (hipStream_t)stream;
     hipError_t e;
-    const WeightView d = planes_view(workspace, v.K, v.N, gemm_ld_q(v.K));
     // (the few-rows form, whose offsets have 64 bits, takes what the GEMM cannot reach)
-    if (M <= S2X_Q4_FEW_ROWS || !gemm_in_reach(d, ldy, p)) {
+    if (M <= S2X_Q4_FEW_ROWS || !gemm_in_reach(v.K, gemm_ld_dw(v.N), ldy, p)) {
         e = launch_mul_mat_q4(v, (const int8_t *)qs, (const uint32_t *)ds, M, y, ldy, p, s);
     } else {
+        const WeightView d = planes_view(workspace, v.K, v.N, gemm_ld_q(v.K));
         e = launch_expand_q4(v, d, s);
         if (e == hipSuccess)
             e = launch_gemm(d, (const int8_t *)qs, (const uint32_t *)ds, v.K / QK_, M, y, ldy, p, s);

@@ -1596,9 +1596,9 @@ static hipError_t run_tiled(const WeightView &w, const int8_t *xq, int64_t ldx, 
                             hipStream_t stream);
 
 // A tile's offsets into the scales, y and the residual are 31-bit bytes.
-bool gemm_in_reach(const WeightView &w, int64_t ldy, const EpiParams &epi) {
+bool gemm_in_reach(int64_t K_pad, int64_t ldT, int64_t ldy, const EpiParams &epi) {
     constexpr int64_t BM = Wide::BM, most = 0x7fffffff;
-    return w.ldT * (w.K_pad / QK) <= most / 2 && ldy <= most / 4 / BM &&
+    return ldT * (K_pad / QK) <= most / 2 && ldy <= most / 4 / BM &&
            (epi.kind != EPI_BIAS_RESID ||
             (epi.ld_resid > 0 && (epi.resid_rows > 0 ? epi.resid_rows : BM) <= most / 4 / epi.ld_resid));
 }
@@ -1617,7 +1617,7 @@ hipError_t launch_gemm(const WeightView &w, const int8_t *xq, const uint32_t *xd
         ((uintptr_t)xds & 3) || (epi.kind != EPI_DUMP_I && (!xds || ld_ds < KB)) ||
         ldx < w.K_pad || ldx % 16 || w.ld_qs < w.K_pad || w.ld_qs % 16 || (int64_t)C::BM * ldx > 0x7fffffff ||
         (int64_t)gemm::BN_MAX * w.ld_qs > 0x7fffffff || C::BM * ld_ds * 4 > 0x7fffffff ||
-        !gemm_in_reach(w, ldy, epi) ||
+        !gemm_in_reach(w.K_pad, w.ldT, ldy, epi) ||
         (epi.kb_split != 0 && (epi.kind != EPI_NONE || epi.kb_split < 0 || epi.y_split < M * ldy)))
         return hipErrorInvalidValue;
 #define S2X_RUN(E)                                                                     \

@@ -103,9 +103,9 @@ hipError_t launch_repack_q8_0(const void *raw, int64_t K_pad, int64_t N, int8_t 
 hipError_t launch_gemm(const WeightView &w, const int8_t *xq, const uint32_t *xds, int64_t ld_ds,
                        int64_t M, float *y, int64_t ldy, const EpiParams &epi,
                        hipStream_t stream, int64_t ldx = 0);
-// Whether launch_gemm can address the weight's scales, rows of y ldy floats
-// apart and the residual; it refuses them otherwise.
-bool gemm_in_reach(const WeightView &w, int64_t ldy, const EpiParams &epi);
+// Whether launch_gemm can address a weight's scales (rows of ldT), rows of y ldy
+// floats apart and the residual; it refuses them otherwise.
+bool gemm_in_reach(int64_t K_pad, int64_t ldT, int64_t ldy, const EpiParams &epi);
 
 // The same product as launch_gemm with EPI_NONE / EPI_BIAS_RESID, its K
 // blocks in n_split contiguous ranges of whole 4-block stages (a function of
