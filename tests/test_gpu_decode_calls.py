@@ -402,7 +402,7 @@ def test_q4_weight_without_memory(from_host):
     qx, ds, _ = q8_1_planes(rng, 3, 64)
     qd, dd = dev(qx), dev(ds)
     before = run_q4(small, qd, dd, 3)
-    raw = torch.zeros(n * k // 32 * 18, dtype=torch.uint8, device="cpu" if from_host else "cuda:0")
+    raw = torch.empty(n * k // 32 * 18, dtype=torch.uint8, device="cpu" if from_host else "cuda:0")
     torch.cuda.empty_cache()
     free, _ = torch.cuda.mem_get_info()
     say(f"free {free >> 20} MiB, all but 1 GiB taken")
