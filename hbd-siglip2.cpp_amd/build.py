@@ -29,8 +29,13 @@ SOURCES = [
     "s2x_tokens.hip",
     "s2x_paged.hip",
     "s2x_q4.hip",
+    "s2x_norm.hip",
+    "s2x_beam.hip",
+    "s2x_pages.hip",
+    "s2x_prefix.hip",
     "s2x_abi.cpp",
     "s2x_decode.cpp",
+    "s2x_search.cpp",
     "s2x_encoders.cpp",
     "s2x_gguf.cpp",
     "siglip2_api.cpp",

@@ -1,0 +1,396 @@
+// s2x_beam.hip -- the best continuations of a beam search.
+//
+//   S[b, v] = score_b + logit[b, v] - log sum_u exp(logit[b, u])
+//
+// and the n_out largest of each request, over all its beams b and tokens v; of
+// equal ones the lower beam, then the lower token.
+//
+// k_beam_rows: a workgroup's part of a row lies in registers, read once.  Its
+// lanes' maxima serve twice: as the reference of each lane's sum of exponentials,
+// and for a bound T, the n_out-th largest of the 256 maxima (found bit by bit, by
+// counting the lanes at or above).  At least n_out values are >= T, so nothing
+// below T is of use; less than n_out lanes hold values > T, so those fit a list in
+// LDS whatever the logits are; of values equal to T the first n_out of each wave,
+// in the order of tokens, are enough.  The list's members count the larger ones
+// among them, which is their rank.
+// k_beam_join: per request, the parts' sums, and the same over their candidates
+// with S in f64: the order of two beams' candidates hangs on two sums of many
+// terms, where f32 would make ties and swaps of its own.
+#include "s2x_device.h"
+#include "s2x_search.h"
+
+namespace s2x {
+
+constexpr int BM_NT = 256, BM_WAVES = BM_NT / WAVE;
+
+template <typename T> struct Bm;
+// per: values of a lane's 16-byte load; low: bits at the end of an f32 that a value
+// of the type leaves 0
+template <> struct Bm<float> {
+    static constexpr int per = 4, low = 0;
+    typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
+    static __device__ __forceinline__ float at(const v4u &r, int j) {
+        const uint32_t u = r[j];  // (a cast of r[j] itself takes r[0])
+        return __builtin_bit_cast(float, u);
+    }
+};
+template <> struct Bm<_Float16> {
+    static constexpr int per = 8, low = 13;
+    typedef _Float16 vec __attribute__((ext_vector_type(8), aligned(2)));
+    static __device__ __forceinline__ float at(const v4u &r, int j) {
+        return f16_bits_to_f32((uint16_t)(j & 1 ? r[j / 2] >> 16 : r[j / 2]));
+    }
+};
+template <> struct Bm<__bf16> {
+    static constexpr int per = 8, low = 16;
+    typedef __bf16 vec __attribute__((ext_vector_type(8), aligned(2)));
+    static __device__ __forceinline__ float at(const v4u &r, int j) {
+        return __builtin_bit_cast(float, j & 1 ? r[j / 2] & 0xffff0000u : r[j / 2] << 16);
+    }
+};
+
+// Integers in the order of the values (-0 as +0).
+__device__ __forceinline__ uint32_t bm_key(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float bm_value(uint32_t k) {
+    return __builtin_bit_cast(float, k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+__device__ __forceinline__ uint64_t bm_key(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x + 0.0);
+    return u >> 63 ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ double bm_value(uint64_t k) {
+    return __builtin_bit_cast(double, k >> 63 ? k & ~(1ull << 63) : ~k);
+}
+
+// The K-th largest of BM_NT keys, 4 of them in each lane of the wave, which are
+// the same in every wave; its last `low` bits as its first bit tells.
+template <typename U>
+__device__ __forceinline__ U bm_kth(const U (&k)[4], int K, int low) {
+    U t = 0;
+    for (int b = 8 * sizeof(U) - 1; b >= low; --b) {
+        const U up = t | (U)1 << b;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k[i] >= up));
+        if (n >= K) t = up;
+    }
+    if (!(t >> (8 * sizeof(U) - 1))) t |= ((U)1 << low) - 1;
+    return t;
+}
+
+// e^x for x <= 0
+__device__ __forceinline__ float bm_exp(float x) {
+    return __builtin_amdgcn_exp2f(fmaf(x, 1.92596299e-08f, x * 1.44269502e+00f));
+}
+// what a sum relative to `from` counts relative to `to` >= from (-inf: an empty sum)
+__device__ __forceinline__ float bm_scale(float from, float to) { return from == -INFINITY ? 0.0f : bm_exp(from - to); }
+
+// Workspace: candidates [row][split][K] (value, token; token -1: none), then the
+// sums [row][split] of 2^(x log2 e - top) and their tops.
+struct BmCand {
+    float   x;
+    int32_t token;
+};
+struct BmSum {
+    double sum;
+    float  top;
+    int    pad;
+};
+struct BmPlan {
+    int loads, span, n_split;
+};
+// Parts of a row: up to 16 loads a lane, fewer where rows are few.
+static BmPlan bm_plan(int64_t rows, int64_t n_vocab, int per) {
+    const int64_t step = (int64_t)BM_NT * per;
+    int loads = 16;
+    while (loads > 2 && rows * ((n_vocab + loads * step - 1) / (loads * step)) < 1024) loads /= 2;
+    const int64_t n = (n_vocab + loads * step - 1) / (loads * step);
+    int64_t span = (n_vocab + n - 1) / n;
+    span = (span + per - 1) / per * per;
+    return BmPlan{loads, (int)span, (int)((n_vocab + span - 1) / span)};
+}
+static int64_t bm_most_splits(int64_t rows, int64_t n_vocab) {  // whatever the type
+    const int a = bm_plan(rows, n_vocab, 4).n_split, b = bm_plan(rows, n_vocab, 8).n_split;
+    return a > b ? a : b;
+}
+size_t beam_select_workspace(int64_t n_req, int64_t n_beam, int64_t n_vocab, int64_t n_out) {
+    const int64_t parts = n_req * n_beam * bm_most_splits(n_req * n_beam, n_vocab);
+    return (size_t)parts * (sizeof(BmSum) + n_out * sizeof(BmCand));
+}
+__device__ __forceinline__ BmSum *bm_sums(const BeamSelect &p) { return (BmSum *)p.ws; }
+__device__ __forceinline__ BmCand *bm_cands(const BeamSelect &p, int n_split) {
+    return (BmCand *)(bm_sums(p) + (int64_t)p.n_req * p.n_beam * n_split);
+}
+// 0: no beam, 1: a beam, 2: one that has ended
+__device__ __forceinline__ int bm_state(const BeamSelect &p, int row) {
+    const float s = p.scores[row];
+    return !(fabsf(s) < INFINITY) ? 0 : p.done && p.done[row] ? 2 : 1;
+}
+
+template <typename T, int NL>
+__global__ __launch_bounds__(BM_NT) void k_beam_rows(BeamSelect p, int span, int n_split, int cap) {
+    constexpr int PER = Bm<T>::per, STEP = BM_NT * PER;
+    extern __shared__ __align__(16) uint8_t lds[];
+    uint64_t *list = reinterpret_cast<uint64_t *>(lds);  // key | ~place, `cap` entries
+    __shared__ float tops[BM_NT];
+    __shared__ double wsum[BM_WAVES];
+    __shared__ float wtop[BM_WAVES];
+    __shared__ int count;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.y, split = blockIdx.x;
+    if (bm_state(p, row) != 1) return;  // (uniform)
+    const int from = split * span, n = min(span, p.n_vocab - from), K = p.n_out;
+    const T *x = (const T *)p.logits + (int64_t)row * p.ld + from;
+    if (tid == 0) count = 0;
+
+    v4u r[NL];
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+        const int c = i * STEP + tid * PER;
+        if (c + PER <= n) {
+            r[i] = __builtin_bit_cast(v4u, *reinterpret_cast<const typename Bm<T>::vec *>(x + c));
+        } else {
+            T t[PER];
+#pragma unroll
+            for (int j = 0; j < PER; ++j) t[j] = c + j < n ? x[c + j] : (T)-INFINITY;
+            __builtin_memcpy(&r[i], t, 16);
+        }
+    }
+    float mi[NL], top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+        mi[i] = Bm<T>::at(r[i], 0);
+#pragma unroll
+        for (int j = 1; j < PER; ++j) mi[i] = fmaxf(mi[i], Bm<T>::at(r[i], j));
+        top = fmaxf(top, mi[i]);
+    }
+    tops[tid] = top;
+    // the sum relative to the lane's largest, log2(e) as a head and a tail
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) sum = sum + bm_exp(Bm<T>::at(r[i], j) - ref);
+    {
+        const float wt = group_max<64>(top);
+        const double ws = wave_dsum((double)sum * (double)bm_scale(top, wt));
+        if (lane == 0) {
+            wsum[wave] = ws;
+            wtop[wave] = wt;
+        }
+    }
+    __syncthreads();
+    uint32_t k4[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k4[i] = bm_key(tops[i * WAVE + lane]);
+    const float bound = bm_value(bm_kth(k4, K, Bm<T>::low));
+
+    // values above the bound, then the wave's first K equal to it
+    auto put = [&](float v, int c, int at) { list[at] = (uint64_t)bm_key(v) << 32 | (uint32_t)~c; };
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+        if (__builtin_amdgcn_ballot_w64(mi[i] > bound) == 0) continue;
+        if (mi[i] > bound) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const float v = Bm<T>::at(r[i], j);
+                if (v > bound) put(v, i * STEP + tid * PER + j, atomicAdd(&count, 1));
+            }
+        }
+    }
+    if (bound > -INFINITY) {
+        int taken = 0;  // (uniform over the wave)
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            if (taken >= K || __builtin_amdgcn_ballot_w64(mi[i] >= bound) == 0) continue;
+            int here = 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) here += Bm<T>::at(r[i], j) == bound;
+            int in = here;
+#pragma unroll
+            for (int o = 1; o < WAVE; o <<= 1) {
+                const int t = __shfl_up(in, o);
+                if (lane >= o) in += t;
+            }
+            int rank = taken + in - here;
+            taken += __shfl(in, WAVE - 1);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                if (Bm<T>::at(r[i], j) == bound && rank++ < K) put(bound, i * STEP + tid * PER + j, atomicAdd(&count, 1));
+            }
+        }
+    }
+    __syncthreads();
+    const int C = min(count, cap);
+    const int64_t part = (int64_t)row * n_split + split;
+    BmCand *out = bm_cands(p, n_split) + part * K;
+    for (int e = tid; e < C; e += BM_NT) {
+        const uint64_t k = list[e];
+        int rank = 0;
+        for (int q = 0; q < C; ++q) rank += list[q] > k;
+        if (rank < K) out[rank] = BmCand{bm_value((uint32_t)(k >> 32)), from + (int)~(uint32_t)k};
+    }
+    for (int e = C + tid; e < K; e += BM_NT) out[e] = BmCand{-INFINITY, -1};
+    if (tid == 0) {
+        float wt = wtop[0];
+#pragma unroll
+        for (int w = 1; w < BM_WAVES; ++w) wt = fmaxf(wt, wtop[w]);
+        double s = 0.0;
+#pragma unroll
+        for (int w = 0; w < BM_WAVES; ++w) s += wsum[w] * (double)bm_scale(wtop[w], wt);
+        bm_sums(p)[part] = BmSum{s, wt, 0};
+    }
+}
+
+constexpr int BJ_PER = 8, BJ_TILE = BM_NT * BJ_PER;  // candidates of a round
+constexpr int BJ_CAP = (BEAM_MAX_OUT - 1) * (BJ_PER + 1) + BM_WAVES * BEAM_MAX_OUT;
+
+__global__ __launch_bounds__(BM_NT) void k_beam_join(BeamSelect p, int n_split) {
+    __shared__ double add[BEAM_MAX_OUT];  // score - lse of the beams; -inf: none
+    __shared__ uint8_t state[BEAM_MAX_OUT];
+    __shared__ uint64_t tops[BM_NT], lk[BJ_CAP];
+    __shared__ int32_t lp[BJ_CAP], lt[BJ_CAP], lb[BJ_CAP];
+    __shared__ uint64_t bk[BEAM_MAX_OUT];  // the best so far, in order
+    __shared__ int32_t bt[BEAM_MAX_OUT], bb[BEAM_MAX_OUT];
+    __shared__ int count;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, req = blockIdx.x, K = p.n_out;
+    const BmSum *sums = bm_sums(p);
+    const BmCand *cands = bm_cands(p, n_split);
+    for (int b = wave; b < p.n_beam; b += BM_WAVES) {
+        const int row = req * p.n_beam + b, st = bm_state(p, row);
+        float top = -INFINITY;
+        double s = 0.0;
+        if (st == 1) {
+            for (int i = lane; i < n_split; i += WAVE) top = fmaxf(top, sums[(int64_t)row * n_split + i].top);
+            top = group_max<64>(top);
+            for (int i = lane; i < n_split; i += WAVE) {
+                const BmSum q = sums[(int64_t)row * n_split + i];
+                s += q.sum * (double)bm_scale(q.top, top);
+            }
+            s = wave_dsum(s);
+        }
+        if (lane == 0) {
+            // (no finite sum, from a NaN or an infinity, and no value at all: no candidates)
+            const double lse = log(s) + (double)top;
+            state[b] = st;
+            add[b] = st == 2 ? (double)p.scores[row] : st == 1 && fabs(lse) < INFINITY ? (double)p.scores[row] - lse : -INFINITY;
+        }
+    }
+    if (tid < K) {
+        bk[tid] = bm_key(-(double)INFINITY);
+        bt[tid] = bb[tid] = -1;
+    }
+    const int per_beam = n_split * K, all = p.n_beam * per_beam;
+    for (int e0 = 0; e0 < all; e0 += BJ_TILE) {
+        __syncthreads();
+        if (tid == 0) count = 0;
+        // this round's candidates, and the best of those before as places below
+        // all of them
+        uint64_t key[BJ_PER + 1];
+        int32_t tok[BJ_PER + 1];
+        int beam[BJ_PER + 1];
+#pragma unroll
+        for (int i = 0; i <= BJ_PER; ++i) {
+            key[i] = bm_key(-(double)INFINITY);
+            tok[i] = -1;
+            beam[i] = -1;
+            if (i == 0) {
+                if (tid < K) {
+                    key[0] = bk[tid];
+                    tok[0] = bt[tid];
+                    beam[0] = bb[tid];
+                }
+                continue;
+            }
+            const int e = e0 + (i - 1) * BM_NT + tid;
+            if (e >= all) continue;
+            const int b = e / per_beam, rest = e - b * per_beam;
+            beam[i] = b;
+            if (state[b] == 2) {
+                if (rest == 0) {
+                    key[i] = bm_key(add[b]);
+                    tok[i] = p.done_token;
+                }
+            } else if (state[b] == 1 && add[b] > -INFINITY) {
+                const BmCand c = cands[((int64_t)req * p.n_beam + b) * per_beam + rest];
+                if (c.token >= 0) key[i] = bm_key(add[b] + (double)c.x);
+                tok[i] = c.token;
+            }
+        }
+        uint64_t top = key[0];
+#pragma unroll
+        for (int i = 1; i <= BJ_PER; ++i) top = max(top, key[i]);
+        tops[tid] = top;
+        __syncthreads();
+        uint64_t k4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k4[i] = tops[i * WAVE + lane];
+        const uint64_t none = bm_key(-(double)INFINITY), bound = bm_kth(k4, K, 0);
+        auto put = [&](int i, int at) {
+            lk[at] = key[i];
+            lp[at] = i * BM_NT + tid;
+            lt[at] = tok[i];
+            lb[at] = beam[i];
+        };
+        int taken = 0;
+#pragma unroll
+        for (int i = 0; i <= BJ_PER; ++i) {
+            if (key[i] > bound) put(i, atomicAdd(&count, 1));
+            const uint64_t eq = __builtin_amdgcn_ballot_w64(key[i] == bound && bound > none);
+            if (key[i] == bound && bound > none) {
+                const int rank = taken + __builtin_popcountll(eq & ((1ull << lane) - 1));
+                if (rank < K) put(i, atomicAdd(&count, 1));
+            }
+            taken += __builtin_popcountll(eq);
+        }
+        __syncthreads();
+        const int C = min(count, BJ_CAP);
+        for (int e = tid; e < C; e += BM_NT) {
+            const uint64_t k = lk[e];
+            const int at = lp[e];
+            int rank = 0;
+            for (int q = 0; q < C; ++q) rank += lk[q] > k || (lk[q] == k && lp[q] < at);
+            if (rank < K) {
+                bk[rank] = k;
+                bt[rank] = lt[e];
+                bb[rank] = lb[e];
+            }
+        }
+        for (int e = C + tid; e < K; e += BM_NT) {
+            bk[e] = none;
+            bt[e] = bb[e] = -1;
+        }
+    }
+    __syncthreads();
+    if (tid < K) {
+        const bool there = bk[tid] > bm_key(-(double)INFINITY);
+        const int64_t at = (int64_t)req * K + tid;
+        p.parent[at] = there ? req * p.n_beam + bb[tid] : -1;
+        p.token[at] = there ? bt[tid] : -1;
+        p.score[at] = there ? (float)bm_value(bk[tid]) : -INFINITY;
+    }
+}
+
+template <typename T>
+static hipError_t run_beam(const BeamSelect &p, hipStream_t stream) {
+    const int rows = p.n_req * p.n_beam;
+    const BmPlan P = bm_plan(rows, p.n_vocab, Bm<T>::per);
+    const int cap = (p.n_out - 1) * P.loads * Bm<T>::per + BM_WAVES * p.n_out;
+    auto kern = P.loads == 16 ? k_beam_rows<T, 16> : P.loads == 8 ? k_beam_rows<T, 8> : P.loads == 4 ? k_beam_rows<T, 4>
+                                                                                                     : k_beam_rows<T, 2>;
+    hipLaunchKernelGGL(kern, dim3(P.n_split, rows), dim3(BM_NT), (size_t)cap * 8, stream, p, P.span, P.n_split, cap);
+    hipLaunchKernelGGL(k_beam_join, dim3(p.n_req), dim3(BM_NT), 0, stream, p, P.n_split);
+    return hipGetLastError();
+}
+hipError_t launch_beam_select(const BeamSelect &p, hipStream_t stream) {
+    switch (p.type) {
+    case TY_F32: return run_beam<float>(p, stream);
+    case TY_F16: return run_beam<_Float16>(p, stream);
+    default: return run_beam<__bf16>(p, stream);
+    }
+}
+
+}  // namespace s2x

@@ -36,17 +36,17 @@ static size_t q4_bytes(int64_t K, int64_t N) {
     return (size_t)round_up_i(round_up_i(K, 128) / 128 * (round_up_i(N, 16) / 16) * (1024 + 128), 256);
 }
 
-static bool type_size(int32_t type, int64_t &size) {
+bool type_size(int32_t type, int64_t &size) {
     size = type == S2X_TYPE_F32 ? 4 : 2;
     return type == S2X_TYPE_F32 || type == S2X_TYPE_F16 || type == S2X_TYPE_BF16;
 }
-static int log2_page(int64_t page) {  // -1: no power of two up to 65,536
+int log2_page(int64_t page) {  // -1: no power of two up to 65,536
     for (int i = 0; i <= 16; ++i)
         if (page == (int64_t)1 << i) return i;
     return -1;
 }
 
-static int check_cache(const s2x_kv_cache *c, KvView &v, const char *who) {
+int check_cache(const s2x_kv_cache *c, KvView &v, const char *who) {
     if (!c) return fail(S2X_ERR_INVALID_ARG, "%s: cache is null", who);
     if (c->type != S2X_TYPE_F16 && c->type != S2X_TYPE_BF16)
         return fail(S2X_ERR_UNSUPPORTED, "%s: cache type %d (F16 or BF16)", who, (int)c->type);

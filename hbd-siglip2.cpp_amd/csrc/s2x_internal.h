@@ -27,6 +27,14 @@ bool aligned(const void *p, size_t a);
 int check_epi(const s2x_epilogue *epi, int64_t N, EpiParams &p);
 int check_q81_planes(const void *qs, const void *ds, int64_t M, const char *who);
 
+// checks shared by the decode step's and the search's entry points: a cache
+// (translated into the kernels' view), an element type's size, a page size's log2
+// (-1: no power of two up to 65,536)
+struct KvView;
+int check_cache(const s2x_kv_cache *c, KvView &v, const char *who);
+bool type_size(int32_t type, int64_t &size);
+int log2_page(int64_t page);
+
 inline int64_t round_up_i(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
 // Planes of a repacked (K_pad, N) weight in one buffer, each at a 256-byte

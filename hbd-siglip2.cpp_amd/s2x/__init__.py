@@ -170,6 +170,17 @@ _sig("s2x_attn_paged", [_p, _i64, ctypes.POINTER(KVCache), _p, _i64, _p, _i64, _
                         _i64, _p, _i32, _i64, _p, _p, _sz, _p])
 _sig("s2x_attn_paged_rows", [_p, _i64, _i64, _p, ctypes.POINTER(KVCache), _p, _i64, _p, _i64, _i64, _i64, _f32,
                              _i64, _p, _i32, _i64, _p, _p, _sz, _p])
+_sig("s2x_add_rmsnorm_quantize_q8_1", [_p, _i32, _i64, _p, _i32, _i64, _i64, _i64, _p, _f32, _p, _i64, _i64, _p, _p, _p,
+                                        _i32, _i64, _p])
+_sig("s2x_beam_select_workspace_size", [_i64, _i64, _i64, _i64], _sz)
+_sig("s2x_beam_select", [_p, _i32, _i64, _i64, _i64, _i64, _p, _p, _i32, _i64, _p, _p, _p, _p, _sz, _p])
+_sig("s2x_kv_pages_workspace_size", [_i64], _sz)
+_sig("s2x_kv_fork", [_p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _sz, _p])
+_sig("s2x_kv_compact", [_p, _p, _i64, _i64, _i64, _i64, _p, _i64, _p, _p, _p, _p, _sz, _p])
+_sig("s2x_kv_copy_pages", [ctypes.POINTER(KVCache), _i64, _p, _p, _p, _i64, _p, _p])
+_sig("s2x_attn_paged_prefix_workspace_size", [_i64, _i64, _i64, _i64, _i64, _i64, _i64], _sz)
+_sig("s2x_attn_paged_prefix", [_p, _i64, _i64, _p, ctypes.POINTER(KVCache), _p, _i64, _p, _i64, _p, _p, _i64, _i64, _i64,
+                               _i64, _i64, _f32, _p, _i32, _i64, _p, _p, _sz, _p])
 _sig("s2x_vision_create", [ctypes.POINTER(VisionWeights), ctypes.POINTER(_p)])
 _sig("s2x_vision_destroy", [_p], None)
 _sig("s2x_vision_set_stream", [_p, _p])

@@ -516,6 +516,134 @@ int s2x_attn_paged_rows(const void *q, int64_t ld_q, int64_t n_row, const int32_
                         float *lse, void *workspace, size_t ws_bytes, void *stream);
 
 /* ------------------------------------------------------------------------ */
+/* Beam search over the paged cache, for the model of the decode step.  No      */
+/* counterpart in the reference.  A step's calls beside those of the decode     */
+/* step: s2x_add_rmsnorm_quantize_q8_1 (between two products),                  */
+/* s2x_attn_paged_prefix (in place of s2x_attn_paged_rows, where sequences      */
+/* share their first tokens), then s2x_beam_select over the logits, s2x_kv_fork */
+/* with its `parent` and s2x_kv_copy_pages.  As in the decode step: the current */
+/* device, no allocation, captured or not; values that only the device knows    */
+/* are checked there; a workspace is the call's own until its work has          */
+/* finished, 256-byte aligned.                                                  */
+/* ------------------------------------------------------------------------ */
+
+/* The residual stream and the next product's activation, one pass over the rows:
+ *   h = x + resid                                  (resid NULL: h = x)
+ *   y = (h * inv) * w,  inv = 1 / sqrt(mean(h^2) + eps)   (w NULL: h * inv)
+ * x: M rows of H in x_type, ld_x apart; resid and h_out (NULL: not written) in
+ * resid_type, F32 or x's type.  h is in f32, and so is what y is taken from; the
+ * mean and inv are computed in f64 and inv rounded once.  Outputs, one or both:
+ * Q8_1 of y as s2x_quantize_q8_1(y, K = H) writes it, bit for bit (qs: M rows of
+ * K_pad int8, 16-byte aligned; ds: M rows of K_pad/32 words; H <= K_pad < H + 32,
+ * columns past H zero), and y itself in y_type.  h_out may be resid or x (same
+ * type and stride); nothing else may overlap.  Rows need only their elements'
+ * alignment (16 bytes are faster).  H <= 32,768, M <= 2^30. */
+int s2x_add_rmsnorm_quantize_q8_1(const void *x, int32_t x_type, int64_t ld_x, const void *resid,
+                                  int32_t resid_type, int64_t ld_resid, int64_t H, int64_t M,
+                                  const float *w, float eps, void *h_out, int64_t ld_h, int64_t K_pad,
+                                  void *qs, void *ds, void *y, int32_t y_type, int64_t ld_y, void *stream);
+
+/* The n_out best continuations of each request.  Request r's beams are rows
+ * r*n_beam .. r*n_beam + n_beam - 1 of logits (rows of n_vocab in `type`, ld
+ * apart) and of scores, their sums of log-probabilities so far.  Token v after
+ * beam b counts
+ *   S = scores[b] + logits[b, v] - log sum_u exp(logits[b, u])
+ * in f64 (the exponentials f32 each, off by some 2^-22); the n_out largest come out
+ * in order, equal ones by the lower beam, then the lower token: parent (the row of
+ * the beam), token, score (S in f32), each n_req x n_out.  A logit of -inf is a
+ * token that cannot follow; the lowest finite value is a value like any other.
+ * done (optional, a byte a beam): not 0, the beam has ended; it is a candidate as it
+ * is, with done_token and its score.  A beam whose score is no finite number is
+ * none (the first step: -inf for all but one), nor has one with a NaN, +inf or no
+ * value above -inf among its logits candidates.  Its logits are not read in the
+ * first two cases.  Where candidates are fewer than n_out the rest are parent and
+ * token -1, score -inf.  Scores are compared as they are, with no regard to
+ * lengths.  n_beam and n_out <= 64, n_req * n_beam <= 65,535, n_vocab <= 2^24.
+ * No output overlaps an input or another one.  workspace of
+ * s2x_beam_select_workspace_size() bytes (0 for shapes that are refused). */
+size_t s2x_beam_select_workspace_size(int64_t n_req, int64_t n_beam, int64_t n_vocab, int64_t n_out);
+int s2x_beam_select(const void *logits, int32_t type, int64_t ld, int64_t n_req, int64_t n_beam,
+                    int64_t n_vocab, const float *scores, const uint8_t *done, int32_t done_token,
+                    int64_t n_out, int32_t *parent, int32_t *token, float *score, void *workspace,
+                    size_t ws_bytes, void *stream);
+
+/* Block tables for the next step: row i of table_out (n_out rows, ld_out >=
+ * ld_table apart) is that of sequence parent[i] (one outside 0 .. n_seq - 1: an empty
+ * one, which is how a sequence is freed), len_out[i] its kv_len.  Entries past its
+ * last page are -1, and so are ids outside 0 .. n_pages - 1.  Rows share the pages
+ * of their parent, but for an open one, the last page of a row where it has room:
+ * the next token of each row must go to a page that no other holds.  Among the rows
+ * whose open page it is the first keeps it, if no row holds it as a page that is
+ * full or not its last and it is not pinned; every other row gets a page of its own
+ * in its place, for s2x_kv_copy_pages to fill:
+ *   copy_src[i], copy_dst[i], copy_tok[i]   of row i: the page to copy, the new one
+ *                 and the places that hold tokens (-1, -1, 0: nothing to copy)
+ *   free_out      the pages that no row of table_out holds, nor pinned (n_pages bytes,
+ *                 optional, not 0: held by others), in order; -1 behind them
+ *                 (n_pages entries, the free_pages of s2x_kv_slots)
+ *   count[0]      pages in free_out, count[1] rows that get a copy
+ * New pages are the lowest free ones (those of rows that are dropped among them; none
+ * is a page to copy).  Where there are fewer than count[1] the last rows that want
+ * one get -1 in copy_dst and in their table, and their last tokens are lost: free
+ * pages first, then call again, as the inputs are as they were.  No output overlaps
+ * an input or another one.  n_seq and n_out <= 8,192, n_pages <= 2^24.  workspace
+ * of s2x_kv_pages_workspace_size() bytes (0 for n_pages that are refused). */
+size_t s2x_kv_pages_workspace_size(int64_t n_pages);
+int s2x_kv_fork(const int32_t *parent, int64_t n_out, const int32_t *kv_len, const int32_t *block_table,
+                int64_t n_seq, int64_t ld_table, int64_t page_size, int64_t n_pages,
+                const uint8_t *pinned, int32_t *table_out, int64_t ld_out, int32_t *len_out,
+                int32_t *copy_src, int32_t *copy_dst, int32_t *copy_tok, int32_t *free_out,
+                int64_t *count, void *workspace, size_t ws_bytes, void *stream);
+
+/* The pages that the tables hold (entries of a row's kv_len tokens, ids outside 0 ..
+ * n_pages - 1 none) moved to ids 0 .. count[0] - 1, with as few copies as that
+ * takes: page copy_src[k] goes to copy_dst[k], k < count[1], both in order, -1
+ * behind them (n_pages / 2 entries each).  No copy_dst is a copy_src, so
+ * s2x_kv_copy_pages does them in any order.  table_out as the tables read then, -1
+ * past a row's last page.  Limits, overlaps and workspace as s2x_kv_fork's. */
+int s2x_kv_compact(const int32_t *kv_len, const int32_t *block_table, int64_t n_seq, int64_t ld_table,
+                   int64_t page_size, int64_t n_pages, int32_t *table_out, int64_t ld_out,
+                   int32_t *copy_src, int32_t *copy_dst, int64_t *count, void *workspace,
+                   size_t ws_bytes, void *stream);
+
+/* Pages src[i] copied to pages dst[i], i < n (and < *n_dev, a number on the device,
+ * unless NULL), keys and values of each of n_cache caches of one layout (a model's
+ * layers; the array is on the host and read before the call returns): the first
+ * n_tok[i] places of each, all where n_tok is NULL.  An id outside 0 .. n_pages - 1
+ * or equal to its partner: nothing is copied.  A page that is a dst is no other
+ * entry's src or dst (its content is not defined otherwise).  n <= 2^24. */
+int s2x_kv_copy_pages(const s2x_kv_cache *caches, int64_t n_cache, const int32_t *src,
+                      const int32_t *dst, const int32_t *n_tok, int64_t n, const int64_t *n_dev,
+                      void *stream);
+
+/* s2x_attn_paged_rows without a window, for sequences in groups that share their
+ * first tokens: group g is sequences group_start[g] .. group_start[g + 1] - 1
+ * (n_group + 1 ascending entries on the device), whose tokens before prefix_len[g]
+ * are the same.  Their keys and values are read once for the whole group, from the
+ * pages of its first sequence; what the other rows of block_table have there is not
+ * looked at.  Sequence s sees the first kv_len[s] tokens as ever: fewer than the
+ * prefix, and it sees that much of it.  tok_start as in s2x_attn_paged_rows, or
+ * NULL: row s of q is sequence s's.  A prefix counts as at most max_prefix tokens
+ * (the others are its sequences' own), a sequence's own tokens as the first max_own
+ * behind it, a group as its first max_group sequences; sequences of no group, or
+ * past those, are left out, their rows as they were.  Probabilities and sums as in
+ * s2x_attn_paged, the order of the sums another.  n_group * max_group <= 65,535,
+ * max_prefix and max_own <= 2^30, n_group * max_group * n_head of the cache <= 2^21
+ * (a key head counted once for each 16 query heads on it).  workspace of
+ * s2x_attn_paged_prefix_workspace_size() bytes (0 for shapes that are refused, and
+ * for no sequences). */
+size_t s2x_attn_paged_prefix_workspace_size(int64_t n_group, int64_t max_group, int64_t max_prefix,
+                                            int64_t max_own, int64_t n_q_head, int64_t n_kv_head,
+                                            int64_t d_head);
+int s2x_attn_paged_prefix(const void *q, int64_t ld_q, int64_t n_row, const int32_t *tok_start,
+                          const s2x_kv_cache *cache, const int32_t *block_table, int64_t ld_table,
+                          const int32_t *kv_len, int64_t n_seq, const int32_t *group_start,
+                          const int32_t *prefix_len, int64_t n_group, int64_t max_group,
+                          int64_t max_prefix, int64_t max_own, int64_t n_q_head, float scale, void *out,
+                          int32_t out_type, int64_t ld_out, float *lse, void *workspace,
+                          size_t ws_bytes, void *stream);
+
+/* ------------------------------------------------------------------------ */
 /* a10  encoders (replace siglip2::VisionEncoder / TextEncoder,               */
 /* src/siglip2_vision.h:37-68, src/siglip2_text.h:25-75).                     */
 /* Weights come from host memory: raw Q8_0 blocks for every matrix, f32 for  */
