@@ -25,27 +25,54 @@ constexpr int BM_NT = 256, BM_WAVES = BM_NT / WAVE;
 
 template <typename T> struct Bm;
 // per: values of a lane's 16-byte load; low: bits at the end of an f32 that a value
-// of the type leaves 0
+// of the type leaves 0; largest(): of a load's values, in pairs where the type has
+// them, right if it is positive (always: exact)
 template <> struct Bm<float> {
     static constexpr int per = 4, low = 0;
+    static constexpr bool exact = true;
     typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
     static __device__ __forceinline__ float at(const v4u &r, int j) {
         const uint32_t u = r[j];  // (a cast of r[j] itself takes r[0])
         return __builtin_bit_cast(float, u);
     }
+    static __device__ __forceinline__ float largest(const v4u &r) {
+        return fmaxf(fmaxf(at(r, 0), at(r, 1)), fmaxf(at(r, 2), at(r, 3)));
+    }
 };
 template <> struct Bm<_Float16> {
     static constexpr int per = 8, low = 13;
+    static constexpr bool exact = true;
     typedef _Float16 vec __attribute__((ext_vector_type(8), aligned(2)));
+    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
     static __device__ __forceinline__ float at(const v4u &r, int j) {
         return f16_bits_to_f32((uint16_t)(j & 1 ? r[j / 2] >> 16 : r[j / 2]));
+    }
+    static __device__ __forceinline__ float largest(const v4u &r) {
+        uint32_t m = r[0];
+#pragma unroll
+        for (int i = 1; i < 4; ++i) {
+            const uint32_t x = r[i];
+            asm("v_pk_max_f16 %0, %0, %1" : "+v"(m) : "v"(x));  // (the builtin quiets its operands first)
+        }
+        const v2 h = __builtin_bit_cast(v2, m);
+        return fmaxf((float)h[0], (float)h[1]);
     }
 };
 template <> struct Bm<__bf16> {
     static constexpr int per = 8, low = 16;
+    static constexpr bool exact = false;
     typedef __bf16 vec __attribute__((ext_vector_type(8), aligned(2)));
+    typedef short v2 __attribute__((ext_vector_type(2)));
     static __device__ __forceinline__ float at(const v4u &r, int j) {
         return __builtin_bit_cast(float, j & 1 ? r[j / 2] & 0xffff0000u : r[j / 2] << 16);
+    }
+    // as integers: positive values in order, above all negative ones
+    static __device__ __forceinline__ float largest(const v4u &r) {
+        const uint32_t a = r[0], b = r[1], c = r[2], d = r[3];
+        const v2 m = __builtin_elementwise_max(__builtin_elementwise_max(__builtin_bit_cast(v2, a), __builtin_bit_cast(v2, b)),
+                                               __builtin_elementwise_max(__builtin_bit_cast(v2, c), __builtin_bit_cast(v2, d)));
+        const uint32_t u = __builtin_bit_cast(uint32_t, m);
+        return fmaxf(__builtin_bit_cast(float, u << 16), __builtin_bit_cast(float, u & 0xffff0000u));
     }
 };
 
@@ -87,6 +114,17 @@ __device__ __forceinline__ float bm_exp(float x) {
 }
 // what a sum relative to `from` counts relative to `to` >= from (-inf: an empty sum)
 __device__ __forceinline__ float bm_scale(float from, float to) { return from == -INFINITY ? 0.0f : bm_exp(from - to); }
+
+// How many of a list's C members are ahead of member e, counted by a quad (its lanes
+// have the same e); ahead(q): whether member q is.
+template <typename F>
+__device__ __forceinline__ int bm_rank(int C, F ahead) {
+    int n = 0;
+#pragma unroll 4
+    for (int q = threadIdx.x & 3; q < C; q += 4) n += ahead(q);
+    n += dpp_i<0xb1>(n);
+    return n + dpp_i<0x4e>(n);
+}
 
 // Workspace: candidates [row][split][K] (value, token; token -1: none), then the
 // sums [row][split] of 2^(x log2 e - top) and their tops.
@@ -159,21 +197,43 @@ __global__ __launch_bounds__(BM_NT) void k_beam_rows(BeamSelect p, int span, int
         }
     }
     float mi[NL], top = -INFINITY;
+    auto each_value = [&]() {  // mi and top from the values one by one
+        top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            mi[i] = Bm<T>::at(r[i], 0);
+#pragma unroll
+            for (int j = 1; j < PER; ++j) mi[i] = fmaxf(mi[i], Bm<T>::at(r[i], j));
+            top = fmaxf(top, mi[i]);
+        }
+    };
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-        mi[i] = Bm<T>::at(r[i], 0);
-#pragma unroll
-        for (int j = 1; j < PER; ++j) mi[i] = fmaxf(mi[i], Bm<T>::at(r[i], j));
+        mi[i] = Bm<T>::largest(r[i]);
         top = fmaxf(top, mi[i]);
     }
+    if (!Bm<T>::exact && __builtin_amdgcn_ballot_w64(!(top > 0.0f)) != 0) each_value();
     tops[tid] = top;
-    // the sum relative to the lane's largest, log2(e) as a head and a tail
-    const float ref = top == -INFINITY ? 0.0f : top;
+    // the sum relative to the lane's largest.  2^(x L - c), c the rounded top L, with
+    // what L lacks of log2(e) and c of top L made up for in the sum: right where x is
+    // near top, and off by 2^-26 of top - x below.  Past 4,096 c lacks too much:
+    // there by differences.
+    const float L = 1.44269502e+00f, LT = 1.92596299e-08f, c = top * L;
     float sum = 0.0f;
+    if (__builtin_amdgcn_ballot_w64(fabsf(top) > 4096.0f && top != -INFINITY) == 0) {
+        const float ref = top == -INFINITY ? 0.0f : c;
 #pragma unroll
-    for (int i = 0; i < NL; ++i)
+        for (int i = 0; i < NL; ++i)
 #pragma unroll
-        for (int j = 0; j < PER; ++j) sum = sum + bm_exp(Bm<T>::at(r[i], j) - ref);
+            for (int j = 0; j < PER; ++j) sum = sum + __builtin_amdgcn_exp2f(fmaf(Bm<T>::at(r[i], j), L, -ref));
+        if (top != -INFINITY) sum = sum * __builtin_amdgcn_exp2f(fmaf(-top, LT, fmaf(-top, L, c)));
+    } else {
+        const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+#pragma unroll
+            for (int j = 0; j < PER; ++j) sum = sum + bm_exp(Bm<T>::at(r[i], j) - ref);
+    }
     {
         const float wt = group_max<64>(top);
         const double ws = wave_dsum((double)sum * (double)bm_scale(top, wt));
@@ -189,6 +249,7 @@ __global__ __launch_bounds__(BM_NT) void k_beam_rows(BeamSelect p, int span, int
     const float bound = bm_value(bm_kth(k4, K, Bm<T>::low));
 
     // values above the bound, then the wave's first K equal to it
+    if (!Bm<T>::exact && !(bound > 0.0f)) each_value();  // (uniform)
     auto put = [&](float v, int c, int at) { list[at] = (uint64_t)bm_key(v) << 32 | (uint32_t)~c; };
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
@@ -227,11 +288,10 @@ __global__ __launch_bounds__(BM_NT) void k_beam_rows(BeamSelect p, int span, int
     const int C = min(count, cap);
     const int64_t part = (int64_t)row * n_split + split;
     BmCand *out = bm_cands(p, n_split) + part * K;
-    for (int e = tid; e < C; e += BM_NT) {
+    for (int e = tid >> 2; e < C; e += BM_NT / 4) {
         const uint64_t k = list[e];
-        int rank = 0;
-        for (int q = 0; q < C; ++q) rank += list[q] > k;
-        if (rank < K) out[rank] = BmCand{bm_value((uint32_t)(k >> 32)), from + (int)~(uint32_t)k};
+        const int rank = bm_rank(C, [&](int q) { return list[q] > k; });
+        if (rank < K && (tid & 3) == 0) out[rank] = BmCand{bm_value((uint32_t)(k >> 32)), from + (int)~(uint32_t)k};
     }
     for (int e = C + tid; e < K; e += BM_NT) out[e] = BmCand{-INFINITY, -1};
     if (tid == 0) {
@@ -246,7 +306,8 @@ __global__ __launch_bounds__(BM_NT) void k_beam_rows(BeamSelect p, int span, int
 }
 
 constexpr int BJ_PER = 8, BJ_TILE = BM_NT * BJ_PER;  // candidates of a round
-constexpr int BJ_CAP = (BEAM_MAX_OUT - 1) * (BJ_PER + 1) + BM_WAVES * BEAM_MAX_OUT;
+constexpr int BJ_CAP = 1024, BJ_SUMS = 1024;         // members of a list, sums kept in LDS
+static_assert((BEAM_MAX_OUT - 1) * (BJ_PER + 1) + BM_WAVES * BEAM_MAX_OUT <= BJ_CAP, "the list's largest length");
 
 __global__ __launch_bounds__(BM_NT) void k_beam_join(BeamSelect p, int n_split) {
     __shared__ double add[BEAM_MAX_OUT];  // score - lse of the beams; -inf: none
@@ -255,67 +316,86 @@ __global__ __launch_bounds__(BM_NT) void k_beam_join(BeamSelect p, int n_split) 
     __shared__ int32_t lp[BJ_CAP], lt[BJ_CAP], lb[BJ_CAP];
     __shared__ uint64_t bk[BEAM_MAX_OUT];  // the best so far, in order
     __shared__ int32_t bt[BEAM_MAX_OUT], bb[BEAM_MAX_OUT];
-    __shared__ int count;
+    __shared__ BmSum ls[BJ_SUMS];
+    __shared__ int count, ties;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, req = blockIdx.x, K = p.n_out;
-    const BmSum *sums = bm_sums(p);
-    const BmCand *cands = bm_cands(p, n_split);
+    const BmSum *sums = bm_sums(p) + (int64_t)req * p.n_beam * n_split;
+    const BmCand *cands = bm_cands(p, n_split) + (int64_t)req * p.n_beam * n_split * K;
+    const int per_beam = n_split * K, all = p.n_beam * per_beam, n_sum = p.n_beam * n_split;
+    // all loads that wait for nothing: the sums (of beams that have none: whatever
+    // is there, not used), the first round's candidates
+    const bool kept = n_sum <= BJ_SUMS;
+    if (kept)
+        for (int i = tid; i < n_sum; i += BM_NT) ls[i] = sums[i];
+    BmCand first[BJ_PER];
+#pragma unroll
+    for (int i = 0; i < BJ_PER; ++i) first[i] = cands[min(i * BM_NT + tid, all - 1)];
+    if (tid < p.n_beam) state[tid] = bm_state(p, req * p.n_beam + tid);
+    if (tid < K) {
+        bk[tid] = bm_key(-(double)INFINITY);
+        bt[tid] = bb[tid] = -1;
+    }
+    __syncthreads();
     for (int b = wave; b < p.n_beam; b += BM_WAVES) {
-        const int row = req * p.n_beam + b, st = bm_state(p, row);
+        const int st = state[b];
+        const BmSum *from = kept ? ls + b * n_split : sums + (int64_t)b * n_split;
         float top = -INFINITY;
         double s = 0.0;
         if (st == 1) {
-            for (int i = lane; i < n_split; i += WAVE) top = fmaxf(top, sums[(int64_t)row * n_split + i].top);
+            for (int i = lane; i < n_split; i += WAVE) top = fmaxf(top, from[i].top);
             top = group_max<64>(top);
             for (int i = lane; i < n_split; i += WAVE) {
-                const BmSum q = sums[(int64_t)row * n_split + i];
+                const BmSum q = from[i];
                 s += q.sum * (double)bm_scale(q.top, top);
             }
             s = wave_dsum(s);
         }
         if (lane == 0) {
             // (no finite sum, from a NaN or an infinity, and no value at all: no candidates)
-            const double lse = log(s) + (double)top;
-            state[b] = st;
-            add[b] = st == 2 ? (double)p.scores[row] : st == 1 && fabs(lse) < INFINITY ? (double)p.scores[row] - lse : -INFINITY;
+            const double score = (double)p.scores[req * p.n_beam + b], lse = log(s) + (double)top;
+            add[b] = st == 2 ? score : st == 1 && fabs(lse) < INFINITY ? score - lse : -INFINITY;
         }
     }
-    if (tid < K) {
-        bk[tid] = bm_key(-(double)INFINITY);
-        bt[tid] = bb[tid] = -1;
-    }
-    const int per_beam = n_split * K, all = p.n_beam * per_beam;
+    const int step_b = BM_NT / per_beam, step_r = BM_NT - step_b * per_beam;
     for (int e0 = 0; e0 < all; e0 += BJ_TILE) {
         __syncthreads();
-        if (tid == 0) count = 0;
+        if (tid == 0) count = ties = 0;
         // this round's candidates, and the best of those before as places below
         // all of them
+        const uint64_t none = bm_key(-(double)INFINITY);
         uint64_t key[BJ_PER + 1];
         int32_t tok[BJ_PER + 1];
         int beam[BJ_PER + 1];
+        key[0] = none;
+        tok[0] = beam[0] = -1;
+        if (tid < K) {
+            key[0] = bk[tid];
+            tok[0] = bt[tid];
+            beam[0] = bb[tid];
+        }
+        int b = (e0 + tid) / per_beam, rest = e0 + tid - b * per_beam;
 #pragma unroll
-        for (int i = 0; i <= BJ_PER; ++i) {
-            key[i] = bm_key(-(double)INFINITY);
-            tok[i] = -1;
-            beam[i] = -1;
-            if (i == 0) {
-                if (tid < K) {
-                    key[0] = bk[tid];
-                    tok[0] = bt[tid];
-                    beam[0] = bb[tid];
+        for (int i = 1; i <= BJ_PER; ++i) {
+            if (i > 1) {
+                b += step_b;
+                rest += step_r;
+                if (rest >= per_beam) {
+                    rest -= per_beam;
+                    ++b;
                 }
-                continue;
             }
+            key[i] = none;
+            tok[i] = beam[i] = -1;
             const int e = e0 + (i - 1) * BM_NT + tid;
             if (e >= all) continue;
-            const int b = e / per_beam, rest = e - b * per_beam;
             beam[i] = b;
             if (state[b] == 2) {
                 if (rest == 0) {
                     key[i] = bm_key(add[b]);
                     tok[i] = p.done_token;
                 }
-            } else if (state[b] == 1 && add[b] > -INFINITY) {
-                const BmCand c = cands[((int64_t)req * p.n_beam + b) * per_beam + rest];
+            } else if (add[b] > -INFINITY) {
+                const BmCand c = e0 ? cands[e] : first[i - 1];
                 if (c.token >= 0) key[i] = bm_key(add[b] + (double)c.x);
                 tok[i] = c.token;
             }
@@ -325,35 +405,52 @@ __global__ __launch_bounds__(BM_NT) void k_beam_join(BeamSelect p, int n_split) 
         for (int i = 1; i <= BJ_PER; ++i) top = max(top, key[i]);
         tops[tid] = top;
         __syncthreads();
+        // a bound by the upper halves of the keys first: enough unless more keys
+        // than the list takes share the bound's (many equal scores), then by whole keys
         uint64_t k4[4];
+        uint32_t h4[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) k4[i] = tops[i * WAVE + lane];
-        const uint64_t none = bm_key(-(double)INFINITY), bound = bm_kth(k4, K, 0);
-        auto put = [&](int i, int at) {
+        for (int i = 0; i < 4; ++i) {
+            k4[i] = tops[i * WAVE + lane];
+            h4[i] = (uint32_t)(k4[i] >> 32);
+        }
+        const uint32_t hb = bm_kth(h4, K, 0);
+        auto put = [&](int i) {
+            const int at = atomicAdd(&count, 1);
             lk[at] = key[i];
             lp[at] = i * BM_NT + tid;
             lt[at] = tok[i];
             lb[at] = beam[i];
         };
-        int taken = 0;
+        int eq = 0;
 #pragma unroll
-        for (int i = 0; i <= BJ_PER; ++i) {
-            if (key[i] > bound) put(i, atomicAdd(&count, 1));
-            const uint64_t eq = __builtin_amdgcn_ballot_w64(key[i] == bound && bound > none);
-            if (key[i] == bound && bound > none) {
-                const int rank = taken + __builtin_popcountll(eq & ((1ull << lane) - 1));
-                if (rank < K) put(i, atomicAdd(&count, 1));
+        for (int i = 0; i <= BJ_PER; ++i) eq += (uint32_t)(key[i] >> 32) == hb && key[i] > none;
+        eq = group_isum<64>(eq);
+        if (lane == 0 && eq) atomicAdd(&ties, eq);
+        __syncthreads();
+        if (ties <= BJ_CAP - (BEAM_MAX_OUT - 1) * (BJ_PER + 1)) {  // (uniform)
+#pragma unroll
+            for (int i = 0; i <= BJ_PER; ++i)
+                if ((uint32_t)(key[i] >> 32) >= hb && key[i] > none) put(i);
+        } else {
+            const uint64_t bound = bm_kth(k4, K, 0);
+            int taken = 0;
+#pragma unroll
+            for (int i = 0; i <= BJ_PER; ++i) {
+                if (key[i] > bound) put(i);
+                const bool is = key[i] == bound && bound > none;
+                const uint64_t m = __builtin_amdgcn_ballot_w64(is);
+                if (is && taken + __builtin_popcountll(m & ((1ull << lane) - 1)) < K) put(i);
+                taken += __builtin_popcountll(m);
             }
-            taken += __builtin_popcountll(eq);
         }
         __syncthreads();
         const int C = min(count, BJ_CAP);
-        for (int e = tid; e < C; e += BM_NT) {
+        for (int e = tid >> 2; e < C; e += BM_NT / 4) {
             const uint64_t k = lk[e];
             const int at = lp[e];
-            int rank = 0;
-            for (int q = 0; q < C; ++q) rank += lk[q] > k || (lk[q] == k && lp[q] < at);
-            if (rank < K) {
+            const int rank = bm_rank(C, [&](int q) { return lk[q] > k || (lk[q] == k && lp[q] < at); });
+            if (rank < K && (tid & 3) == 0) {
                 bk[rank] = k;
                 bt[rank] = lt[e];
                 bb[rank] = lb[e];

@@ -102,6 +102,23 @@ __device__ __forceinline__ PaGroup pa_group(const AttnPrefix &p, int g) {
     r.len = min((int64_t)min(max(p.prefix_len[g], 0), p.max_prefix), p.a.ld_table << p.a.kv.page_shift);
     return r;
 }
+// The last group that begins at or before sequence s (starts ascend; none: the
+// first), and where it begins: each lane of the wave looks at one of 64 parts of
+// the groups left, until one is.
+__device__ __forceinline__ int pa_find(const AttnPrefix &p, int s, int &first) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = p.n_group;
+    for (;;) {
+        const int step = (n + 63) / 64;
+        const int at = p.group_start[lo + min(lane * step, n - 1)];
+        const int k = max(__builtin_popcountll(__builtin_amdgcn_ballot_w64(lane * step < n && at <= s)) - 1, 0);
+        lo += k * step;
+        n = min(step, n - k * step);
+        if (n > 1) continue;
+        first = __shfl(at, k);
+        return lo;
+    }
+}
 // tokens of sequence s (its table's, at most)
 __device__ __forceinline__ int64_t pa_len(const AttnPaged &p, int s) {
     return min((int64_t)max(p.kv_len[s], 0), p.ld_table << p.kv.page_shift);
@@ -127,11 +144,37 @@ enum PaMode { PA_ROWS, PA_PACKED, PA_PREFIX, PA_OWN };
 __device__ __forceinline__ const AttnPaged &pa_base(const AttnPaged &p) { return p; }
 __device__ __forceinline__ const AttnPaged &pa_base(const AttnPrefix &p) { return p.a; }
 
+// Workgroup (or wave) bid -> (unit, chunk), head.  Workgroups go round the 8 XCDs: the
+// heads of one chunk follow each other on one XCD (a token-major row's
+// cache lines are shared between heads), and the chunks of a sequence
+// lie on different ones (u = chunk n_seq + (s + chunk) % n_seq), since
+// ragged sequences leave the later chunks empty.
+struct PaWork {
+    int unit, split, hp;
+};
+__device__ __forceinline__ PaWork pa_work(int bid, int n_unit, int n_split, int H) {
+    const int U = n_unit * n_split, octs = U / 8 * 8;
+    PaWork w;
+    int u;
+    if (bid < octs * H) {
+        const int q8 = bid / 8, o = q8 / H;
+        u = 8 * o + bid % 8;
+        w.hp = q8 - o * H;
+    } else {
+        const int b = bid - octs * H;
+        w.hp = b / (U - octs);
+        u = octs + b - w.hp * (U - octs);
+    }
+    w.split = u / n_unit;
+    w.unit = (u - w.split * n_unit + w.split) % n_unit;
+    return w;
+}
+
 // DC: 32-value chunks of a head; EXACT: d_head = 32 DC; KT: 16-key parts of a
-// tile; NW: waves of a workgroup.  PREFIX, OWN: parts of this launch are n_split
-// of the n_parts that a row of the workspace has, from part0 on.
+// tile; NW: waves of a workgroup.  w: what it does of its form's n_split chunks (of
+// the n_parts that a row of the workspace has, from part0 on: PREFIX, OWN).
 template <typename TC, int DC, bool EXACT, int KT, int NW, PaMode MODE, typename ARGS>
-__device__ __forceinline__ void pa_body(const ARGS &args, int chunk, int n_split, int n_parts, int part0) {
+__device__ __forceinline__ void pa_body(const ARGS &args, const PaWork &w, int chunk, int n_split, int n_parts, int part0) {
     constexpr bool PACKED = MODE == PA_PACKED, GROUPS = MODE == PA_PREFIX || MODE == PA_OWN;
     const AttnPaged &p = pa_base(args);
     typedef typename Pa<TC>::vec vec;
@@ -139,40 +182,23 @@ __device__ __forceinline__ void pa_body(const ARGS &args, int chunk, int n_split
     constexpr int TILE = 16 * KT, STEP = NW * TILE, NT = NW * WAVE, NP = Pa<TC>::terms;
     extern __shared__ __align__(16) uint8_t lds[];  // V tiles of the waves, then their sums
     __shared__ float ml[NW][2][16];
-    const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // (one wave: it may be any of its workgroup, with a part of LDS of its own)
+    const int place = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = NW == 1 ? 0 : place;
+    const int tid = NW == 1 ? threadIdx.x & 63 : threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int d = EXACT ? DP : p.kv.d_head, nch = d / 8;
-    const int group = p.n_q_head / p.kv.n_head, parts = MODE == PA_PREFIX ? 1 : (group + 15) / 16, H = p.kv.n_head * parts;
-    int n_unit = p.n_seq;
-    if constexpr (MODE == PA_PREFIX) n_unit = args.n_group;
-    if constexpr (MODE == PA_OWN) n_unit = args.n_group * args.max_group;
-    // Workgroup -> (sequence, chunk), head.  Workgroups go round the 8 XCDs: the
-    // heads of one chunk follow each other on one XCD (a token-major row's
-    // cache lines are shared between heads), and the chunks of a sequence
-    // lie on different ones (u = chunk n_seq + (s + chunk) % n_seq), since
-    // ragged sequences leave the later chunks empty.
-    const int U = n_unit * n_split, octs = U / 8 * 8;
-    int u, hp;
-    if ((int)blockIdx.x < octs * H) {
-        const int q8 = blockIdx.x / 8, o = q8 / H;
-        u = 8 * o + blockIdx.x % 8;
-        hp = q8 - o * H;
-    } else {
-        const int b = blockIdx.x - octs * H;
-        hp = b / (U - octs);
-        u = octs + b - hp * (U - octs);
-    }
-    const int split = u / n_unit, unit = (u - split * n_unit + split) % n_unit;
-    const int hk = hp / parts, h0 = hk * group + (hp - hk * parts) * 16;
-    int s = unit, R = min(16, (hk + 1) * group - h0);
+    const int group = p.n_q_head / p.kv.n_head, parts = MODE == PA_PREFIX ? 1 : (group + 15) / 16;
+    const int hk = w.hp / parts, h0 = hk * group + (w.hp - hk * parts) * 16, split = w.split;
+    int s = w.unit, R = min(16, (hk + 1) * group - h0), slot = 0;
     PaRange kr;
     PaGroup gr = {};
     if constexpr (GROUPS) {
-        const int g = MODE == PA_OWN ? unit / args.max_group : unit, i = MODE == PA_OWN ? unit - g * args.max_group : 0;
-        gr = pa_group(args, g);
-        if (i >= gr.size) return;  // (uniform)
-        s = gr.first + i;
+        int first;
+        const int gi = MODE == PA_OWN ? pa_find(args, s, first) : w.unit;
+        gr = pa_group(args, gi);
+        slot = gi * args.max_group + (MODE == PA_OWN ? s - gr.first : 0);
+        if (MODE == PA_OWN ? s < gr.first || s >= gr.first + gr.size : gr.size == 0) return;  // (uniform)
         if constexpr (MODE == PA_PREFIX) {
+            s = gr.first;
             R = gr.size * group;
             kr = PaRange{0, gr.len, 0};
         } else {
@@ -201,7 +227,7 @@ __device__ __forceinline__ void pa_body(const ARGS &args, int chunk, int n_split
     const TC *kp = (const TC *)p.kv.k + hk * p.kv.ld_head, *vp = (const TC *)p.kv.v + hk * p.kv.ld_head;
     const int32_t *row = p.table + s * p.ld_table;
     const uint32_t pmask = (1u << p.kv.page_shift) - 1, ldp = (uint32_t)p.kv.ld_page, ldt = (uint32_t)p.kv.ld_tok;
-    TC *vl = reinterpret_cast<TC *>(lds) + wave * TILE * d;
+    TC *vl = reinterpret_cast<TC *>(lds) + place * TILE * d;
 
     vec q[DC];
 #pragma unroll
@@ -369,6 +395,19 @@ __device__ __forceinline__ void pa_body(const ARGS &args, int chunk, int n_split
     // join the waves: o[i] is values 16 i + 4 g .. + 3 of head r
     l = l + __shfl_xor(l, 16);
     l = l + __shfl_xor(l, 32);
+    if constexpr (NW == 1) {  // (nothing to join; a form that leaves its sums)
+        if (r >= R) return;
+        const int64_t at = ((int64_t)slot * p.n_q_head + h0 + r) * n_parts + part0 + split;
+        float *ws = (float *)p.ws;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+            if (!EXACT && 16 * i + 4 * g >= d) break;
+            reinterpret_cast<v4f *>(ws)[at * (nch * 2) + 4 * i + g] = o[i];
+        }
+        if (g == 0)
+            reinterpret_cast<float2 *>(ws + (int64_t)args.n_group * args.max_group * p.n_q_head * n_parts * d)[at] = make_float2(m, l);
+        return;
+    }
     float *ol = reinterpret_cast<float *>(lds);  // [wave][head < R][DP + 4]
     __syncthreads();
     if (r < R) {
@@ -399,8 +438,8 @@ __device__ __forceinline__ void pa_body(const ARGS &args, int chunk, int n_split
         }
         if constexpr (GROUPS) {
             // (a column's slot: its group's place and its own in it)
-            const int slot = MODE == PA_OWN ? unit : unit * args.max_group + h / group;
-            const int64_t at = ((int64_t)slot * p.n_q_head + (MODE == PA_OWN ? h0 + h : hk * group + h % group)) * n_parts + part0 + split;
+            const int64_t at = ((int64_t)(slot + (MODE == PA_OWN ? 0 : h / group)) * p.n_q_head +
+                                (MODE == PA_OWN ? h0 + h : hk * group + h % group)) * n_parts + part0 + split;
             float *ws = (float *)p.ws;
             reinterpret_cast<v4f *>(ws)[at * (nch * 2) + e] = a;
             if (e == 0)

@@ -31,7 +31,8 @@ constexpr int PJ_NT = 256;  // threads of the join
 // PACKED: rows by tok_start
 template <typename TC, int DC, bool EXACT, int KT, int NW, bool PACKED>
 __global__ __launch_bounds__(NW * WAVE) void k_attn_paged(AttnPaged p, int chunk, int n_split) {
-    pa_body<TC, DC, EXACT, KT, NW, PACKED ? PA_PACKED : PA_ROWS>(p, chunk, n_split, n_split, 0);
+    const PaWork w = pa_work(blockIdx.x, p.n_seq, n_split, p.kv.n_head * ((p.n_q_head / p.kv.n_head + 15) / 16));
+    pa_body<TC, DC, EXACT, KT, NW, PACKED ? PA_PACKED : PA_ROWS>(p, w, chunk, n_split, n_split, 0);
 }
 
 // Chunks of a sequence joined: a workgroup per query head and 4 LANES values of

@@ -13,38 +13,90 @@
 
 namespace s2x {
 
-template <typename TC, int DC, bool EXACT, int KT, int NW, PaMode MODE>
-__global__ __launch_bounds__(NW * WAVE) void k_attn_group(AttnPrefix p, int chunk, int n_split, int n_parts, int part0) {
-    pa_body<TC, DC, EXACT, KT, NW, MODE>(p, chunk, n_split, n_parts, part0);
+// Parts of a launch: the prefixes' in chunks of chunk_p, then the own tokens'.
+struct PxPlan {
+    int     nc, tiles;  // of the prefix; nc 0: the form of up to 16 columns
+    int     chunk_p, split_p, chunk_o, split_o;
+    int64_t wgs_p, wgs_o;
+    __host__ __device__ int parts() const { return split_p + split_o; }
+};
+
+// Own tokens: a wave a sequence, key head and chunk (of few keys, mostly: four waves
+// on one would be tiles of which some have none).  The four of a workgroup are
+// neighbours in the order of workgroups of its XCD.
+template <typename TC, int DC, bool EXACT, int KT>
+__device__ __forceinline__ void px_own(const AttnPrefix &p, const PxPlan &P) {
+    const int w = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int H = p.a.kv.n_head * ((p.a.n_q_head / p.a.kv.n_head + 15) / 16);
+    for (int bid = w / 8 * 32 + wave * 8 + w % 8; bid < p.a.n_seq * P.split_o * H; bid += (int)P.wgs_o * 4)
+        pa_body<TC, DC, EXACT, KT, 1, PA_OWN>(p, pa_work(bid, p.a.n_seq, P.split_o, H), P.chunk_o, P.split_o, P.parts(), P.split_p);
 }
 
-constexpr int PX_TK = 64;  // keys of a tile
-constexpr int PX_PAD_K = 8, PX_PAD_V = 16;  // rows in LDS end with these: reads of 16 rows spread over the banks
+// A workgroup's part of the prefixes: the tiles of columns, then the heads, of one
+// chunk follow each other on one XCD.
+struct PxWork {
+    int tile, hk, group, split;
+};
+__device__ __forceinline__ PxWork px_work(const AttnPrefix &p, const PxPlan &P) {
+    int u = xcd_linear(blockIdx.x - (int)P.wgs_o, (int)P.wgs_p);  // (wgs_o: a multiple of 8)
+    PxWork w;
+    w.tile = u % P.tiles;
+    u /= P.tiles;
+    w.hk = u % p.a.kv.n_head;
+    u /= p.a.kv.n_head;
+    w.group = u % p.n_group;
+    w.split = u / p.n_group;
+    return w;
+}
 
-// DC, EXACT as in s2x_paged.h; NC: 16-column parts of a wave; NW: waves.
-// A step: the next tile's pieces into registers, the products of this one, the
-// pieces into the other half of LDS, one barrier.  S^T and O^T as in s2x_paged.h.
-template <typename TC, int DC, bool EXACT, int NC, int NW>
-__global__ __launch_bounds__(NW * WAVE) void k_attn_prefix(AttnPrefix args, int chunk, int n_split, int n_parts, int tiles) {
+constexpr int PX_TK = 32, PX_NT = 4 * WAVE;  // keys of a tile, threads
+constexpr int PX_PAD_K = 8, PX_PAD_V = 16;   // rows in LDS end with these: reads of 16 rows spread over the banks
+
+// The reference of a column's exponentials follows its largest score in steps: it
+// moves once that is PX_ROOM (as a power of two) above, so that few tiles rescale
+// the sums.  A probability is up to 2^PX_ROOM then, times 2^px_up for f16, whose
+// second term reaches 2^-35 of the largest; the sums leave as Pa::up has them.
+constexpr float PX_ROOM = 4.0f;
+template <typename TC> constexpr float px_up = 0.0f;
+template <> constexpr float px_up<_Float16> = 11.0f;
+
+// Two probabilities (times 2^px_up) as sums of terms of the cache's type: bf16 by
+// cutting off, which leaves nothing after three; f16 by rounding.
+__device__ __forceinline__ void px_terms(float x, float y, uint32_t (&t)[2]) {
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+    const v2h h = __builtin_convertvector((v2f{f32_materialize(x), f32_materialize(y)}), v2h);
+    const v2f r = {fmaf((float)h[0], -1.0f, x), fmaf((float)h[1], -1.0f, y)};
+    t[0] = __builtin_bit_cast(uint32_t, h);
+    t[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, v2h));
+}
+__device__ __forceinline__ void px_terms(float x, float y, uint32_t (&t)[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const uint32_t a = __builtin_bit_cast(uint32_t, x), b = __builtin_bit_cast(uint32_t, y);
+        t[i] = __builtin_amdgcn_perm(b, a, 0x07060302);  // the upper halves
+        x = x - __builtin_bit_cast(float, a & 0xffff0000u);
+        y = y - __builtin_bit_cast(float, b & 0xffff0000u);
+    }
+}
+
+// NC: 16-column parts of a wave.  A step: the next tile's pieces into registers,
+// the products of this one, the pieces into the other half of LDS, one barrier.
+// S^T and O^T as in s2x_paged.h.
+template <typename TC, int DC, bool EXACT, int NC>
+__device__ __forceinline__ void px_wide(const AttnPrefix &args, const PxPlan &P, const PxWork &w, const PaGroup &gr) {
     typedef typename Pa<TC>::vec vec;
-    constexpr int DP = 32 * DC, DT = 2 * DC, NT = NW * WAVE, NP = Pa<TC>::terms;
+    constexpr int DP = 32 * DC, DT = 2 * DC, NT = PX_NT, NP = Pa<TC>::terms;
     constexpr int PER = (PX_TK * (DP / 8) + NT - 1) / NT;  // pieces of a thread
+    constexpr bool ALL = EXACT && PX_TK * (DP / 8) % NT == 0;  // all of them there
     extern __shared__ __align__(16) uint8_t lds[];
     const AttnPaged &p = args.a;
     const int tid = threadIdx.x, lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int d = EXACT ? DP : p.kv.d_head, nch = d / 8, sk = d + PX_PAD_K, sv = d + PX_PAD_V;
     const int share = p.n_q_head / p.kv.n_head;
-    // the tiles of columns, then the heads, of one chunk follow each other on one XCD
-    int u = xcd_linear(blockIdx.x, gridDim.x);
-    const int tile = u % tiles;
-    u /= tiles;
-    const int hk = u % p.kv.n_head;
-    u /= p.kv.n_head;
-    const int gi = u % args.n_group, split = u / args.n_group;
-    const PaGroup gr = pa_group(args, gi);
-    const int cols = gr.size * share, c0 = tile * (16 * NC * NW);
-    const int64_t start = (int64_t)split * chunk, end = min(start + chunk, gr.len);
+    const int hk = w.hk, split = w.split, cols = gr.size * share, c0 = w.tile * (16 * NC * 4);
+    const int64_t start = (int64_t)split * P.chunk_p, end = min(start + P.chunk_p, gr.len);
     if (c0 >= cols || start >= end) return;  // (uniform)
 
     const TC *kp = (const TC *)p.kv.k + hk * p.kv.ld_head, *vp = (const TC *)p.kv.v + hk * p.kv.ld_head;
@@ -52,8 +104,66 @@ __global__ __launch_bounds__(NW * WAVE) void k_attn_prefix(AttnPrefix args, int 
     const uint32_t pmask = (1u << p.kv.page_shift) - 1, ldp = (uint32_t)p.kv.ld_page, ldt = (uint32_t)p.kv.ld_tok;
     TC *kl = reinterpret_cast<TC *>(lds), *vl = kl + 2 * PX_TK * sk;
 
+    // Table entry of key t0 + lane % 32 (the row's last one for keys past it)
+    auto entry_of = [&](int64_t t0) { return row[min((t0 + (lane & (PX_TK - 1))) >> p.kv.page_shift, p.ld_table - 1)]; };
+    const uint32_t magic = (65536u + nch - 1) / nch;  // f / nch for f < 1,024
+    // Two tiles under way where the registers allow: a step of a workgroup takes a
+    // microsecond, a load from memory two under full use.
+    constexpr int AHEAD = DC > 4 ? 1 : 2;
+    struct Piece {
+        vec      k[PER], v[PER];
+        uint32_t seen;
+    } even, odd;
+    auto load = [&](Piece &x, int64_t t0, int32_t entry) {
+        const uint32_t seen = x.seen = (uint32_t)__builtin_amdgcn_ballot_w64(t0 + (lane & (PX_TK - 1)) < end && (uint32_t)entry < (uint32_t)p.kv.n_pages);
+        uint64_t at[PER];
+        bool ok[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t f = i * NT + tid, key = (EXACT ? f / (DP / 8) : f * magic >> 16) & (PX_TK - 1);
+            const uint32_t pid = (uint32_t)__shfl(entry, (int)key);
+            at[i] = (uint64_t)pid * ldp + ((((uint32_t)t0 + key) & pmask) * (uint64_t)ldt + 8 * (f - key * nch));
+            ok[i] = (ALL || f < (uint32_t)(PX_TK * nch)) && (seen >> key & 1);
+        }
+        if (ALL && seen == ~0u) {  // (uniform; no lane masks)
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                x.k[i] = *reinterpret_cast<const vec *>(kp + at[i]);
+                x.v[i] = *reinterpret_cast<const vec *>(vp + at[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                x.k[i] = x.v[i] = vec{};
+                if (ok[i]) {
+                    x.k[i] = *reinterpret_cast<const vec *>(kp + at[i]);
+                    x.v[i] = *reinterpret_cast<const vec *>(vp + at[i]);
+                }
+            }
+        }
+    };
+    auto store = [&](const Piece &x, int buf) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t f = i * NT + tid, key = EXACT ? f / (DP / 8) : f * magic >> 16;
+            if (ALL || f < (uint32_t)(PX_TK * nch)) {
+                *reinterpret_cast<vec *>(kl + (buf * PX_TK + key) * sk + 8 * (f - key * nch)) = x.k[i];
+                *reinterpret_cast<vec *>(vl + (buf * PX_TK + key) * sv + 8 * (f - key * nch)) = x.v[i];
+            }
+        }
+    };
+    load(even, start, entry_of(start));
+    int32_t next = entry_of(start + PX_TK);
+    if constexpr (AHEAD == 2) {
+        load(odd, start + PX_TK, next);
+        next = entry_of(start + 2 * PX_TK);
+    }
+
+    // the queries; a negative scale goes into them, so that the largest score is
+    // the largest product, and so does one of zero (an unseen place is -inf)
     const int w0 = c0 + wave * 16 * NC;
-    const bool live = w0 < cols;
+    const bool live = w0 < cols, neg = p.scale < 0.0f;
+    const float sc = p.scale == 0.0f ? 1.0f : fabsf(p.scale) * 1.44269504088896341f;  // log2(e)
     vec q[NC][DC];
     int64_t lim[NC];
     bool ragged = false;
@@ -65,41 +175,15 @@ __global__ __launch_bounds__(NW * WAVE) void k_attn_prefix(AttnPrefix args, int 
         ragged |= __builtin_amdgcn_ballot_w64(lim[n] < end) != 0;
 #pragma unroll
         for (int k = 0; k < DC; ++k) {
-            q[n][k] = vec{};
+            v4u t = {0, 0, 0, 0};
             if (c < cols && qrow >= 0 && (EXACT || 32 * k + 8 * g < d))
-                q[n][k] = *reinterpret_cast<const vec *>((const TC *)p.q + qrow * p.ld_q + (int64_t)(hk * share + c - i * share) * d +
-                                                         32 * k + 8 * g);
+                t = *reinterpret_cast<const v4u *>((const TC *)p.q + qrow * p.ld_q + (int64_t)(hk * share + c - i * share) * d +
+                                                   32 * k + 8 * g);
+            if (neg) t = t ^ 0x80008000u;
+            if (p.scale == 0.0f) t = v4u{0, 0, 0, 0};
+            q[n][k] = __builtin_bit_cast(vec, t);
         }
     }
-
-    auto entry_of = [&](int64_t t0) { return row[min((t0 + lane) >> p.kv.page_shift, p.ld_table - 1)]; };
-    const uint32_t magic = (65536u + nch - 1) / nch;  // f / nch for f < 2,048
-    vec kr[PER], vr[PER];
-    uint64_t seen = 0;
-    auto load = [&](int64_t t0, int32_t entry) {
-        seen = __builtin_amdgcn_ballot_w64(t0 + lane < end && (uint32_t)entry < (uint32_t)p.kv.n_pages);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const uint32_t f = i * NT + tid, key = EXACT ? f / (DP / 8) : f * magic >> 16;
-            const uint32_t pid = (uint32_t)__shfl(entry, (int)(key & 63));
-            kr[i] = vr[i] = vec{};
-            if (f < (uint32_t)(PX_TK * nch) && (seen >> (key & 63) & 1)) {
-                const uint64_t at = (uint64_t)pid * ldp + (((uint32_t)t0 + key) & pmask) * (uint64_t)ldt + 8 * (f - key * nch);
-                kr[i] = *reinterpret_cast<const vec *>(kp + at);
-                vr[i] = *reinterpret_cast<const vec *>(vp + at);
-            }
-        }
-    };
-    auto store = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const uint32_t f = i * NT + tid, key = EXACT ? f / (DP / 8) : f * magic >> 16;
-            if (f < (uint32_t)(PX_TK * nch)) {
-                *reinterpret_cast<vec *>(kl + (buf * PX_TK + key) * sk + 8 * (f - key * nch)) = kr[i];
-                *reinterpret_cast<vec *>(vl + (buf * PX_TK + key) * sv + 8 * (f - key * nch)) = vr[i];
-            }
-        }
-    };
 
     float m[NC], l[NC];
     v4f o[NC][DT];
@@ -110,107 +194,113 @@ __global__ __launch_bounds__(NW * WAVE) void k_attn_prefix(AttnPrefix args, int 
 #pragma unroll
         for (int i = 0; i < DT; ++i) o[n][i] = v4f{0, 0, 0, 0};
     }
-    const float sc = p.scale * 1.44269504088896341f;  // log2(e)
-
-    load(start, entry_of(start));
-    int32_t next = entry_of(start + PX_TK);
-    store(0);
-    uint64_t mask = seen;
+    store(even, 0);
     __syncthreads();
-    int buf = 0;
-    for (int64_t t0 = start; t0 < end; t0 += PX_TK, buf ^= 1) {
-        const bool more = t0 + PX_TK < end;  // (uniform)
-        if (more) {
-            load(t0 + PX_TK, next);
-            next = entry_of(t0 + 2 * PX_TK);
+    auto step = [&](Piece &x, Piece &y, int buf, int64_t t0) {  // tile t0, loaded by way of x; y: the next one
+        const uint32_t mask = x.seen;
+        if (t0 + AHEAD * PX_TK < end) {  // (uniform)
+            load(x, t0 + AHEAD * PX_TK, next);
+            next = entry_of(t0 + (AHEAD + 1) * PX_TK);
         }
         if (live) {
             const TC *kt = kl + buf * PX_TK * sk;
             TC *vt = vl + buf * PX_TK * sv;
-            v4f st[NC][4];
+            v4f st[NC][2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int k = 0; k < DC; ++k)
 #pragma unroll
-                for (int n = 0; n < NC; ++n) st[n][j] = v4f{0, 0, 0, 0};
-#pragma unroll
-                for (int k = 0; k < DC; ++k) {
+                for (int j = 0; j < 2; ++j) {
                     vec kk = vec{};
                     if (EXACT || 32 * k + 8 * g < d) kk = *reinterpret_cast<const vec *>(kt + (16 * j + r) * sk + 32 * k + 8 * g);
 #pragma unroll
-                    for (int n = 0; n < NC; ++n) st[n][j] = Pa<TC>::mfma(kk, q[n][k], st[n][j]);
+                    for (int n = 0; n < NC; ++n) st[n][j] = Pa<TC>::mfma(kk, q[n][k], k ? st[n][j] : v4f{0, 0, 0, 0});
                 }
+            // V's fragments (columns past d: the row's end, into sums that are not kept)
+            vec a8[DT];
+#pragma unroll
+            for (int i = 0; i < DT; ++i) {
+                v4s a[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    TC *src = vt + (16 * j + 4 * g + (r >> 2)) * sv + min(16 * i, EXACT ? DP : d) + (r & 3) * 4;
+                    a[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)src);
+                }
+                a8[i] = __builtin_bit_cast(vec, __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7));
             }
-            vec pt[NC][NP][2];
+            if (mask != ~0u || ragged) {  // (uniform)
 #pragma unroll
-            for (int n = 0; n < NC; ++n) {
-                float mt = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        st[n][j][i] = st[n][j][i] * sc;
-                    }
-                if (mask != ~0ull || ragged) {  // (uniform)
+                for (int n = 0; n < NC; ++n) {
                     const int left = (int)min(max(lim[n] - t0, (int64_t)0), (int64_t)PX_TK);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int key = 16 * j + 4 * g + i;
-                            if (!(mask >> key & 1) || key >= left) st[n][j][i] = -INFINITY;
-                        }
+                    for (int e = 0; e < 8; ++e) {
+                        const int key = 16 * (e >> 2) + 4 * g + (e & 3);
+                        if (!(mask >> key & 1) || key >= left) st[n][e >> 2][e & 3] = -INFINITY;
+                    }
                 }
+            }
+            float mt[NC];
+            bool above = false;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+            for (int n = 0; n < NC; ++n) {
+                mt[n] = st[n][0][0];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) mt = fmaxf(mt, st[n][j][i]);
-                mt = fmaxf(mt, __shfl_xor(mt, 16));
-                mt = fmaxf(mt, __shfl_xor(mt, 32));
-                if (__builtin_amdgcn_ballot_w64(mt > m[n]) != 0) {
-                    const float mn = fmaxf(m[n], mt), b = mn == -INFINITY ? 0.0f : mn;
+                for (int e = 1; e < 8; ++e) mt[n] = fmaxf(mt[n], st[n][e >> 2][e & 3]);
+                mt[n] = mt[n] * sc;
+                above |= mt[n] > m[n] + PX_ROOM;
+            }
+            if (__builtin_amdgcn_ballot_w64(above) != 0) {
+#pragma unroll
+                for (int n = 0; n < NC; ++n) {
+                    mt[n] = fmaxf(mt[n], __shfl_xor(mt[n], 16));
+                    mt[n] = fmaxf(mt[n], __shfl_xor(mt[n], 32));
+                    const float mn = fmaxf(m[n], mt[n]), b = mn == -INFINITY ? 0.0f : mn;
                     const float alpha = __builtin_amdgcn_exp2f(m[n] - b);
                     m[n] = mn;
                     l[n] = l[n] * alpha;
 #pragma unroll
                     for (int i = 0; i < DT; ++i) o[n][i] = o[n][i] * alpha;
                 }
-                const float base = m[n] == -INFINITY ? 0.0f : m[n];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float e = __builtin_amdgcn_exp2f(st[n][j][i] - base);
-                        l[n] = l[n] + e;
-                        float x = e * Pa<TC>::up;
-#pragma unroll
-                        for (int t = 0; t < NP; ++t) {
-                            pt[n][t][j >> 1][4 * (j & 1) + i] = (TC)x;
-                            x = x - (float)pt[n][t][j >> 1][4 * (j & 1) + i];
-                        }
-                    }
             }
+            // column part n's probabilities, then its products while n + 1's
+            // probabilities are computed
+            uint32_t pt[NC][NP][4];
 #pragma unroll
-            for (int i = 0; i < DT; ++i) {
-                if (!EXACT && 16 * i >= d) break;
+            for (int n = 0; n < NC; ++n) {
+                // (times 2^px_up, which the sum of them is then divided by)
+                const float base = (m[n] == -INFINITY ? 0.0f : m[n]) - px_up<TC>;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    v4s a[2];
+                for (int e = 0; e < 8; e += 2) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(st[n][e >> 2][e & 3], sc, -base));
+                    const float y = __builtin_amdgcn_exp2f(fmaf(st[n][e >> 2][(e & 3) + 1], sc, -base));
+                    l[n] = l[n] + (x + y);
+                    uint32_t t[NP];
+                    px_terms(x, y, t);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        TC *src = vt + (32 * h + 16 * j + 4 * g + (r >> 2)) * sv + 16 * i + (r & 3) * 4;
-                        a[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)src);
-                    }
-                    const vec a8 = __builtin_bit_cast(vec, __builtin_shufflevector(a[0], a[1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                    for (int n = 0; n < NC; ++n)
-#pragma unroll
-                        for (int t = 0; t < NP; ++t) o[n][i] = Pa<TC>::mfma(a8, pt[n][t][h], o[n][i]);
+                    for (int k = 0; k < NP; ++k) pt[n][k][e >> 1] = t[k];
                 }
+#pragma unroll
+                for (int k = 0; k < NP; ++k)
+#pragma unroll
+                    for (int i = 0; i < DT; ++i)
+                        o[n][i] = Pa<TC>::mfma(a8[i], __builtin_bit_cast(vec, (v4u{pt[n][k][0], pt[n][k][1], pt[n][k][2], pt[n][k][3]})),
+                                               o[n][i]);
+            }
+            if constexpr (NC == 2) {
+                __builtin_amdgcn_sched_group_barrier(0x406, 80, 0);  // part 0's probabilities
+#pragma unroll
+                for (int i = 0; i < NP * DT; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x406, 4, 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x8, NP * DT, 0);
             }
         }
-        if (more) store(buf ^ 1);
-        mask = seen;
+        if (t0 + PX_TK < end) store(y, buf ^ 1);
         __syncthreads();
+    };
+    for (int64_t t0 = start; t0 < end; t0 += 2 * PX_TK) {
+        step(even, AHEAD == 2 ? odd : even, 0, t0);
+        if (t0 + PX_TK < end) step(AHEAD == 2 ? odd : even, even, 1, t0 + PX_TK);
     }
 
     // o[n][i] is values 16 i + 4 g .. + 3 of column w0 + 16 n + r
@@ -220,23 +310,47 @@ __global__ __launch_bounds__(NW * WAVE) void k_attn_prefix(AttnPrefix args, int 
         l[n] = l[n] + __shfl_xor(l[n], 32);
         const int c = w0 + 16 * n + r;
         if (c >= cols) continue;
+        // (both sums carry 2^px_up; the join takes o with Pa::up, l without)
+        l[n] = l[n] * (px_up<TC> == 0.0f ? 1.0f : 0x1p-11f);
+        const float more = px_up<TC> == 0.0f ? 1.0f : 16.0f;
         const int i = c / share;
-        const int64_t at = ((int64_t)(gi * args.max_group + i) * p.n_q_head + hk * share + c - i * share) * n_parts + split;
+        const int64_t at = ((int64_t)(w.group * args.max_group + i) * p.n_q_head + hk * share + c - i * share) * P.parts() + split;
         v4f *ov = reinterpret_cast<v4f *>(p.ws) + at * (d / 4);
 #pragma unroll
         for (int k = 0; k < DT; ++k) {
             if (!EXACT && 16 * k + 4 * g >= d) break;
-            ov[4 * k + g] = o[n][k];
+            ov[4 * k + g] = o[n][k] * more;
         }
         if (g == 0)
-            reinterpret_cast<float2 *>((float *)p.ws + (int64_t)args.n_group * args.max_group * p.n_q_head * n_parts * d)[at] =
+            reinterpret_cast<float2 *>((float *)p.ws + (int64_t)args.n_group * args.max_group * p.n_q_head * P.parts() * d)[at] =
                 make_float2(m[n], l[n]);
     }
 }
 
+// One launch of all parts.  WIDE: some group may have more than 16 columns; each
+// takes the form of its own number.  (The second bound: two workgroups a CU, the
+// registers that leaves.)
+template <typename TC, int DC, bool EXACT, int KT, bool WIDE>
+__global__ __launch_bounds__(PX_NT, 2) void k_attn_prefix(AttnPrefix p, PxPlan P) {
+    if (blockIdx.x < P.wgs_o) return px_own<TC, DC, EXACT, KT>(p, P);
+    const PxWork w = px_work(p, P);
+    if constexpr (WIDE) {
+        const PaGroup gr = pa_group(p, w.group);
+        const int cols = gr.size * (p.a.n_q_head / p.a.kv.n_head);
+        if (cols > 16) {
+            if constexpr (DC <= 4)
+                if (P.nc == 2 && cols > 64) return px_wide<TC, DC, EXACT, 2>(p, P, w, gr);
+            return px_wide<TC, DC, EXACT, 1>(p, P, w, gr);
+        }
+        if (w.tile) return;
+    }
+    pa_body<TC, DC, EXACT, KT, 4, PA_PREFIX>(p, PaWork{w.group, w.split, w.hk}, P.chunk_p, P.split_p, P.parts(), 0);
+}
+
 // The parts of a sequence's prefix and of its own tokens joined, as k_attn_join
 // does the chunks: a workgroup per query head and 4 LANES values of it.
-constexpr int PXJ_NT = 256;
+// The first PXJ_AHEAD parts of a thread are loaded before their number is known.
+constexpr int PXJ_NT = 256, PXJ_AHEAD = 4;
 template <typename TC, int LANES>
 __global__ __launch_bounds__(PXJ_NT) void k_prefix_join(AttnPrefix args, int chunk_p, int split_p, int chunk_o, int n_parts) {
     constexpr int GROUPS = PXJ_NT / LANES;
@@ -244,32 +358,52 @@ __global__ __launch_bounds__(PXJ_NT) void k_prefix_join(AttnPrefix args, int chu
     __shared__ float gm[GROUPS], gl[GROUPS];
     const AttnPaged &p = args.a;
     const int tid = threadIdx.x, d = p.kv.d_head, nq = d / 4, pieces = (nq + LANES - 1) / LANES;
-    const int h = blockIdx.x / pieces, slot = blockIdx.y, gi = slot / args.max_group;
+    const int h = blockIdx.x / pieces, s = blockIdx.y;
+    int first;
+    const int gi = pa_find(args, s, first);
     const int grp = tid / LANES, e = (blockIdx.x - h * pieces) * LANES + tid % LANES;
-    const PaGroup gr = pa_group(args, gi);
-    const int s = gr.first + slot - gi * args.max_group;
-    if (s >= gr.first + gr.size) return;  // (uniform)
-    const int64_t qrow = pa_row_of(p, s);
-    if (qrow < 0) return;  // (uniform)
-    const PaRange own = pa_own(args, gr, s);
-    const int np = (int)((gr.len + chunk_p - 1) / chunk_p);
-    const int n = np + (own.len > own.begin ? (int)((own.len - own.begin + chunk_o - 1) / chunk_o) : 0);
+    if (first < 0 || s < first || s - first >= args.max_group) return;  // (uniform; no difference past 31 bits)
+    const int slot = gi * args.max_group + s - first;
     const int64_t at = ((int64_t)slot * p.n_q_head + h) * n_parts;
     const v4f *ov = reinterpret_cast<const v4f *>(p.ws) + at * nq + min(e, nq - 1);
     const float2 *mlp =
         reinterpret_cast<const float2 *>((const float *)p.ws + (int64_t)args.n_group * args.max_group * p.n_q_head * n_parts * d) + at;
+    float2 t[PXJ_AHEAD];
+    v4f x[PXJ_AHEAD];
+    // part i of those that there are (np of the prefix): its place
+    auto fetch = [&](int i0, int np, int n) {
+#pragma unroll
+        for (int k = 0; k < PXJ_AHEAD; ++k) {
+            const int i = i0 + k * GROUPS, q = min(i < np ? i : split_p + i - np, n_parts - 1);
+            if (i < n) {
+                t[k] = mlp[q];
+                x[k] = ov[(int64_t)q * nq];
+            }
+        }
+    };
+    fetch(grp, split_p, n_parts);  // (right where the prefix has all its parts)
+    const PaGroup gr = pa_group(args, gi);
+    const int64_t qrow = pa_row_of(p, s);
+    if (s >= gr.first + gr.size || qrow < 0) return;  // (uniform)
+    const PaRange own = pa_own(args, gr, s);
+    const int np = (int)((gr.len + chunk_p - 1) / chunk_p);
+    const int n = np + (own.len > own.begin ? (int)((own.len - own.begin + chunk_o - 1) / chunk_o) : 0);
+    if (np < split_p) fetch(grp, np, n);
     v4f a = {0, 0, 0, 0};
     float M = -INFINITY, L = 0.0f;
-    for (int i = grp; i < n; i += GROUPS) {
-        const int k = i < np ? i : split_p + i - np;
-        const float2 t = mlp[k];
-        const v4f x = ov[(int64_t)k * nq];
-        const float mn = fmaxf(M, t.x), base = mn == -INFINITY ? 0.0f : mn;
-        const float f0 = __builtin_amdgcn_exp2f(M - base), f1 = __builtin_amdgcn_exp2f(t.x - base);
-        L = fmaf(t.y, f1, L * f0);
+    for (int i0 = grp; i0 < n;) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) a[c] = fmaf(x[c], f1, a[c] * f0);
-        M = mn;
+        for (int k = 0; k < PXJ_AHEAD; ++k) {
+            if (i0 + k * GROUPS >= n) break;
+            const float mn = fmaxf(M, t[k].x), base = mn == -INFINITY ? 0.0f : mn;
+            const float f0 = __builtin_amdgcn_exp2f(M - base), f1 = __builtin_amdgcn_exp2f(t[k].x - base);
+            L = fmaf(t[k].y, f1, L * f0);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) a[c] = fmaf(x[k][c], f1, a[c] * f0);
+            M = mn;
+        }
+        i0 += PXJ_AHEAD * GROUPS;
+        fetch(i0, np, n);
     }
     *reinterpret_cast<v4f *>(&part[grp][(tid % LANES) * 4]) = a;
     if (tid % LANES == 0) {
@@ -295,11 +429,6 @@ __global__ __launch_bounds__(PXJ_NT) void k_prefix_join(AttnPrefix args, int chu
     pa_write<TC>(p, qrow, h, d, e, y, top, L);
 }
 
-struct PxPlan {
-    int nw, nc, tiles;             // of the prefix; nc 0: the form of up to 16 columns
-    int chunk_p, split_p, chunk_o, split_o;
-    int parts() const { return split_p + split_o; }
-};
 static int64_t px_round(int64_t v, int64_t to, int64_t lo, int64_t hi) {
     v = v < lo ? lo : v > hi ? hi : v;
     return (v + to - 1) / to * to;
@@ -308,24 +437,20 @@ static PxPlan px_plan(int64_t n_group, int64_t max_group, int64_t max_prefix, in
                       int64_t n_kv_head, int64_t d_head) {
     PxPlan P;
     const int64_t share = n_q_head / n_kv_head, cols = share * max_group;
-    if (cols <= 16) {
-        P.nc = 0, P.nw = 4, P.tiles = 1;
-    } else {
-        P.nc = cols > 64 && d_head <= 128 ? 2 : 1;
-        P.nw = cols <= 32 ? 2 : cols <= 128 ? 4 : 8;
-        P.tiles = (int)((cols + 16 * P.nc * P.nw - 1) / (16 * P.nc * P.nw));
-    }
-    const int64_t units = n_group * n_kv_head * P.tiles, most = 1 << 20;
-    int64_t c = px_round(max_prefix * units / (P.nc == 2 ? 256 : 512), 128, 128, most);
+    P.nc = cols <= 16 ? 0 : cols > 64 && d_head <= 128 ? 2 : 1;
+    P.tiles = P.nc ? (int)((cols + 64 * P.nc - 1) / (64 * P.nc)) : 1;
+    const int64_t units = n_group * n_kv_head * P.tiles, most = 1 << 20, wgs = 512 * (n_group < 2 ? n_group : 2);
+    int64_t c = px_round(max_prefix * units / wgs, 128, 128, most);
     if (units * ((max_prefix + c - 1) / c) > 1 << 22) c = px_round(max_prefix * units >> 21, 128, 128, 1 << 30);
     P.chunk_p = (int)c;
     P.split_p = (int)((max_prefix + c - 1) / c);
+    P.wgs_p = P.split_p * units;
     const int64_t units_o = n_group * max_group * n_kv_head * ((share + 15) / 16), span = max_own + PA_ALIGN;
-    c = max_own <= 320 ? span : px_round(span * units_o / 1536, 128, 256, most);
-    c = (c + 127) / 128 * 128;
-    if (units_o * ((span + c - 1) / c) > 1 << 22) c = px_round(span * units_o >> 21, 128, 128, 1 << 30);
+    c = px_round(span * units_o / 4096, 32, 32, 128);
+    if (span > 48 * c) c = px_round(span / 48, 32, 128, (int64_t)1 << 30);
     P.chunk_o = (int)c;
     P.split_o = (int)((span + c - 1) / c);
+    P.wgs_o = 0;  // (with the number of sequences)
     return P;
 }
 size_t attn_prefix_workspace(int64_t n_group, int64_t max_group, int64_t max_prefix, int64_t max_own, int64_t n_q_head,
@@ -334,50 +459,24 @@ size_t attn_prefix_workspace(int64_t n_group, int64_t max_group, int64_t max_pre
     return (size_t)(n_group * max_group * n_q_head) * P.parts() * (d_head + 2) * 4;
 }
 
-template <typename TC, int DC, bool EXACT, PaMode MODE>
-static hipError_t run_group(const AttnPrefix &p, const PxPlan &P, hipStream_t stream) {
-    constexpr int KT = DC > 4 ? 1 : 2, NW = 4;
-    const int share = p.a.n_q_head / p.a.kv.n_head, d = p.a.kv.d_head;
-    const int R = MODE == PA_PREFIX ? share * p.max_group : share < 16 ? share : 16;
-    const int n_split = MODE == PA_PREFIX ? P.split_p : P.split_o;
-    const int64_t units = MODE == PA_PREFIX ? p.n_group : (int64_t)p.n_group * p.max_group * ((share + 15) / 16);
-    const int v = NW * KT * 16 * d * 2 + 64, o = NW * R * (DC * 32 + 4) * 4, lds = v > o ? v : o;
-    auto kern = k_attn_group<TC, DC, EXACT, KT, NW, MODE>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(units * p.a.kv.n_head * n_split)), dim3(NW * WAVE), lds, stream, p,
-                       MODE == PA_PREFIX ? P.chunk_p : P.chunk_o, n_split, P.parts(), MODE == PA_PREFIX ? 0 : P.split_p);
-    return hipGetLastError();
-}
-template <typename TC, int DC, bool EXACT, int NC, int NW>
-static hipError_t run_wide_w(const AttnPrefix &p, const PxPlan &P, hipStream_t stream) {
-    const int64_t wgs = (int64_t)P.split_p * p.n_group * p.a.kv.n_head * P.tiles;
-    const int lds = 2 * PX_TK * (2 * p.a.kv.d_head + PX_PAD_K + PX_PAD_V) * 2;
-    auto kern = k_attn_prefix<TC, DC, EXACT, NC, NW>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(NW * WAVE), lds, stream, p, P.chunk_p, P.split_p, P.parts(), P.tiles);
-    return hipGetLastError();
-}
 template <typename TC, int DC, bool EXACT>
 static hipError_t run_prefix(const AttnPrefix &p, hipStream_t stream) {
-    const PxPlan P = px_plan(p.n_group, p.max_group, p.max_prefix, p.max_own, p.a.n_q_head, p.a.kv.n_head, p.a.kv.d_head);
-    hipError_t e = hipSuccess;
-    if (P.split_p) {
-        if (P.nc == 0) {
-            e = run_group<TC, DC, EXACT, PA_PREFIX>(p, P, stream);
-        } else if constexpr (DC <= 4) {
-            e = P.nc == 2 ? (P.nw == 8 ? run_wide_w<TC, DC, EXACT, 2, 8>(p, P, stream) : run_wide_w<TC, DC, EXACT, 2, 4>(p, P, stream))
-                          : (P.nw == 4 ? run_wide_w<TC, DC, EXACT, 1, 4>(p, P, stream) : run_wide_w<TC, DC, EXACT, 1, 2>(p, P, stream));
-        } else {
-            e = P.nw == 8   ? run_wide_w<TC, DC, EXACT, 1, 8>(p, P, stream)
-                : P.nw == 4 ? run_wide_w<TC, DC, EXACT, 1, 4>(p, P, stream)
-                            : run_wide_w<TC, DC, EXACT, 1, 2>(p, P, stream);
-        }
-    }
-    if (e != hipSuccess) return e;
-    e = run_group<TC, DC, EXACT, PA_OWN>(p, P, stream);
-    if (e != hipSuccess) return e;
-    const bool few = P.parts() <= 16;
-    const int width = few ? 128 : 32, d = p.a.kv.d_head;
+    constexpr int KT = DC > 4 ? 1 : 2;
+    const int d = p.a.kv.d_head, share = p.a.n_q_head / p.a.kv.n_head;
+    PxPlan P = px_plan(p.n_group, p.max_group, p.max_prefix, p.max_own, p.a.n_q_head, p.a.kv.n_head, d);
+    P.wgs_o = ((int64_t)P.split_o * p.a.n_seq * p.a.kv.n_head * ((share + 15) / 16) + 31) / 32 * 8;
+    if (P.wgs_o > 1 << 20) P.wgs_o = 1 << 20;  // (each takes several then; at most 2^21 x 49 parts in all)
+    // LDS of the forms in the launch: pa_body's V tiles and sums of R columns, px_wide's tiles
+    const int cols = share * p.max_group, R = cols < 16 ? cols : 16;
+    const int v = 4 * KT * 16 * d * 2 + 64, o = 4 * R * (DC * 32 + 4) * 4;
+    const int w = P.nc ? 2 * PX_TK * (2 * d + PX_PAD_K + PX_PAD_V) * 2 : 0;
+    const int lds = w > v ? (w > o ? w : o) : (v > o ? v : o);
+    auto kern = P.nc ? k_attn_prefix<TC, DC, EXACT, KT, true> : k_attn_prefix<TC, DC, EXACT, KT, false>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(P.wgs_p + P.wgs_o)), dim3(PX_NT), lds, stream, p, P);
+    const bool few = P.parts() <= 16 || (int64_t)p.a.n_seq * p.a.n_q_head >= 512;
+    const int width = few ? 128 : 32;
     auto join = few ? k_prefix_join<TC, 32> : k_prefix_join<TC, 8>;
-    hipLaunchKernelGGL(join, dim3(p.a.n_q_head * ((d + width - 1) / width), p.n_group * p.max_group), dim3(PXJ_NT), 0, stream, p,
+    hipLaunchKernelGGL(join, dim3(p.a.n_q_head * ((d + width - 1) / width), p.a.n_seq), dim3(PXJ_NT), 0, stream, p,
                        P.chunk_p, P.split_p, P.chunk_o, P.parts());
     return hipGetLastError();
 }

@@ -292,8 +292,10 @@ int s2x_attn_paged_prefix(const void *q, int64_t ld_q, int64_t n_row, const int3
     if (st != S2X_OK) return st;
     st = check_prefix(who, n_group, max_group, max_prefix, max_own, n_q_head, v.n_head, v.d_head);
     if (st != S2X_OK) return st;
-    if (n_seq < 0 || n_row < 0 || n_row > INT32_MAX || n_seq > INT32_MAX)
+    if (n_seq < 0 || n_row < 0 || n_row > INT32_MAX)
         return fail(S2X_ERR_INVALID_ARG, "%s: n_seq=%lld n_row=%lld", who, (long long)n_seq, (long long)n_row);
+    if (n_seq > 65535 || n_seq * v.n_head * ((n_q_head / v.n_head + 15) / 16) > (1 << 21))
+        return fail(S2X_ERR_UNSUPPORTED, "%s: at most 65,535 sequences, 2^21 x key heads (in 16 query heads each)", who);
     if (out_type != S2X_TYPE_F32 && out_type != v.type)
         return fail(S2X_ERR_UNSUPPORTED, "%s: out_type %d (F32 or the cache's type)", who, (int)out_type);
     if (ld_table < 0 || ld_table > INT32_MAX)
