@@ -178,7 +178,8 @@ __global__ __launch_bounds__(BM_NT) void k_beam_rows(BeamSelect p, int span, int
     __shared__ float wtop[BM_WAVES];
     __shared__ int count;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.y, split = blockIdx.x;
-    if (bm_state(p, row) != 1) return;  // (uniform)
+    // (few loads a lane: latency counts, and they do not wait for the beam's state)
+    if (NL > 4 && bm_state(p, row) != 1) return;  // (uniform)
     const int from = split * span, n = min(span, p.n_vocab - from), K = p.n_out;
     const T *x = (const T *)p.logits + (int64_t)row * p.ld + from;
     if (tid == 0) count = 0;
@@ -196,6 +197,7 @@ __global__ __launch_bounds__(BM_NT) void k_beam_rows(BeamSelect p, int span, int
             __builtin_memcpy(&r[i], t, 16);
         }
     }
+    if (NL <= 4 && bm_state(p, row) != 1) return;  // (uniform)
     float mi[NL], top = -INFINITY;
     auto each_value = [&]() {  // mi and top from the values one by one
         top = -INFINITY;

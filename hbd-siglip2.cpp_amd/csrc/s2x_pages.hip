@@ -17,10 +17,10 @@ constexpr int KP_NT = 1024, KP_TILE = 4 * KP_NT;  // pages of a workgroup's tile
 constexpr uint32_t KP_FREE = 0xffffffffu;
 
 // Workspace: marks, the tiles' counts, the rows that get copies and their number
-// (fork) or the moved pages' ranks (compact).
+// (fork) or the moved pages' ranks (compact), the rows' open pages (fork).
 struct KpWs {
     uint32_t *mark;
-    int32_t  *tile, *list;
+    int32_t  *tile, *list, *last;
     int       tiles;
 };
 static __host__ __device__ inline int kp_tiles(int64_t n_pages) { return (int)((n_pages + KP_TILE - 1) / KP_TILE); }
@@ -29,12 +29,13 @@ static __host__ __device__ inline KpWs kp_ws(const KvPages &p) {
     w.tiles = kp_tiles(p.n_pages);
     w.mark = (uint32_t *)p.ws;
     w.tile = (int32_t *)(w.mark + p.n_pages);
-    w.list = w.tile + w.tiles + 1;
+    w.last = w.tile + w.tiles + 1;
+    w.list = w.last + KV_MAX_SEQ;
     return w;
 }
 size_t kv_pages_workspace(int64_t n_pages) {
     const int64_t list = n_pages > KV_MAX_SEQ ? n_pages : KV_MAX_SEQ;
-    return (size_t)(n_pages + kp_tiles(n_pages) + 1 + list) * 4;
+    return (size_t)(n_pages + kp_tiles(n_pages) + 1 + KV_MAX_SEQ + list) * 4;
 }
 
 // Sum over the workgroup's KP_NT threads in every thread, and the sum before
@@ -95,7 +96,10 @@ __global__ __launch_bounds__(256) void k_fork_mark(KvPages p) {
     const KpWs w = kp_ws(p);
     const int i = blockIdx.y;
     const KpRow r = kp_row(p, i);
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.len_out[i] = r.len;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        p.len_out[i] = r.len;
+        w.last[i] = r.open ? kp_entry(p, r.src, r.have - 1) : -1;
+    }
     for (int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x; j < p.ld_out; j += (int64_t)gridDim.x * 256) {
         int id = -1;
         if (j < r.have) {
@@ -104,6 +108,19 @@ __global__ __launch_bounds__(256) void k_fork_mark(KvPages p) {
         }
         p.table_out[(int64_t)i * p.ld_out + j] = id;
     }
+}
+
+// Row i and the page that it copies (-1: none), until it gets its own.
+__device__ __forceinline__ void kp_want(const KvPages &p, int i, int last) {
+    const int len = p.len_out[i];
+    p.copy_src[i] = last;
+    p.copy_dst[i] = -1;
+    p.copy_tok[i] = last >= 0 ? len & ((1 << p.page_shift) - 1) : 0;
+    if (last >= 0) p.table_out[(int64_t)i * p.ld_out + kp_have(p, len) - 1] = -1;
+}
+__device__ __forceinline__ void kp_give(const KvPages &p, int row, int page) {
+    p.copy_dst[row] = page;
+    p.table_out[(int64_t)row * p.ld_out + kp_have(p, p.len_out[row]) - 1] = page;
 }
 
 // Tiles' counts of free pages (fork) or held ones (compact); fork's last
@@ -127,23 +144,12 @@ __global__ __launch_bounds__(KP_NT) void k_pages_count(KvPages p) {
     int base = 0;
     for (int i0 = 0; i0 < p.n_out; i0 += KP_NT) {
         const int i = i0 + threadIdx.x;
-        int last = -1;
-        KpRow r = {};
-        if (i < p.n_out) {
-            r = kp_row(p, i);
-            if (r.open) last = kp_entry(p, r.src, r.have - 1);
-        }
+        const int last = i < p.n_out ? w.last[i] : -1;
         const bool want = last >= 0 && w.mark[last] != 1u + i;
         const int at = base + kp_scan(want, total, sums);
         base += total;
-        if (i >= p.n_out) continue;
-        p.copy_src[i] = want ? last : -1;
-        p.copy_dst[i] = -1;
-        p.copy_tok[i] = want ? r.len & ((1 << p.page_shift) - 1) : 0;
-        if (want) {
-            p.table_out[(int64_t)i * p.ld_out + r.have - 1] = -1;  // (until it gets its page)
-            w.list[at] = i;
-        }
+        if (i < p.n_out) kp_want(p, i, want ? last : -1);
+        if (want) w.list[at] = i;
     }
     if (threadIdx.x == 0) w.tile[w.tiles] = base;
 }
@@ -188,12 +194,157 @@ __global__ __launch_bounds__(KP_NT) void k_fork_assign(KvPages p) {
         if (i >= left && i < p.n_pages) p.free_out[i] = -1;
         if (!is[k]) continue;
         if (f < n_copy) {
-            const int row = w.list[f];
-            const KpRow r = kp_row(p, row);
-            p.copy_dst[row] = (int)i;
-            p.table_out[(int64_t)row * p.ld_out + r.have - 1] = (int)i;
+            kp_give(p, w.list[f], (int)i);
         } else {
             p.free_out[f - n_copy] = (int)i;
+        }
+        ++f;
+    }
+}
+
+// The same of few pages, where a workgroup counts all marks, and all rows that get
+// copies, itself rather than after another launch.
+constexpr int KP_FEW = 8 * KP_TILE;
+__device__ __forceinline__ void kp_marks(const KpWs &w, int64_t n_pages, uint32_t what, uint32_t (&is)[KP_FEW / KP_TILE]) {
+    v4u m[KP_FEW / KP_TILE];
+#pragma unroll
+    for (int t = 0; t < KP_FEW / KP_TILE; ++t) {  // bit k of is[t]: page t KP_TILE + 4 tid + k
+        const int64_t i0 = (int64_t)t * KP_TILE + 4 * threadIdx.x;
+        m[t] = v4u{~what, ~what, ~what, ~what};
+        if (i0 + 4 <= n_pages) {
+            m[t] = *reinterpret_cast<const v4u *>(w.mark + i0);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 3; ++k)
+                if (i0 + k < n_pages) m[t][k] = w.mark[i0 + k];
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < KP_FEW / KP_TILE; ++t) {
+        is[t] = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) is[t] |= (uint32_t)(m[t][k] == what) << k;
+    }
+}
+__global__ __launch_bounds__(KP_NT) void k_fork_assign_few(KvPages p) {
+    __shared__ int32_t sums[KP_NT / WAVE];
+    __shared__ int32_t list[KV_MAX_SEQ];
+    const KpWs w = kp_ws(p);
+    uint32_t is[KP_FEW / KP_TILE];
+    kp_marks(w, p.n_pages, KP_FREE, is);
+    int n_copy = 0, all, before, total;
+    for (int i0 = 0; i0 < p.n_out; i0 += KP_NT) {
+        const int i = i0 + threadIdx.x, last = i < p.n_out ? w.last[i] : -1;
+        const bool want = last >= 0 && w.mark[last] != 1u + i;
+        const int at = n_copy + kp_scan(want, total, sums);
+        n_copy += total;
+        if (want) list[at] = i;
+        // (a row that gets a page has its place and table entry from the workgroup of that page)
+        if (blockIdx.x == 0 && i < p.n_out) {
+            p.copy_src[i] = want ? last : -1;
+            p.copy_tok[i] = want ? p.len_out[i] & ((1 << p.page_shift) - 1) : 0;
+            if (!want) p.copy_dst[i] = -1;
+        }
+    }
+    int a = 0, b = 0, mine = 0;
+#pragma unroll
+    for (int t = 0; t < KP_FEW / KP_TILE; ++t) {
+        const int n = __builtin_popcount(is[t]);
+        if (t < (int)blockIdx.x) a += n;
+        if (t == (int)blockIdx.x) mine = n;
+        b += n;
+    }
+    kp_scan(a, before, sums);
+    kp_scan(b, all, sums);
+    int f = before + kp_scan(mine, total, sums);  // (and the list is there)
+    const int left = max(all - n_copy, 0);
+    if (blockIdx.x == 0) {
+        if (threadIdx.x == 0) {
+            p.count[0] = left;
+            p.count[1] = n_copy;
+        }
+        for (int k = all + threadIdx.x; k < n_copy; k += KP_NT) kp_give(p, list[k], -1);
+    }
+    uint32_t bits = 0;
+#pragma unroll
+    for (int t = 0; t < KP_FEW / KP_TILE; ++t)
+        if (t == (int)blockIdx.x) bits = is[t];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int64_t i = (int64_t)blockIdx.x * KP_TILE + 4 * threadIdx.x + k;
+        if (i >= left && i < p.n_pages) p.free_out[i] = -1;
+        if (!(bits >> k & 1)) continue;
+        if (f < n_copy) kp_give(p, list[f], (int)i);
+        else p.free_out[f - n_copy] = (int)i;
+        ++f;
+    }
+}
+
+// All of a fork in one workgroup, marks in LDS: few entries and pages, whose time
+// would be that of the launches (4 rows of 26 entries: 3.9 us, in three launches 14;
+// 96 rows of 112 11 against 13, 240 21 against 14).
+constexpr int KP_ONE_PAGES = 16 * KP_NT, KP_ONE_ENTRIES = 12 * KP_NT;
+__global__ __launch_bounds__(KP_NT) void k_fork_one(KvPages p) {
+    __shared__ uint32_t mark[KP_ONE_PAGES];
+    __shared__ int32_t sums[KP_NT / WAVE], src[KP_NT], have[KP_NT], list[KP_NT], last[KP_NT];
+    __shared__ bool open[KP_NT];
+    const int tid = threadIdx.x, n_pages = (int)p.n_pages, ld = (int)p.ld_out;
+    KpRow r = {};
+    if (tid < p.n_out) {
+        r = kp_row(p, tid);
+        src[tid] = r.src;
+        have[tid] = (int)r.have;
+        open[tid] = r.open;
+        last[tid] = -1;
+        p.len_out[tid] = r.len;
+    }
+    for (int i = tid; i < n_pages; i += KP_NT) mark[i] = p.pinned && p.pinned[i] ? 0u : KP_FREE;
+    __syncthreads();
+#pragma unroll 4
+    for (int e = tid; e < p.n_out * ld; e += KP_NT) {
+        const int i = e / ld, j = e - i * ld;
+        int id = -1;
+        if (j < have[i]) {
+            id = kp_entry(p, src[i], j);
+            if (id >= 0) {
+                const bool o = open[i] && j == have[i] - 1;
+                atomicMin(&mark[id], o ? 1u + i : 0u);
+                if (o) last[i] = id;
+            }
+        }
+        p.table_out[e] = id;
+    }
+    __syncthreads();
+    int n_copy, all;
+    const int page = tid < p.n_out ? last[tid] : -1;
+    const bool want = page >= 0 && mark[page] != 1u + tid;
+    const int at = kp_scan(want, n_copy, sums);
+    if (want) list[at] = tid;
+    const int per = (n_pages + KP_NT - 1) / KP_NT;  // pages of a thread, at most 16
+    int n = 0;
+    for (int k = 0; k < per; ++k) n += tid * per + k < n_pages && mark[tid * per + k] == KP_FREE;
+    int f = kp_scan(n, all, sums);
+    const int left = max(all - n_copy, 0);
+    if (tid == 0) {
+        p.count[0] = left;
+        p.count[1] = n_copy;
+    }
+    if (tid < p.n_out) {
+        p.copy_src[tid] = want ? page : -1;
+        p.copy_tok[tid] = want ? r.len & ((1 << p.page_shift) - 1) : 0;
+        if (!want || at >= all) p.copy_dst[tid] = -1;
+        if (want && at >= all) p.table_out[tid * ld + r.have - 1] = -1;
+    }
+    for (int i = left + tid; i < n_pages; i += KP_NT) p.free_out[i] = -1;
+    for (int k = 0; k < per; ++k) {
+        const int i = tid * per + k;
+        if (i >= n_pages || mark[i] != KP_FREE) continue;
+        if (f < n_copy) {
+            const int row = list[f];
+            p.copy_dst[row] = i;
+            p.table_out[row * ld + have[row] - 1] = i;
+        } else {
+            p.free_out[f - n_copy] = i;
         }
         ++f;
     }
@@ -208,8 +359,21 @@ __global__ __launch_bounds__(256) void k_compact_mark(KvPages p) {
     }
 }
 
-// N pages are held.  Page i >= N that is held is the (held before i - held before
-// N)-th to move, page i < N that is not the (i - held before i)-th to be filled.
+// `all` pages are held, `below` of them among the first `all`, `before` of them
+// before page i.  Page i >= all that is held is the (before - below)-th to move, page
+// i < all that is not the (i - before)-th to be filled.
+__device__ __forceinline__ void kp_place(const KvPages &p, const KpWs &w, int64_t i, bool held, int &before, int all, int below) {
+    if (i >= p.n_pages) return;
+    if (i >= all - below && i < p.n_pages / 2) p.copy_src[i] = p.copy_dst[i] = -1;
+    if (held && i >= all) {
+        const int rank = before - below;
+        p.copy_src[rank] = (int)i;
+        w.list[i] = rank;
+    } else if (!held && i < all) {
+        p.copy_dst[(int)i - before] = (int)i;
+    }
+    before += held;
+}
 __global__ __launch_bounds__(KP_NT) void k_compact_assign(KvPages p) {
     __shared__ int32_t sums[KP_NT / WAVE];
     const KpWs w = kp_ws(p);
@@ -236,19 +400,43 @@ __global__ __launch_bounds__(KP_NT) void k_compact_assign(KvPages p) {
         p.count[1] = n_move;
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int64_t i = i0 + k;
-        if (i >= p.n_pages) break;
-        if (i >= n_move && i < p.n_pages / 2) p.copy_src[i] = p.copy_dst[i] = -1;
-        if (is[k] && i >= all) {
-            const int rank = before - tiles_below;
-            p.copy_src[rank] = (int)i;
-            w.list[i] = rank;
-        } else if (!is[k] && i < all) {
-            p.copy_dst[(int)i - before] = (int)i;
+    for (int k = 0; k < 4; ++k) kp_place(p, w, i0 + k, is[k], before, all, tiles_below);
+}
+
+// (as k_fork_assign_few)
+__global__ __launch_bounds__(KP_NT) void k_compact_assign_few(KvPages p) {
+    __shared__ int32_t sums[KP_NT / WAVE];
+    const KpWs w = kp_ws(p);
+    uint32_t is[KP_FEW / KP_TILE];
+    kp_marks(w, p.n_pages, 1u, is);
+    int a = 0, b = 0, mine = 0, c = 0, first, all, below, total;
+    uint32_t bits = 0;
+#pragma unroll
+    for (int t = 0; t < KP_FEW / KP_TILE; ++t) {
+        const int n = __builtin_popcount(is[t]);
+        if (t < (int)blockIdx.x) a += n;
+        if (t == (int)blockIdx.x) {
+            mine = n;
+            bits = is[t];
         }
-        before += is[k];
+        b += n;
     }
+    kp_scan(a, first, sums);
+    kp_scan(b, all, sums);
+    int before = first + kp_scan(mine, total, sums);
+#pragma unroll
+    for (int t = 0; t < KP_FEW / KP_TILE; ++t) {
+        const int n = min(max(all - t * KP_TILE - 4 * (int)threadIdx.x, 0), 4);  // of this thread's below N
+        c += __builtin_popcount(is[t] & ((1u << n) - 1));
+    }
+    kp_scan(c, below, sums);
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        p.count[0] = all;
+        p.count[1] = all - below;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        kp_place(p, w, (int64_t)blockIdx.x * KP_TILE + 4 * threadIdx.x + k, bits >> k & 1, before, all, below);
 }
 
 __global__ __launch_bounds__(256) void k_compact_tables(KvPages p) {
@@ -266,19 +454,31 @@ static dim3 kp_rows(int64_t width, int64_t rows) {
     return dim3((unsigned)(x < 1 ? 1 : x > 64 ? 64 : x), (unsigned)rows);
 }
 hipError_t launch_kv_fork(const KvPages &p, hipStream_t stream) {
+    if (p.n_out <= KP_NT && p.n_out * p.ld_out <= KP_ONE_ENTRIES && p.n_pages <= KP_ONE_PAGES) {
+        hipLaunchKernelGGL(k_fork_one, dim3(1), dim3(KP_NT), 0, stream, p);
+        return hipGetLastError();
+    }
     const int tiles = kp_tiles(p.n_pages);
     if (tiles) hipLaunchKernelGGL(k_pages_clear<true>, dim3((unsigned)((p.n_pages + 255) / 256)), dim3(256), 0, stream, p);
     if (p.n_out) hipLaunchKernelGGL(k_fork_mark, kp_rows(p.ld_out, p.n_out), dim3(256), 0, stream, p);
+    if (p.n_pages <= KP_FEW) {
+        hipLaunchKernelGGL(k_fork_assign_few, dim3(tiles ? tiles : 1), dim3(KP_NT), 0, stream, p);
+        return hipGetLastError();
+    }
     hipLaunchKernelGGL(k_pages_count<true>, dim3(tiles + 1), dim3(KP_NT), 0, stream, p);
-    hipLaunchKernelGGL(k_fork_assign, dim3(tiles ? tiles : 1), dim3(KP_NT), 0, stream, p);
+    hipLaunchKernelGGL(k_fork_assign, dim3(tiles), dim3(KP_NT), 0, stream, p);
     return hipGetLastError();
 }
 hipError_t launch_kv_compact(const KvPages &p, hipStream_t stream) {
     const int tiles = kp_tiles(p.n_pages);
     if (tiles) hipLaunchKernelGGL(k_pages_clear<false>, dim3((unsigned)((p.n_pages + 255) / 256)), dim3(256), 0, stream, p);
     if (p.n_seq) hipLaunchKernelGGL(k_compact_mark, kp_rows(p.ld_table, p.n_seq), dim3(256), 0, stream, p);
-    if (tiles) hipLaunchKernelGGL(k_pages_count<false>, dim3(tiles), dim3(KP_NT), 0, stream, p);
-    hipLaunchKernelGGL(k_compact_assign, dim3(tiles ? tiles : 1), dim3(KP_NT), 0, stream, p);
+    if (p.n_pages <= KP_FEW) {
+        hipLaunchKernelGGL(k_compact_assign_few, dim3(tiles ? tiles : 1), dim3(KP_NT), 0, stream, p);
+    } else {
+        hipLaunchKernelGGL(k_pages_count<false>, dim3(tiles), dim3(KP_NT), 0, stream, p);
+        hipLaunchKernelGGL(k_compact_assign, dim3(tiles), dim3(KP_NT), 0, stream, p);
+    }
     if (p.n_seq) hipLaunchKernelGGL(k_compact_tables, kp_rows(p.ld_out, p.n_seq), dim3(256), 0, stream, p);
     return hipGetLastError();
 }

@@ -555,8 +555,8 @@ int s2x_add_rmsnorm_quantize_q8_1(const void *x, int32_t x_type, int64_t ld_x, c
  * done (optional, a byte a beam): not 0, the beam has ended; it is a candidate as it
  * is, with done_token and its score.  A beam whose score is no finite number is
  * none (the first step: -inf for all but one), nor has one with a NaN, +inf or no
- * value above -inf among its logits candidates.  Its logits are not read in the
- * first two cases.  Where candidates are fewer than n_out the rest are parent and
+ * value above -inf among its logits candidates.  In the first two cases its logits
+ * count for nothing, whatever they are.  Where candidates are fewer than n_out the rest are parent and
  * token -1, score -inf.  Scores are compared as they are, with no regard to
  * lengths.  n_beam and n_out <= 64, n_req * n_beam <= 65,535, n_vocab <= 2^24.
  * No output overlaps an input or another one.  workspace of
