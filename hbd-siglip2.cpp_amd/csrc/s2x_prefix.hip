@@ -26,27 +26,21 @@ struct PxPlan {
 // neighbours in the order of workgroups of its XCD.
 template <typename TC, int DC, bool EXACT, int KT>
 __device__ __forceinline__ void px_own(const AttnPrefix &p, const PxPlan &P) {
-    const int w = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int w = blockIdx.x - (int)P.wgs_p, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int H = p.a.kv.n_head * ((p.a.n_q_head / p.a.kv.n_head + 15) / 16);
     for (int bid = w / 8 * 32 + wave * 8 + w % 8; bid < p.a.n_seq * P.split_o * H; bid += (int)P.wgs_o * 4)
         pa_body<TC, DC, EXACT, KT, 1, PA_OWN>(p, pa_work(bid, p.a.n_seq, P.split_o, H), P.chunk_o, P.split_o, P.parts(), P.split_p);
 }
 
 // A workgroup's part of the prefixes: the tiles of columns, then the heads, of one
-// chunk follow each other on one XCD.
+// chunk follow each other on one XCD, the chunks of a group lie on different ones.
 struct PxWork {
     int tile, hk, group, split;
 };
 __device__ __forceinline__ PxWork px_work(const AttnPrefix &p, const PxPlan &P) {
-    int u = xcd_linear(blockIdx.x - (int)P.wgs_o, (int)P.wgs_p);  // (wgs_o: a multiple of 8)
-    PxWork w;
-    w.tile = u % P.tiles;
-    u /= P.tiles;
-    w.hk = u % p.a.kv.n_head;
-    u /= p.a.kv.n_head;
-    w.group = u % p.n_group;
-    w.split = u / p.n_group;
-    return w;
+    const PaWork w = pa_work(blockIdx.x, p.n_group, P.split_p, p.a.kv.n_head * P.tiles);
+    const int hk = w.hp / P.tiles;
+    return PxWork{w.hp - hk * P.tiles, hk, w.unit, w.split};
 }
 
 constexpr int PX_TK = 32, PX_NT = 4 * WAVE;  // keys of a tile, threads
@@ -104,45 +98,50 @@ __device__ __forceinline__ void px_wide(const AttnPrefix &args, const PxPlan &P,
     const uint32_t pmask = (1u << p.kv.page_shift) - 1, ldp = (uint32_t)p.kv.ld_page, ldt = (uint32_t)p.kv.ld_tok;
     TC *kl = reinterpret_cast<TC *>(lds), *vl = kl + 2 * PX_TK * sk;
 
-    // Table entry of key t0 + lane % 32 (the row's last one for keys past it)
-    auto entry_of = [&](int64_t t0) { return row[min((t0 + (lane & (PX_TK - 1))) >> p.kv.page_shift, p.ld_table - 1)]; };
+    // Table entries: of key t0 + lane % 32 (`mask`, for which keys there are) and of
+    // the keys of this thread's pieces; the row's last one for keys past it.
+    struct Entries {
+        int32_t mask, piece[PER];
+    };
+    const int last = (int)p.ld_table - 1, shift = p.kv.page_shift;
     const uint32_t magic = (65536u + nch - 1) / nch;  // f / nch for f < 1,024
+    auto key_of = [&](int i) -> uint32_t {
+        const uint32_t f = i * NT + tid;
+        return (EXACT ? f / (DP / 8) : f * magic >> 16) & (PX_TK - 1);
+    };
+    auto entries = [&](int64_t t0) {
+        Entries e;
+        e.mask = row[min((int)((uint32_t)(t0 + (lane & (PX_TK - 1))) >> shift), last)];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) e.piece[i] = row[min((int)((uint32_t)(t0 + key_of(i)) >> shift), last)];
+        return e;
+    };
     // Two tiles under way where the registers allow: a step of a workgroup takes a
-    // microsecond, a load from memory two under full use.
+    // microsecond, a load from memory two under full use.  Where a page is none the
+    // first one is loaded, and zeros are stored.
     constexpr int AHEAD = DC > 4 ? 1 : 2;
     struct Piece {
         vec      k[PER], v[PER];
         uint32_t seen;
     } even, odd;
-    auto load = [&](Piece &x, int64_t t0, int32_t entry) {
-        const uint32_t seen = x.seen = (uint32_t)__builtin_amdgcn_ballot_w64(t0 + (lane & (PX_TK - 1)) < end && (uint32_t)entry < (uint32_t)p.kv.n_pages);
-        uint64_t at[PER];
-        bool ok[PER];
+    auto load = [&](Piece &x, int64_t t0, const Entries &e) {
+        x.seen = (uint32_t)__builtin_amdgcn_ballot_w64(t0 + (lane & (PX_TK - 1)) < end && (uint32_t)e.mask < (uint32_t)p.kv.n_pages);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const uint32_t f = i * NT + tid, key = (EXACT ? f / (DP / 8) : f * magic >> 16) & (PX_TK - 1);
-            const uint32_t pid = (uint32_t)__shfl(entry, (int)key);
-            at[i] = (uint64_t)pid * ldp + ((((uint32_t)t0 + key) & pmask) * (uint64_t)ldt + 8 * (f - key * nch));
-            ok[i] = (ALL || f < (uint32_t)(PX_TK * nch)) && (seen >> key & 1);
-        }
-        if (ALL && seen == ~0u) {  // (uniform; no lane masks)
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                x.k[i] = *reinterpret_cast<const vec *>(kp + at[i]);
-                x.v[i] = *reinterpret_cast<const vec *>(vp + at[i]);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                x.k[i] = x.v[i] = vec{};
-                if (ok[i]) {
-                    x.k[i] = *reinterpret_cast<const vec *>(kp + at[i]);
-                    x.v[i] = *reinterpret_cast<const vec *>(vp + at[i]);
-                }
-            }
+            const uint32_t f = i * NT + tid, key = key_of(i);
+            const uint32_t pid = (uint32_t)e.piece[i] < (uint32_t)p.kv.n_pages ? (uint32_t)e.piece[i] : 0u;
+            const uint32_t piece = ALL || f < (uint32_t)(PX_TK * nch) ? f - (EXACT ? f / (DP / 8) : f * magic >> 16) * nch : 0u;
+            const uint64_t at = (uint64_t)pid * ldp + ((((uint32_t)t0 + key) & pmask) * (uint64_t)ldt + 8 * piece);
+            x.k[i] = *reinterpret_cast<const vec *>(kp + at);
+            x.v[i] = *reinterpret_cast<const vec *>(vp + at);
         }
     };
-    auto store = [&](const Piece &x, int buf) {
+    auto store = [&](Piece &x, int buf) {
+        if (x.seen != ~0u) {  // (uniform)
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if (!(x.seen >> key_of(i) & 1)) x.k[i] = x.v[i] = vec{};
+        }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const uint32_t f = i * NT + tid, key = EXACT ? f / (DP / 8) : f * magic >> 16;
@@ -152,11 +151,12 @@ __device__ __forceinline__ void px_wide(const AttnPrefix &args, const PxPlan &P,
             }
         }
     };
-    load(even, start, entry_of(start));
-    int32_t next = entry_of(start + PX_TK);
-    if constexpr (AHEAD == 2) {
-        load(odd, start + PX_TK, next);
-        next = entry_of(start + 2 * PX_TK);
+    Entries next;
+    {
+        const Entries e0 = entries(start), e1 = entries(start + PX_TK);
+        next = AHEAD == 2 ? entries(start + 2 * PX_TK) : e1;
+        load(even, start, e0);
+        if constexpr (AHEAD == 2) load(odd, start + PX_TK, e1);
     }
 
     // the queries; a negative scale goes into them, so that the largest score is
@@ -198,23 +198,31 @@ __device__ __forceinline__ void px_wide(const AttnPrefix &args, const PxPlan &P,
     __syncthreads();
     auto step = [&](Piece &x, Piece &y, int buf, int64_t t0) {  // tile t0, loaded by way of x; y: the next one
         const uint32_t mask = x.seen;
+        // the keys out of LDS, then the loads of tiles to come (their entries first: a
+        // wait for one is a wait for the loads before it, too), then the scores
+        const TC *kt = kl + buf * PX_TK * sk;
+        vec kk[DC][2];
+#pragma unroll
+        for (int k = 0; k < DC; ++k)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                kk[k][j] = vec{};
+                if (EXACT || 32 * k + 8 * g < d) kk[k][j] = *reinterpret_cast<const vec *>(kt + (16 * j + r) * sk + 32 * k + 8 * g);
+            }
         if (t0 + AHEAD * PX_TK < end) {  // (uniform)
+            const Entries after = entries(t0 + (AHEAD + 1) * PX_TK);
             load(x, t0 + AHEAD * PX_TK, next);
-            next = entry_of(t0 + (AHEAD + 1) * PX_TK);
+            next = after;
         }
         if (live) {
-            const TC *kt = kl + buf * PX_TK * sk;
             TC *vt = vl + buf * PX_TK * sv;
             v4f st[NC][2];
 #pragma unroll
             for (int k = 0; k < DC; ++k)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    vec kk = vec{};
-                    if (EXACT || 32 * k + 8 * g < d) kk = *reinterpret_cast<const vec *>(kt + (16 * j + r) * sk + 32 * k + 8 * g);
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int n = 0; n < NC; ++n) st[n][j] = Pa<TC>::mfma(kk, q[n][k], k ? st[n][j] : v4f{0, 0, 0, 0});
-                }
+                    for (int n = 0; n < NC; ++n) st[n][j] = Pa<TC>::mfma(kk[k][j], q[n][k], k ? st[n][j] : v4f{0, 0, 0, 0});
             // V's fragments (columns past d: the row's end, into sums that are not kept)
             vec a8[DT];
 #pragma unroll
@@ -332,7 +340,7 @@ __device__ __forceinline__ void px_wide(const AttnPrefix &args, const PxPlan &P,
 // registers that leaves.)
 template <typename TC, int DC, bool EXACT, int KT, bool WIDE>
 __global__ __launch_bounds__(PX_NT, 2) void k_attn_prefix(AttnPrefix p, PxPlan P) {
-    if (blockIdx.x < P.wgs_o) return px_own<TC, DC, EXACT, KT>(p, P);
+    if (blockIdx.x >= P.wgs_p) return px_own<TC, DC, EXACT, KT>(p, P);
     const PxWork w = px_work(p, P);
     if constexpr (WIDE) {
         const PaGroup gr = pa_group(p, w.group);
@@ -350,13 +358,14 @@ __global__ __launch_bounds__(PX_NT, 2) void k_attn_prefix(AttnPrefix p, PxPlan P
 // The parts of a sequence's prefix and of its own tokens joined, as k_attn_join
 // does the chunks: a workgroup per query head and 4 LANES values of it.
 // The first PXJ_AHEAD parts of a thread are loaded before their number is known.
-constexpr int PXJ_NT = 256, PXJ_AHEAD = 4;
-template <typename TC, int LANES>
-__global__ __launch_bounds__(PXJ_NT) void k_prefix_join(AttnPrefix args, int chunk_p, int split_p, int chunk_o, int n_parts) {
-    constexpr int GROUPS = PXJ_NT / LANES;
+constexpr int PXJ_AHEAD = 4;
+template <typename TC, int LANES, int NT>
+__global__ __launch_bounds__(NT) void k_prefix_join(AttnPrefix args, PxPlan P) {
+    constexpr int GROUPS = NT / LANES;
     __shared__ __align__(16) float part[GROUPS][LANES * 4 + 4];
     __shared__ float gm[GROUPS], gl[GROUPS];
     const AttnPaged &p = args.a;
+    const int n_parts = P.parts(), split_p = P.split_p, chunk_o = P.chunk_o;
     const int tid = threadIdx.x, d = p.kv.d_head, nq = d / 4, pieces = (nq + LANES - 1) / LANES;
     const int h = blockIdx.x / pieces, s = blockIdx.y;
     int first;
@@ -386,7 +395,7 @@ __global__ __launch_bounds__(PXJ_NT) void k_prefix_join(AttnPrefix args, int chu
     const int64_t qrow = pa_row_of(p, s);
     if (s >= gr.first + gr.size || qrow < 0) return;  // (uniform)
     const PaRange own = pa_own(args, gr, s);
-    const int np = (int)((gr.len + chunk_p - 1) / chunk_p);
+    const int np = (int)((gr.len + P.chunk_p - 1) / P.chunk_p);
     const int n = np + (own.len > own.begin ? (int)((own.len - own.begin + chunk_o - 1) / chunk_o) : 0);
     if (np < split_p) fetch(grp, np, n);
     v4f a = {0, 0, 0, 0};
@@ -473,11 +482,13 @@ static hipError_t run_prefix(const AttnPrefix &p, hipStream_t stream) {
     const int lds = w > v ? (w > o ? w : o) : (v > o ? v : o);
     auto kern = P.nc ? k_attn_prefix<TC, DC, EXACT, KT, true> : k_attn_prefix<TC, DC, EXACT, KT, false>;
     hipLaunchKernelGGL(kern, dim3((unsigned)(P.wgs_p + P.wgs_o)), dim3(PX_NT), lds, stream, p, P);
-    const bool few = P.parts() <= 16 || (int64_t)p.a.n_seq * p.a.n_q_head >= 512;
-    const int width = few ? 128 : 32;
-    auto join = few ? k_prefix_join<TC, 32> : k_prefix_join<TC, 8>;
-    hipLaunchKernelGGL(join, dim3(p.a.n_q_head * ((d + width - 1) / width), p.a.n_seq), dim3(PXJ_NT), 0, stream, p,
-                       P.chunk_p, P.split_p, P.chunk_o, P.parts());
+    const bool many = (int64_t)p.a.n_seq * p.a.n_q_head >= 512, few = P.parts() <= 16;
+    // (many rows: a wave each, so that all are at work at once; 64 sequences of 32 heads
+    // and 2 parts 7.1 us, in four waves 8.5)
+    const int width = few || many ? 128 : 32;
+    auto join = width == 32 ? k_prefix_join<TC, 8, 256> : many ? k_prefix_join<TC, 32, 64> : k_prefix_join<TC, 32, 256>;
+    hipLaunchKernelGGL(join, dim3(p.a.n_q_head * ((d + width - 1) / width), p.a.n_seq), dim3(many && width > 32 ? 64 : 256), 0,
+                       stream, p, P);
     return hipGetLastError();
 }
 template <typename TC>
