@@ -355,6 +355,35 @@ __global__ __launch_bounds__(PX_NT, 2) void k_attn_prefix(AttnPrefix p, PxPlan P
     pa_body<TC, DC, EXACT, KT, 4, PA_PREFIX>(p, PaWork{w.group, w.split, w.hk}, P.chunk_p, P.split_p, P.parts(), 0);
 }
 
+// Four values, from c on, of the sum over the prefix's keys [from, to), relative to
+// the score m: for a sequence that ends inside a chunk.  The chunk's sums count keys
+// behind its end 0 times their value, which is no 0 where that is infinite or NaN;
+// then those that it sees once more, one after the other.  (A wrong sum shows: it is
+// no number.  m and the sum of the exponentials do not hang on the values.)
+template <typename TC>
+__device__ __forceinline__ v4f px_seen_only(const AttnPaged &p, int seq, int hk, const TC *q, int c, int64_t from, int64_t to, float m) {
+    typedef TC vec4 __attribute__((ext_vector_type(4)));
+    const int32_t *row = p.table + seq * p.ld_table;
+    v4f o = {0, 0, 0, 0};
+    for (int64_t t = from; t < to; ++t) {
+        const int32_t id = row[t >> p.kv.page_shift];
+        if (id < 0 || id >= p.kv.n_pages) continue;
+        const int64_t at = (int64_t)hk * p.kv.ld_head + id * p.kv.ld_page + (t & ((1 << p.kv.page_shift) - 1)) * p.kv.ld_tok;
+        const TC *kp = (const TC *)p.kv.k + at;
+        float s = 0.0f;
+        for (int i = 0; i < p.kv.d_head; i += 4) {
+            const vec4 a = *reinterpret_cast<const vec4 *>(kp + i), b = *reinterpret_cast<const vec4 *>(q + i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s = fmaf((float)a[k], (float)b[k], s);
+        }
+        const float x = __builtin_amdgcn_exp2f(s * (p.scale * 1.44269504088896341f) - (m == -INFINITY ? 0.0f : m)) * Pa<TC>::up;
+        const vec4 v = *reinterpret_cast<const vec4 *>((const TC *)p.kv.v + at + c);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = fmaf(x, (float)v[k], o[k]);
+    }
+    return o;
+}
+
 // The parts of a sequence's prefix and of its own tokens joined, as k_attn_join
 // does the chunks: a workgroup per query head and 4 LANES values of it.
 // The first PXJ_AHEAD parts of a thread are loaded before their number is known.
@@ -395,11 +424,12 @@ __global__ __launch_bounds__(NT) void k_prefix_join(AttnPrefix args, PxPlan P) {
     const int64_t qrow = pa_row_of(p, s);
     if (s >= gr.first + gr.size || qrow < 0) return;  // (uniform)
     const PaRange own = pa_own(args, gr, s);
-    const int np = (int)((gr.len + P.chunk_p - 1) / P.chunk_p);
+    const int np = (int)((own.first + P.chunk_p - 1) / P.chunk_p);  // (those that it sees something of)
     const int n = np + (own.len > own.begin ? (int)((own.len - own.begin + chunk_o - 1) / chunk_o) : 0);
     if (np < split_p) fetch(grp, np, n);
     v4f a = {0, 0, 0, 0};
-    float M = -INFINITY, L = 0.0f;
+    float M = -INFINITY, L = 0.0f, redo = NAN;
+    const int ends = own.first < min(gr.len, (int64_t)np * P.chunk_p) ? np - 1 : -1;  // the chunk that it ends in
     for (int i0 = grp; i0 < n;) {
 #pragma unroll
         for (int k = 0; k < PXJ_AHEAD; ++k) {
@@ -407,12 +437,24 @@ __global__ __launch_bounds__(NT) void k_prefix_join(AttnPrefix args, PxPlan P) {
             const float mn = fmaxf(M, t[k].x), base = mn == -INFINITY ? 0.0f : mn;
             const float f0 = __builtin_amdgcn_exp2f(M - base), f1 = __builtin_amdgcn_exp2f(t[k].x - base);
             L = fmaf(t[k].y, f1, L * f0);
+            if (i0 + k * GROUPS == ends && !(fabsf(x[k][0]) + fabsf(x[k][1]) + fabsf(x[k][2]) + fabsf(x[k][3]) < INFINITY)) {
+                redo = t[k].x;
+                x[k] = v4f{0, 0, 0, 0};
+            }
 #pragma unroll
             for (int c = 0; c < 4; ++c) a[c] = fmaf(x[k][c], f1, a[c] * f0);
             M = mn;
         }
         i0 += PXJ_AHEAD * GROUPS;
         fetch(i0, np, n);
+    }
+    if (redo == redo) {
+        const int share = p.n_q_head / p.kv.n_head, ec = min(e, nq - 1);
+        const v4f y = px_seen_only<TC>(p, gr.first, h / share, (const TC *)p.q + qrow * p.ld_q + (int64_t)h * d, 4 * ec,
+                                       (int64_t)ends * P.chunk_p, own.first, redo);
+        const float f = __builtin_amdgcn_exp2f(redo - (M == -INFINITY ? 0.0f : M));
+#pragma unroll
+        for (int c = 0; c < 4; ++c) a[c] = fmaf(y[c], f, a[c]);
     }
     *reinterpret_cast<v4f *>(&part[grp][(tid % LANES) * 4]) = a;
     if (tid % LANES == 0) {

@@ -318,3 +318,45 @@ def test_cache_past_32_bits():
     for hq in (4, 24):
         got, lse = run_prefix(q[:, :hq].contiguous(), cache, table, lens, np.array([0, 2]), np.array([192]), 0.09, "f32")
         compare(got, lse, q[:, :hq], cache, table, lens, 0.09, "f32")
+
+
+@pytest.mark.parametrize("share,size,d,kind", [(2, 5, 128, "f16"), (1, 3, 72, "bf16"), (2, 20, 64, "bf16"), (4, 40, 128, "f16"),
+                                               (4, 33, 128, "bf16"), (3, 9, 256, "f16"), (8, 6, 200, "bf16")])
+@pytest.mark.parametrize("what", [NAN, np.inf])
+def test_prefix_unseen_tokens(share, size, d, kind, what):
+    """Tokens of the prefix that a shorter sequence does not see, whatever they are:
+    NaN or infinite keys and values that others see, or none."""
+    rng = np.random.default_rng(size)
+    p, at = 700, 333
+    owns = [int(x) for x in rng.integers(0, 30, size)]
+    short = {1: at - p, 2: at - 13 - p, 0: -p}  # sees up to the bad token, the tile before, nothing
+    if size > 8:
+        short[size - 1] = short[size // 2] = at - 1 - p
+    for s, o in short.items():
+        owns[s] = o
+    q, cache, table, ref, lens, starts, plen = prefix_inputs(rng, [(p, owns)], 2 * share, 2, d, kind, 16, "head")
+    for c in (cache.k, cache.v):
+        c[int(ref[0, at // 16]), :, at % 16] = what
+    cache.v[int(ref[0, (at + 300) // 16]), :, 3] = what
+    got, lse = run_prefix(q, cache, table, lens, starts, plen, 0.1, "f32")
+    rows = np.array(sorted(short))
+    compare(got[rows], lse[rows], q[rows], cache, ref[rows], lens[rows], 0.1, "f32")
+    assert (got[0] == 0).all() and (lse[0] == -np.inf).all()
+    others = np.setdiff1d(np.arange(size), rows)
+    assert np.isnan(got[others]).all(axis=2).all()
+    # no sequence as long as the prefix: nothing behind the longest is a token
+    lens = np.minimum(lens, at)
+    got, lse = run_prefix(q, cache, table, lens, starts, plen, 0.1, "f32")
+    compare(got, lse, q, cache, ref, lens, 0.1, "f32")
+    # a bad value that a shorter sequence does see, and only that
+    bad = torch.zeros_like(cache.v[0, :, 0, 0])
+    bad[0] = what
+    cache.v[int(ref[0, 20]), :, 2, 1] = bad
+    lens = np.where(np.arange(size) % 2, lens, np.minimum(lens, 322))
+    got, lse = run_prefix(q, cache, table, lens, starts, plen, 0.1, "f32")
+    sees = lens > 322
+    clean = got.copy()
+    clean[sees, :share, 1] = 0
+    assert not np.isfinite(got[sees, :share, 1]).any() and np.isfinite(clean).all() and np.isfinite(lse[lens > 0]).all()
+    rows = np.flatnonzero(~sees)
+    compare(got[rows], lse[rows], q[rows], cache, ref[rows], lens[rows], 0.1, "f32")
