@@ -580,7 +580,9 @@ int s2x_beam_select(const void *logits, int32_t type, int64_t ld, int64_t n_req,
  *                 and the places that hold tokens (-1, -1, 0: nothing to copy)
  *   free_out      the pages that no row of table_out holds, nor pinned (n_pages bytes,
  *                 optional, not 0: held by others), in order; -1 behind them
- *                 (n_pages entries, the free_pages of s2x_kv_slots)
+ *                 (n_pages entries: the free_pages of s2x_kv_slots, whose n_free may
+ *                 be n_pages, since an entry of -1 is no page there; it had
+ *                 enough of them if its used[0] <= count[0])
  *   count[0]      pages in free_out, count[1] rows that get a copy
  * New pages are the lowest free ones (those of rows that are dropped among them; none
  * is a page to copy).  Where there are fewer than count[1] the last rows that want
@@ -627,11 +629,11 @@ int s2x_kv_copy_pages(const s2x_kv_cache *caches, int64_t n_cache, const int32_t
  * (the others are its sequences' own), a sequence's own tokens as the first max_own
  * behind it, a group as its first max_group sequences; sequences of no group, or
  * past those, are left out, their rows as they were.  Probabilities and sums as in
- * s2x_attn_paged, the order of the sums another.  n_group * max_group <= 65,535,
- * max_prefix and max_own <= 2^30, n_group * max_group * n_head of the cache <= 2^21
- * (a key head counted once for each 16 query heads on it).  workspace of
- * s2x_attn_paged_prefix_workspace_size() bytes (0 for shapes that are refused, and
- * for no sequences). */
+ * s2x_attn_paged, the order of the sums another.  n_seq and n_group * max_group <=
+ * 65,535, max_prefix and max_own <= 2^30, n_seq and n_group * max_group times n_head of
+ * the cache <= 2^21 (a key head counted once for each 16 query heads on it).
+ * workspace of s2x_attn_paged_prefix_workspace_size() bytes (0 for shapes that are
+ * refused, and for no sequences). */
 size_t s2x_attn_paged_prefix_workspace_size(int64_t n_group, int64_t max_group, int64_t max_prefix,
                                             int64_t max_own, int64_t n_q_head, int64_t n_kv_head,
                                             int64_t d_head);

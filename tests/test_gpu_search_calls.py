@@ -10,7 +10,7 @@ import s2x
 from decode_util import TYPES, Cache, attn_ref
 from gpu_util import assert_same, dev, empty, host, ptr, say, stream
 from test_gpu_decode import NAN, U, Q4, q4_weight, within
-from test_gpu_search import beam_case, beams_case, compare, ints, nans, prefix_inputs, rms_case, run_beam, run_fork, run_prefix, run_rms
+from test_gpu_search import beam_case, beams_case, check_beam, compare, ints, nans, prefix_inputs, rms_case, run_beam, run_fork, run_prefix, run_rms
 
 pytestmark = pytest.mark.gpu
 
@@ -360,3 +360,83 @@ def test_prefix_unseen_tokens(share, size, d, kind, what):
     assert not np.isfinite(got[sees, :share, 1]).any() and np.isfinite(clean).all() and np.isfinite(lse[lens > 0]).all()
     rows = np.flatnonzero(~sees)
     compare(got[rows], lse[rows], q[rows], cache, ref[rows], lens[rows], 0.1, "f32")
+
+
+@pytest.mark.parametrize("m,h", [((1 << 22) + 4099, 8), ((1 << 20) + 777, 520)])
+def test_rms_more_rows_than_workgroups(m, h):
+    x = torch.randn(m, h, device="cuda:0").half()
+    w = torch.randn(h, device="cuda:0")
+
+    def run(x):
+        n, k_pad = len(x), -(-h // 32) * 32
+        out = nans(n, h, dtype=torch.float16), empty((n, k_pad), torch.int8), empty((n, k_pad // 32), torch.int32)
+        s2x.call("s2x_add_rmsnorm_quantize_q8_1", ptr(x), s2x.TYPE_F16, h, ptr(x), s2x.TYPE_F16, h, h, n, ptr(w), 1e-5, None, 0, k_pad,
+                 ptr(out[1]), ptr(out[2]), ptr(out[0]), s2x.TYPE_F16, h, stream())
+        return out
+    whole = run(x)
+    for a, b in ((0, 5000), (m // 2, m // 2 + 70000), (m - 9000, m)):
+        for g, w_ in zip(whole, run(x[a:b].clone())):
+            assert torch.equal(g[a:b], w_), (a, b)
+    y = 2 * x.double()
+    y = y / torch.sqrt((y * y).mean(1, keepdim=True) + 1e-5) * w.double()
+    # (an eps of f32, inv and two products of f32, the rounding to f16)
+    assert ((whole[0].double() - y).abs() <= (2.0 ** -11 + 4 * U) * y.abs() + 2.0 ** -25).all()
+
+
+def test_rms_rows_far_apart():
+    """Rows 2^32 elements apart, the largest stride."""
+    far, h = 1 << 32, 1157
+    mem = torch.zeros(2 * far + h, dtype=torch.float16, device="cuda:0")
+    rows = torch.as_strided(mem, (3, h), (far, 1))
+    x, r, w = rms_case(1, 3, h, "f16", "f16")
+    rows.copy_(x)
+    wd, rd, y = dev(w), r.to("cuda:0"), nans(3, h)
+    s2x.call("s2x_add_rmsnorm_quantize_q8_1", ptr(mem), s2x.TYPE_F16, far, ptr(rd), s2x.TYPE_F16, h, h, 3, ptr(wd), 1e-6, ptr(mem), far,
+             0, None, None, ptr(y), 0, h, stream())
+    near, want, _, _ = run_rms(x, r, w, out="y")
+    torch.cuda.synchronize()
+    assert torch.equal(y, want) and torch.equal(rows, near)
+    assert not mem[h:far].any() and not mem[far + h:2 * far].any()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_beam_many_long_rows(kind):
+    """The longest parts of rows with the most continuations: the largest lists."""
+    n, beams, vocab = 40, 8, 131072
+    g = torch.Generator(device="cuda:0").manual_seed(3)
+    x = torch.randn(n, beams, vocab, device="cuda:0", generator=g).to(TYPES[kind])
+    x[1], x[2] = 1.5, torch.arange(vocab, device="cuda:0") / 2048  # (all equal; ascending)
+    sc = -np.arange(n * beams, dtype=np.float32).reshape(n, beams) % 7
+    got = run_beam(x, sc, 64)
+    for r in (0, 1, 2, n - 1):
+        one = run_beam(x[r:r + 1].clone(), sc[r:r + 1], 64)
+        assert_same(got[0][r], one[0][0] + r * beams, f"parent {r}")
+        assert_same(got[1][r], one[1][0], f"token {r}")
+        # (other parts of a row: other orders of its sum)
+        assert np.allclose(got[2][r], one[2][0], rtol=0, atol=2 * (128 + 60) * U + 4 * U * 20)
+    check_beam(x[3:5].cpu(), sc[3:5], 64)
+
+
+def test_prefix_most_sequences():
+    """65,535 sequences, more own tokens' parts than workgroups."""
+    n, h, d, page, own = 65535, 32, 64, 16, 300
+    rng = np.random.default_rng(6)
+    cache = Cache(500, h, page, d, "f16")
+    for c in (cache.k, cache.v):
+        c.copy_(torch.randn(c.shape, device="cuda:0"))
+    lens = rng.integers(0, own + 1, n)
+    lens[-1], lens[0] = own, 1
+    table = rng.integers(0, 500, (n, -(-own // page))).astype(np.int32)
+    q = torch.randn(n, h * d, device="cuda:0").half()
+    t = [ints(a) for a in (table, lens, np.arange(0, n + 1, 3), np.zeros(n // 3))]
+    size = s2x.lib.s2x_attn_paged_prefix_workspace_size(n // 3, 3, 0, own, h, h, d)
+    say(f"prefix: {n} sequences, workspace {size >> 20} MiB")
+    ws, out, lse = torch.full((size,), 0xff, dtype=torch.uint8, device="cuda:0"), nans(n, h * d, dtype=torch.float16), nans(n, h)
+    s2x.call("s2x_attn_paged_prefix", ptr(q), h * d, n, None, cache.ref(), ptr(t[0]), table.shape[1], ptr(t[1]), n, ptr(t[2]), ptr(t[3]),
+             n // 3, 3, 0, own, h, 0.1, ptr(out), s2x.TYPE_F16, h * d, ptr(lse), ptr(ws), size, stream())
+    torch.cuda.synchronize()
+    assert torch.isfinite(out).all()
+    rows = np.concatenate([[0, 1, 2, n - 2, n - 1], rng.integers(0, n, 60)])
+    at = torch.from_numpy(rows).to("cuda:0")
+    compare(out[at].double().cpu().numpy().reshape(-1, h, d), host(lse[at]), q[at].cpu().reshape(-1, h, d), cache, table[rows], lens[rows],
+            0.1, "f16")

@@ -164,6 +164,7 @@ def prefix(**kw):
     (dict(cache=None), INVALID), (dict(n_group=-1), INVALID), (dict(max_group=-1), INVALID), (dict(max_prefix=-1), INVALID),
     (dict(max_own=-1), INVALID), (dict(n_group=65536), UNSUPPORTED), (dict(n_group=300, max_group=300), UNSUPPORTED),
     (dict(max_prefix=(1 << 30) + 1), UNSUPPORTED), (dict(max_own=(1 << 30) + 1), UNSUPPORTED), (dict(n_q_head=3), INVALID),
+    (dict(n_seq=65536), UNSUPPORTED), (dict(n_seq=40000, n_q_head=1024), UNSUPPORTED),
     (dict(n_q_head=0), INVALID), (dict(n_q_head=1026), UNSUPPORTED), (dict(n_seq=-1), INVALID), (dict(n_row=-1), INVALID),
     (dict(out_type=BF16), UNSUPPORTED), (dict(out_type=9), UNSUPPORTED), (dict(ld_table=-1), INVALID),
     (dict(ld_q=504), INVALID), (dict(ld_q=516), INVALID), (dict(ld_out=504), INVALID), (dict(q=None), INVALID),
