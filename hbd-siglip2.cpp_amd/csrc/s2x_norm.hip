@@ -4,6 +4,10 @@
 //
 // A row lies in the registers of its waves, 8 columns a lane and piece, from its
 // load to its last store: each input is read once and each output written once.
+// Bound by the bytes: 8,191 rows of 4,096, all bf16, 52 us = 5.2 TB/s, what a large
+// copy reaches; 8,191 of 2,048 in f32 to Q8_1 41 us = 5.3; one row of 1,152 3.2 us, an
+// empty launch about 2.  Rows of more than 16,384 columns, 32 a lane, spill: 500 of 32,768
+// f32 76 us = 2.8.
 // The mean is a sum in f64 (a row's f32 sum would be off by some 2^-21, and
 // overflow from |h| = 2^64 on), inv is rounded once to f32.  A Q8_1 block is a
 // quad's 32 columns.
@@ -161,6 +165,10 @@ static hipError_t run_rms(const AddRmsNorm &p, hipStream_t stream) {
     hipLaunchKernelGGL(kern, dim3((unsigned)(wgs < most ? wgs : most)), dim3(NW == 1 ? 256 : NW * WAVE), 0, stream, p);
     return hipGetLastError();
 }
+// 8 columns a lane up to 4,096, 16 above: workgroups of which several fit a CU, so
+// that some load while others are at their barrier.  bf16, 8,191 rows of 4,096: 8 waves
+// of 8 columns 57.2 us, 4 of 16 58.8; 4,000 of 5,120: 8 of 16 45.0, 16 of 8 55.7, 4 of 32
+// 66.7; 1,000 of 16,384: 16 of 16 28.2, 8 of 32 32.2; 30,000 of 480: a wave 23.6, two 34.6.
 template <typename TX, typename TR>
 static hipError_t run_rms_h(const AddRmsNorm &p, hipStream_t stream) {
     const int cols = p.qs ? p.K_pad : p.H;
@@ -168,7 +176,7 @@ static hipError_t run_rms_h(const AddRmsNorm &p, hipStream_t stream) {
     if (cols <= 1024) return run_rms<TX, TR, 1, 2>(p, stream);
     if (cols <= 2048) return run_rms<TX, TR, 1, 4>(p, stream);
     if (cols <= 4096) return run_rms<TX, TR, 1, 8>(p, stream);
-    if (cols <= 8192) return run_rms<TX, TR, 1, 16>(p, stream);
+    if (cols <= 8192) return run_rms<TX, TR, 2, 8>(p, stream);
     if (cols <= 16384) return run_rms<TX, TR, 2, 16>(p, stream);
     return run_rms<TX, TR, 4, 16>(p, stream);
 }

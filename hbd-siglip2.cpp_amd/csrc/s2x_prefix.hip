@@ -7,8 +7,17 @@
 // The prefix's keys and values are read once for all query heads of the group that
 // share a key head (its columns).  Up to 16 columns take the kernel of the decode
 // step's attention, a wave a tile (s2x_paged.h), and so do the own tokens.  More
-// columns: k_attn_prefix, whose waves share tiles of 64 keys in LDS and have 16 or
-// 32 columns each.  All leave sums in the workspace; k_prefix_join adds them.
+// columns: px_wide, whose waves share tiles of 32 keys in LDS and have 16 or 32
+// columns each.  All leave sums in the workspace; k_prefix_join adds them.
+//
+// Measured (both launches): 3 groups of 4 on up to 700 tokens, 16 heads of 72, 11.9 us,
+// latency and launches; 9 groups of up to 30, up to 6,000 tokens, 32 / 8 heads of 128, 71
+// us = 2.3 TB/s, the own tokens 15 to 20 of it; 1 group of 64 on 32,001 tokens, bf16, 91 to
+// 98 us = 345 to 370 TFLOP/s of the two products counted once (three terms of a
+// probability make the second one three).  px_wide is bound by the issue of its
+// instructions: a step of 32 keys and 128 columns takes a workgroup some 3,000 cycles, of
+// which the matrix units work 46 %, with two workgroups a CU for the other half.  Each
+// 256 registers; 8 waves of 16 columns in 128 spill (109 us against 79 of that time's).
 #include "s2x_paged.h"
 
 namespace s2x {
@@ -116,7 +125,7 @@ __device__ __forceinline__ void px_wide(const AttnPrefix &args, const PxPlan &P,
         for (int i = 0; i < PER; ++i) e.piece[i] = row[min((int)((uint32_t)(t0 + key_of(i)) >> shift), last)];
         return e;
     };
-    // Two tiles under way where the registers allow: a step of a workgroup takes a
+    // Two tiles under way where the registers allow: a step of a workgroup takes over a
     // microsecond, a load from memory two under full use.  Where a page is none the
     // first one is loaded, and zeros are stored.
     constexpr int AHEAD = DC > 4 ? 1 : 2;
@@ -385,12 +394,12 @@ __device__ __forceinline__ v4f px_seen_only(const AttnPaged &p, int seq, int hk,
 }
 
 // The parts of a sequence's prefix and of its own tokens joined, as k_attn_join
-// does the chunks: a workgroup per query head and 4 LANES values of it.
+// does the chunks: a workgroup per query head and 128 values of it.
 // The first PXJ_AHEAD parts of a thread are loaded before their number is known.
 constexpr int PXJ_AHEAD = 4;
-template <typename TC, int LANES, int NT>
+template <typename TC, int NT>
 __global__ __launch_bounds__(NT) void k_prefix_join(AttnPrefix args, PxPlan P) {
-    constexpr int GROUPS = NT / LANES;
+    constexpr int LANES = 32, GROUPS = NT / LANES;
     __shared__ __align__(16) float part[GROUPS][LANES * 4 + 4];
     __shared__ float gm[GROUPS], gl[GROUPS];
     const AttnPaged &p = args.a;
@@ -484,14 +493,21 @@ static int64_t px_round(int64_t v, int64_t to, int64_t lo, int64_t hi) {
     v = v < lo ? lo : v > hi ? hi : v;
     return (v + to - 1) / to * to;
 }
+// Chunks of the prefixes for about 512 workgroups, what the card holds of k_attn_prefix
+// at once (1 group of 64 on 32,001 tokens: for 256, 512, 1,024, 2,048 107, 97.5, 108, 132 us;
+// 2 of 32 on 12,000: for 512 54, 1,024 59; 9 ragged ones 88, 70.7, 71.5).  Own tokens in
+// chunks of 32, up to 128 where that is more than 4,096 waves (12 sequences of 16 heads with
+// up to 60: 32 a chunk 11.9 us, 128 15.6; 140 of 8 with up to 900: 83 and 72.6), and at most
+// 48 of them a sequence.  Columns of a wave: 16 up to 64 of a group, 32 from there (9 ragged
+// groups with 16 83.4 us, with 32 73.0; 1 of 64: 112 and 97.7).
 static PxPlan px_plan(int64_t n_group, int64_t max_group, int64_t max_prefix, int64_t max_own, int64_t n_q_head,
                       int64_t n_kv_head, int64_t d_head) {
     PxPlan P;
     const int64_t share = n_q_head / n_kv_head, cols = share * max_group;
     P.nc = cols <= 16 ? 0 : cols > 64 && d_head <= 128 ? 2 : 1;
     P.tiles = P.nc ? (int)((cols + 64 * P.nc - 1) / (64 * P.nc)) : 1;
-    const int64_t units = n_group * n_kv_head * P.tiles, most = 1 << 20, wgs = 512 * (n_group < 2 ? n_group : 2);
-    int64_t c = px_round(max_prefix * units / wgs, 128, 128, most);
+    const int64_t units = n_group * n_kv_head * P.tiles, most = 1 << 20;
+    int64_t c = px_round(max_prefix * units / 512, 128, 128, most);
     if (units * ((max_prefix + c - 1) / c) > 1 << 22) c = px_round(max_prefix * units >> 21, 128, 128, 1 << 30);
     P.chunk_p = (int)c;
     P.split_p = (int)((max_prefix + c - 1) / c);
@@ -524,13 +540,12 @@ static hipError_t run_prefix(const AttnPrefix &p, hipStream_t stream) {
     const int lds = w > v ? (w > o ? w : o) : (v > o ? v : o);
     auto kern = P.nc ? k_attn_prefix<TC, DC, EXACT, KT, true> : k_attn_prefix<TC, DC, EXACT, KT, false>;
     hipLaunchKernelGGL(kern, dim3((unsigned)(P.wgs_p + P.wgs_o)), dim3(PX_NT), lds, stream, p, P);
-    const bool many = (int64_t)p.a.n_seq * p.a.n_q_head >= 512, few = P.parts() <= 16;
-    // (many rows: a wave each, so that all are at work at once; 64 sequences of 32 heads
-    // and 2 parts 7.1 us, in four waves 8.5)
-    const int width = few || many ? 128 : 32;
-    auto join = width == 32 ? k_prefix_join<TC, 8, 256> : many ? k_prefix_join<TC, 32, 64> : k_prefix_join<TC, 32, 256>;
-    hipLaunchKernelGGL(join, dim3(p.a.n_q_head * ((d + width - 1) / width), p.a.n_seq), dim3(many && width > 32 ? 64 : 256), 0,
-                       stream, p, P);
+    // (a wave a row and 128 values where rows are many, so that all are at work at once: 74
+    // sequences of 32 heads and 2 parts 6.8 us, in four waves 8.5; few rows: four, for
+    // their parts' sake)
+    const bool many = (int64_t)p.a.n_seq * p.a.n_q_head >= 512;
+    auto join = many ? k_prefix_join<TC, 64> : k_prefix_join<TC, 256>;
+    hipLaunchKernelGGL(join, dim3(p.a.n_q_head * ((d + 127) / 128), p.a.n_seq), dim3(many ? 64 : 256), 0, stream, p, P);
     return hipGetLastError();
 }
 template <typename TC>
