@@ -144,23 +144,27 @@ struct BmPlan {
     int loads, span, n_split;
 };
 // Parts of a row: up to 16 loads a lane, fewer where rows are few, as long as there
-// are less than 1,024 workgroups.  2, 4, 8, 16 loads: 4 rows of 32,000 12.7, 13.3, 13.8,
-// 14.7 us (both launches); 512 rows of 256,000 bf16 137, 91, 70, 64.
-static BmPlan bm_plan(int64_t rows, int64_t n_vocab, int per) {
-    const int64_t step = (int64_t)BM_NT * per;
+// are less than 1,024 workgroups and the join takes a request's candidates in one
+// round.  2, 4, 8, 16 loads, both launches: 1 request of 4 beams of 32,000 f32 12.6, 13.2,
+// 14.0, 14.7 us; 1 of 8 of 100,000 (8 out) 22.2, 16.5, 16.9, 17.8; 13 of 12 of 50,000 (24
+// out) 54.7, 36.0, 28.6, 29.1; 1 of 32 of 32,000 (64 out) 182, 99, 62, 47; 64 of 8 of
+// 256,000 bf16 (16 out) 137, 91, 70, 64.
+constexpr int BJ_PER = 8, BJ_TILE = BM_NT * BJ_PER;  // candidates of a round
+static BmPlan bm_plan(int64_t n_req, int64_t n_beam, int64_t n_vocab, int64_t n_out, int per) {
+    auto parts = [&](int loads) { return (n_vocab + loads * BM_NT * per - 1) / (loads * BM_NT * per); };
     int loads = 16;
-    while (loads > 2 && rows * ((n_vocab + loads * step - 1) / (loads * step)) < 1024) loads /= 2;
-    const int64_t n = (n_vocab + loads * step - 1) / (loads * step);
+    while (loads > 2 && n_req * n_beam * parts(loads) < 1024 && n_beam * n_out * parts(loads / 2) <= BJ_TILE) loads /= 2;
+    const int64_t n = parts(loads);
     int64_t span = (n_vocab + n - 1) / n;
     span = (span + per - 1) / per * per;
     return BmPlan{loads, (int)span, (int)((n_vocab + span - 1) / span)};
 }
-static int64_t bm_most_splits(int64_t rows, int64_t n_vocab) {  // whatever the type
-    const int a = bm_plan(rows, n_vocab, 4).n_split, b = bm_plan(rows, n_vocab, 8).n_split;
+static int64_t bm_most_splits(int64_t n_req, int64_t n_beam, int64_t n_vocab, int64_t n_out) {  // whatever the type
+    const int a = bm_plan(n_req, n_beam, n_vocab, n_out, 4).n_split, b = bm_plan(n_req, n_beam, n_vocab, n_out, 8).n_split;
     return a > b ? a : b;
 }
 size_t beam_select_workspace(int64_t n_req, int64_t n_beam, int64_t n_vocab, int64_t n_out) {
-    const int64_t parts = n_req * n_beam * bm_most_splits(n_req * n_beam, n_vocab);
+    const int64_t parts = n_req * n_beam * bm_most_splits(n_req, n_beam, n_vocab, n_out);
     return (size_t)parts * (sizeof(BmSum) + n_out * sizeof(BmCand));
 }
 __device__ __forceinline__ BmSum *bm_sums(const BeamSelect &p) { return (BmSum *)p.ws; }
@@ -312,7 +316,6 @@ __global__ __launch_bounds__(BM_NT) void k_beam_rows(BeamSelect p, int span, int
     }
 }
 
-constexpr int BJ_PER = 8, BJ_TILE = BM_NT * BJ_PER;  // candidates of a round
 constexpr int BJ_CAP = 1024, BJ_SUMS = 1024;         // members of a list, sums kept in LDS
 static_assert((BEAM_MAX_OUT - 1) * (BJ_PER + 1) + BM_WAVES * BEAM_MAX_OUT <= BJ_CAP, "the list's largest length");
 
@@ -481,7 +484,7 @@ __global__ __launch_bounds__(BM_NT) void k_beam_join(BeamSelect p, int n_split) 
 template <typename T>
 static hipError_t run_beam(const BeamSelect &p, hipStream_t stream) {
     const int rows = p.n_req * p.n_beam;
-    const BmPlan P = bm_plan(rows, p.n_vocab, Bm<T>::per);
+    const BmPlan P = bm_plan(p.n_req, p.n_beam, p.n_vocab, p.n_out, Bm<T>::per);
     const int cap = (p.n_out - 1) * P.loads * Bm<T>::per + BM_WAVES * p.n_out;
     auto kern = P.loads == 16 ? k_beam_rows<T, 16> : P.loads == 8 ? k_beam_rows<T, 8> : P.loads == 4 ? k_beam_rows<T, 4>
                                                                                                      : k_beam_rows<T, 2>;
