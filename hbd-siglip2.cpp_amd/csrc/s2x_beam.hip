@@ -143,17 +143,18 @@ struct BmSum {
 struct BmPlan {
     int loads, span, n_split;
 };
-// Parts of a row: up to 16 loads a lane, fewer where rows are few, as long as there
-// are less than 1,024 workgroups and the join takes a request's candidates in one
+// Parts of a row: up to 16 loads a lane, fewer where rows are few, as long as that
+// takes no more than 512 workgroups and the join has a request's candidates in one
 // round.  2, 4, 8, 16 loads, both launches: 1 request of 4 beams of 32,000 f32 12.6, 13.2,
-// 14.0, 14.7 us; 1 of 8 of 100,000 (8 out) 22.2, 16.5, 16.9, 17.8; 13 of 12 of 50,000 (24
-// out) 54.7, 36.0, 28.6, 29.1; 1 of 32 of 32,000 (64 out) 182, 99, 62, 47; 64 of 8 of
-// 256,000 bf16 (16 out) 137, 91, 70, 64.
+// 14.0, 14.7 us; 14 of 5 of 56,284 20.9, 18.8, 17.9, 19.0; 60 of 2 of 30,000 18.1, 15.8,
+// 15.0, 15.3; 1 of 8 of 100,000 (8 out) 22.2, 16.5, 16.9, 17.8; 13 of 12 of 50,000 (24 out)
+// 54.7, 36.0, 28.6, 29.1; 1 of 32 of 32,000 (64 out) 182, 99, 62, 47; 64 of 8 of 256,000
+// bf16 (16 out) 137, 91, 70, 64.
 constexpr int BJ_PER = 8, BJ_TILE = BM_NT * BJ_PER;  // candidates of a round
 static BmPlan bm_plan(int64_t n_req, int64_t n_beam, int64_t n_vocab, int64_t n_out, int per) {
     auto parts = [&](int loads) { return (n_vocab + loads * BM_NT * per - 1) / (loads * BM_NT * per); };
     int loads = 16;
-    while (loads > 2 && n_req * n_beam * parts(loads) < 1024 && n_beam * n_out * parts(loads / 2) <= BJ_TILE) loads /= 2;
+    while (loads > 2 && n_req * n_beam * parts(loads / 2) <= 512 && n_beam * n_out * parts(loads / 2) <= BJ_TILE) loads /= 2;
     const int64_t n = parts(loads);
     int64_t span = (n_vocab + n - 1) / n;
     span = (span + per - 1) / per * per;

@@ -92,16 +92,16 @@ __device__ __forceinline__ void quantize8(const AddRmsNorm &p, int64_t row, cons
 }
 
 // NW waves a row, NV pieces of 8 columns a lane.  One wave a row: four rows a
-// workgroup.
-template <typename TX, typename TR, int NV, int NW>
+// workgroup; LN < 64: LN lanes a row.
+template <typename TX, typename TR, int NV, int NW, int LN = WAVE>
 __global__ __launch_bounds__(NW == 1 ? 256 : NW * WAVE) void k_add_rmsnorm(AddRmsNorm p) {
     __shared__ double part[2][NW];
-    constexpr int ROWS = NW == 1 ? 4 : 1, LANES = NW * WAVE;
-    const int lane = NW == 1 ? threadIdx.x & 63 : threadIdx.x, wave = threadIdx.x >> 6;
+    constexpr int LANES = NW * LN, ROWS = NW == 1 ? 256 / LN : 1;
+    const int lane = NW == 1 ? threadIdx.x % LN : threadIdx.x, wave = threadIdx.x >> 6;
     const int H = p.H, cols = p.qs ? p.K_pad : H;
     const int64_t step = (int64_t)gridDim.x * ROWS;
     int turn = 0;
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + (NW == 1 ? wave : 0); row < p.M; row += step, turn ^= 1) {
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + (NW == 1 ? threadIdx.x / LN : 0); row < p.M; row += step, turn ^= 1) {
         float h[NV][8], w[NV][8];
         const TX *x = (const TX *)p.x + row * p.ld_x;
         const TR *r = (const TR *)p.resid + row * p.ld_resid;
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * WAVE) void k_add_rmsnorm(AddRm
 #pragma unroll
             for (int n = 0; n < NV; ++n) load8(w[n], p.w, 8 * (n * LANES + lane), H);
         }
-        s = wave_dsum(s);
+        s = LN == WAVE ? wave_dsum(s) : group_dsum<LN>(s);
         if constexpr (NW > 1) {
             if ((threadIdx.x & 63) == 0) part[turn][wave] = s;
             __syncthreads();  // (the other half is written next: one barrier a row)
@@ -158,20 +158,26 @@ __global__ __launch_bounds__(NW == 1 ? 256 : NW * WAVE) void k_add_rmsnorm(AddRm
     }
 }
 
-template <typename TX, typename TR, int NV, int NW>
+template <typename TX, typename TR, int NV, int NW, int LN = WAVE>
 static hipError_t run_rms(const AddRmsNorm &p, hipStream_t stream) {
-    const int64_t wgs = NW == 1 ? (p.M + 3) / 4 : p.M, most = 1 << 20;
-    auto kern = k_add_rmsnorm<TX, TR, NV, NW>;
+    constexpr int ROWS = 256 / LN;
+    const int64_t wgs = NW == 1 ? (p.M + ROWS - 1) / ROWS : p.M, most = 1 << 20;
+    auto kern = k_add_rmsnorm<TX, TR, NV, NW, LN>;
     hipLaunchKernelGGL(kern, dim3((unsigned)(wgs < most ? wgs : most)), dim3(NW == 1 ? 256 : NW * WAVE), 0, stream, p);
     return hipGetLastError();
 }
-// 8 columns a lane up to 4,096, 16 above: workgroups of which several fit a CU, so
-// that some load while others are at their barrier.  bf16, 8,191 rows of 4,096: 8 waves
-// of 8 columns 57.2 us, 4 of 16 58.8; 4,000 of 5,120: 8 of 16 45.0, 16 of 8 55.7, 4 of 32
-// 66.7; 1,000 of 16,384: 16 of 16 28.2, 8 of 32 32.2; 30,000 of 480: a wave 23.6, two 34.6.
+// 8 columns a lane up to 4,096, in as much of a wave or as many as that takes, 16 above:
+// workgroups of which several fit a CU, so that some load while others are at their
+// barrier.  bf16, 8,191 rows of 4,096: 8 waves of 8 columns 57.2 us, 4 of 16 58.8; 4,000
+// of 5,120: 8 of 16 45.0, 16 of 8 55.7, 4 of 32 66.7; 1,000 of 16,384: 16 of 16 28.2, 8 of 32 32.2; 30,000 of 480: a wave 23.6, two 34.6;
+// 60,000 of 256: half a wave 21.9, a wave 31.8; 100,000 of 128: a quarter 19.2, a wave 48.1;
+// 300,000 of 64: an eighth 32.2, a wave 147.
 template <typename TX, typename TR>
 static hipError_t run_rms_h(const AddRmsNorm &p, hipStream_t stream) {
     const int cols = p.qs ? p.K_pad : p.H;
+    if (cols <= 64) return run_rms<TX, TR, 1, 1, 8>(p, stream);
+    if (cols <= 128) return run_rms<TX, TR, 1, 1, 16>(p, stream);
+    if (cols <= 256) return run_rms<TX, TR, 1, 1, 32>(p, stream);
     if (cols <= 512) return run_rms<TX, TR, 1, 1>(p, stream);
     if (cols <= 1024) return run_rms<TX, TR, 1, 2>(p, stream);
     if (cols <= 2048) return run_rms<TX, TR, 1, 4>(p, stream);

@@ -10,7 +10,7 @@ import s2x
 from decode_util import TYPES, Cache, attn_ref
 from gpu_util import assert_same, dev, empty, host, ptr, say, stream
 from test_gpu_decode import NAN, U, Q4, q4_weight, within
-from test_gpu_search import beam_case, beams_case, check_beam, compare, ints, nans, prefix_inputs, rms_case, run_beam, run_fork, run_prefix, run_rms
+from test_gpu_search import beam_case, beams_case, check_beam, check_rms, compare, ints, nans, prefix_inputs, rms_case, run_beam, run_fork, run_prefix, run_rms
 
 pytestmark = pytest.mark.gpu
 
@@ -381,6 +381,14 @@ def test_rms_more_rows_than_workgroups(m, h):
     y = y / torch.sqrt((y * y).mean(1, keepdim=True) + 1e-5) * w.double()
     # (an eps of f32, inv and two products of f32, the rounding to f16)
     assert ((whole[0].double() - y).abs() <= (2.0 ** -11 + 4 * U) * y.abs() + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("m", [1, 7, 131])
+@pytest.mark.parametrize("h", [8, 63, 64, 65, 127, 128, 129, 255, 256, 257, 4097, 8192, 8193])
+def test_rms_widths_around_the_rules(m, h):
+    """Rows of an eighth of a wave and up, the last workgroup not full."""
+    for x_kind, r_kind in (("f32", "f32"), ("bf16", "bf16")):
+        check_rms(*rms_case(m * h, m, h, x_kind, r_kind))
 
 
 def test_rms_rows_far_apart():
