@@ -95,16 +95,16 @@ __device__ __forceinline__ double bm_value(uint64_t k) {
     return __builtin_bit_cast(double, k >> 63 ? k & ~(1ull << 63) : ~k);
 }
 
-// The K-th largest of BM_NT keys, 4 of them in each lane of the wave, which are
+// The K-th largest of 64 N keys, N of them in each lane of the wave, which are
 // the same in every wave; its last `low` bits as its first bit tells.
-template <typename U>
-__device__ __forceinline__ U bm_kth(const U (&k)[4], int K, int low) {
+template <typename U, int N>
+__device__ __forceinline__ U bm_kth(const U (&k)[N], int K, int low) {
     U t = 0;
     for (int b = 8 * sizeof(U) - 1; b >= low; --b) {
         const U up = t | (U)1 << b;
         int n = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k[i] >= up));
+        for (int i = 0; i < N; ++i) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k[i] >= up));
         if (n >= K) t = up;
     }
     if (!(t >> (8 * sizeof(U) - 1))) t |= ((U)1 << low) - 1;
@@ -148,9 +148,9 @@ struct BmPlan {
 // round.  2, 4, 8, 16 loads, both launches: 1 request of 4 beams of 32,000 f32 12.6, 13.2,
 // 14.0, 14.7 us; 14 of 5 of 56,284 20.9, 18.8, 17.9, 19.0; 60 of 2 of 30,000 18.1, 15.8,
 // 15.0, 15.3; 1 of 8 of 100,000 (8 out) 22.2, 16.5, 16.9, 17.8; 13 of 12 of 50,000 (24 out)
-// 54.7, 36.0, 28.6, 29.1; 1 of 32 of 32,000 (64 out) 182, 99, 62, 47; 64 of 8 of 256,000
+// 54.7, 36.0, 28.6, 29.1; 1 of 32 of 32,000 (64 out) 86, 51, 35, 38; 64 of 8 of 256,000
 // bf16 (16 out) 137, 91, 70, 64.
-constexpr int BJ_PER = 8, BJ_TILE = BM_NT * BJ_PER;  // candidates of a round
+constexpr int BJ_PER = 8, BJ_TILE = BM_NT * BJ_PER;  // candidates of a round of 256 threads
 static BmPlan bm_plan(int64_t n_req, int64_t n_beam, int64_t n_vocab, int64_t n_out, int per) {
     auto parts = [&](int loads) { return (n_vocab + loads * BM_NT * per - 1) / (loads * BM_NT * per); };
     int loads = 16;
@@ -317,13 +317,15 @@ __global__ __launch_bounds__(BM_NT) void k_beam_rows(BeamSelect p, int span, int
     }
 }
 
-constexpr int BJ_CAP = 1024, BJ_SUMS = 1024;         // members of a list, sums kept in LDS
-static_assert((BEAM_MAX_OUT - 1) * (BJ_PER + 1) + BM_WAVES * BEAM_MAX_OUT <= BJ_CAP, "the list's largest length");
+constexpr int BJ_SUMS = 1024;  // sums kept in LDS
 
-__global__ __launch_bounds__(BM_NT) void k_beam_join(BeamSelect p, int n_split) {
+template <int NT>
+__global__ __launch_bounds__(NT) void k_beam_join(BeamSelect p, int n_split) {
+    constexpr int WAVES = NT / WAVE, TILE = NT * BJ_PER, BJ_CAP = NT == 256 ? 1024 : 2048;  // members of a list
+    static_assert((BEAM_MAX_OUT - 1) * (BJ_PER + 1) + WAVES * BEAM_MAX_OUT <= BJ_CAP, "the list's largest length");
     __shared__ double add[BEAM_MAX_OUT];  // score - lse of the beams; -inf: none
     __shared__ uint8_t state[BEAM_MAX_OUT];
-    __shared__ uint64_t tops[BM_NT], lk[BJ_CAP];
+    __shared__ uint64_t tops[NT], lk[BJ_CAP];
     __shared__ int32_t lp[BJ_CAP], lt[BJ_CAP], lb[BJ_CAP];
     __shared__ uint64_t bk[BEAM_MAX_OUT];  // the best so far, in order
     __shared__ int32_t bt[BEAM_MAX_OUT], bb[BEAM_MAX_OUT];
@@ -337,17 +339,17 @@ __global__ __launch_bounds__(BM_NT) void k_beam_join(BeamSelect p, int n_split) 
     // is there, not used), the first round's candidates
     const bool kept = n_sum <= BJ_SUMS;
     if (kept)
-        for (int i = tid; i < n_sum; i += BM_NT) ls[i] = sums[i];
+        for (int i = tid; i < n_sum; i += NT) ls[i] = sums[i];
     BmCand first[BJ_PER];
 #pragma unroll
-    for (int i = 0; i < BJ_PER; ++i) first[i] = cands[min(i * BM_NT + tid, all - 1)];
+    for (int i = 0; i < BJ_PER; ++i) first[i] = cands[min(i * NT + tid, all - 1)];
     if (tid < p.n_beam) state[tid] = bm_state(p, req * p.n_beam + tid);
     if (tid < K) {
         bk[tid] = bm_key(-(double)INFINITY);
         bt[tid] = bb[tid] = -1;
     }
     __syncthreads();
-    for (int b = wave; b < p.n_beam; b += BM_WAVES) {
+    for (int b = wave; b < p.n_beam; b += WAVES) {
         const int st = state[b];
         const BmSum *from = kept ? ls + b * n_split : sums + (int64_t)b * n_split;
         float top = -INFINITY;
@@ -367,8 +369,8 @@ __global__ __launch_bounds__(BM_NT) void k_beam_join(BeamSelect p, int n_split) 
             add[b] = st == 2 ? score : st == 1 && fabs(lse) < INFINITY ? score - lse : -INFINITY;
         }
     }
-    const int step_b = BM_NT / per_beam, step_r = BM_NT - step_b * per_beam;
-    for (int e0 = 0; e0 < all; e0 += BJ_TILE) {
+    const int step_b = NT / per_beam, step_r = NT - step_b * per_beam;
+    for (int e0 = 0; e0 < all; e0 += TILE) {
         __syncthreads();
         if (tid == 0) count = ties = 0;
         // this round's candidates, and the best of those before as places below
@@ -397,7 +399,7 @@ __global__ __launch_bounds__(BM_NT) void k_beam_join(BeamSelect p, int n_split) 
             }
             key[i] = none;
             tok[i] = beam[i] = -1;
-            const int e = e0 + (i - 1) * BM_NT + tid;
+            const int e = e0 + (i - 1) * NT + tid;
             if (e >= all) continue;
             beam[i] = b;
             if (state[b] == 2) {
@@ -418,10 +420,10 @@ __global__ __launch_bounds__(BM_NT) void k_beam_join(BeamSelect p, int n_split) 
         __syncthreads();
         // a bound by the upper halves of the keys first: enough unless more keys
         // than the list takes share the bound's (many equal scores), then by whole keys
-        uint64_t k4[4];
-        uint32_t h4[4];
+        uint64_t k4[WAVES];
+        uint32_t h4[WAVES];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < WAVES; ++i) {
             k4[i] = tops[i * WAVE + lane];
             h4[i] = (uint32_t)(k4[i] >> 32);
         }
@@ -429,7 +431,7 @@ __global__ __launch_bounds__(BM_NT) void k_beam_join(BeamSelect p, int n_split) 
         auto put = [&](int i) {
             const int at = atomicAdd(&count, 1);
             lk[at] = key[i];
-            lp[at] = i * BM_NT + tid;
+            lp[at] = i * NT + tid;
             lt[at] = tok[i];
             lb[at] = beam[i];
         };
@@ -457,7 +459,7 @@ __global__ __launch_bounds__(BM_NT) void k_beam_join(BeamSelect p, int n_split) 
         }
         __syncthreads();
         const int C = min(count, BJ_CAP);
-        for (int e = tid >> 2; e < C; e += BM_NT / 4) {
+        for (int e = tid >> 2; e < C; e += NT / 4) {
             const uint64_t k = lk[e];
             const int at = lp[e];
             const int rank = bm_rank(C, [&](int q) { return lk[q] > k || (lk[q] == k && lp[q] < at); });
@@ -467,7 +469,7 @@ __global__ __launch_bounds__(BM_NT) void k_beam_join(BeamSelect p, int n_split) 
                 bb[rank] = lb[e];
             }
         }
-        for (int e = C + tid; e < K; e += BM_NT) {
+        for (int e = C + tid; e < K; e += NT) {
             bk[e] = none;
             bt[e] = bb[e] = -1;
         }
@@ -490,7 +492,10 @@ static hipError_t run_beam(const BeamSelect &p, hipStream_t stream) {
     auto kern = P.loads == 16 ? k_beam_rows<T, 16> : P.loads == 8 ? k_beam_rows<T, 8> : P.loads == 4 ? k_beam_rows<T, 4>
                                                                                                      : k_beam_rows<T, 2>;
     hipLaunchKernelGGL(kern, dim3(P.n_split, rows), dim3(BM_NT), (size_t)cap * 8, stream, p, P.span, P.n_split, cap);
-    hipLaunchKernelGGL(k_beam_join, dim3(p.n_req), dim3(BM_NT), 0, stream, p, P.n_split);
+    // (1,024 threads where 256 need more than a round: 7 requests of 32 beams of 4 parts of
+    // 64 candidates 48.6 us, both launches, 75.5 with 256; 64 of 8 of 8 of 16 71.8 and 63.8)
+    const bool wide = (int64_t)p.n_beam * P.n_split * p.n_out > BJ_TILE;
+    hipLaunchKernelGGL(wide ? k_beam_join<1024> : k_beam_join<256>, dim3(p.n_req), dim3(wide ? 1024 : 256), 0, stream, p, P.n_split);
     return hipGetLastError();
 }
 hipError_t launch_beam_select(const BeamSelect &p, hipStream_t stream) {

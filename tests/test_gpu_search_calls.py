@@ -425,6 +425,17 @@ def test_beam_many_long_rows(kind):
     check_beam(x[3:5].cpu(), sc[3:5], 64)
 
 
+@pytest.mark.parametrize("n,beams,vocab,kind,n_out", [(2, 32, 40000, "f32", 64), (1, 64, 100000, "bf16", 64), (3, 9, 270000, "f16", 60)])
+def test_beam_joins_of_many_candidates(n, beams, vocab, kind, n_out):
+    """More candidates than a round of the join takes, of 256 threads and of 1,024; equal
+    ones among them."""
+    x, sc = beam_case(beams, n, beams, vocab, kind)
+    check_beam(x, sc, n_out)
+    x[:], sc[:] = 0.5, -3.0
+    parent, token, score = run_beam(x, sc, n_out)
+    assert (parent == np.arange(n)[:, None] * beams).all() and (token == np.arange(n_out)).all()
+
+
 def test_prefix_most_sequences():
     """65,535 sequences, more own tokens' parts than workgroups."""
     n, h, d, page, own = 65535, 32, 64, 16, 300
