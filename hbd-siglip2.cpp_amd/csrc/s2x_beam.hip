@@ -226,11 +226,12 @@ __global__ __launch_bounds__(BM_NT) void k_beam_rows(BeamSelect p, int span, int
     }
     if (!Bm<T>::exact && __builtin_amdgcn_ballot_w64(!(top > 0.0f)) != 0) each_value();
     tops[tid] = top;
-    // the sum relative to the lane's largest.  2^(x L - c), c the rounded top L, with
-    // what L lacks of log2(e) and c of top L made up for in the sum: right where x is
-    // near top, and off by 2^-26 of top - x below.  Past 4,096 c lacks too much:
-    // there by differences.
-    const float L = 1.44269502e+00f, LT = 1.92596299e-08f, c = top * L;
+    // the sum relative to the lane's largest, of 2^(x L - c), c the rounded top L.  With
+    // log2(e) = L + LT the exponent is (x - top) (L + LT) = (x L - c) + (c - top L) +
+    // (x - top) LT: the second part is the same for all, a factor of the sum, and the
+    // third is left out, 2^-26 of x - top.  Past 4,096 c lacks too much: there by
+    // differences.
+    const float L = 1.44269502e+00f, c = top * L;
     float sum = 0.0f;
     if (__builtin_amdgcn_ballot_w64(fabsf(top) > 4096.0f && top != -INFINITY) == 0) {
         const float ref = top == -INFINITY ? 0.0f : c;
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(BM_NT) void k_beam_rows(BeamSelect p, int span, int
         for (int i = 0; i < NL; ++i)
 #pragma unroll
             for (int j = 0; j < PER; ++j) sum = sum + __builtin_amdgcn_exp2f(fmaf(Bm<T>::at(r[i], j), L, -ref));
-        if (top != -INFINITY) sum = sum * __builtin_amdgcn_exp2f(fmaf(-top, LT, fmaf(-top, L, c)));
+        if (top != -INFINITY) sum = sum * __builtin_amdgcn_exp2f(fmaf(-top, L, c));
     } else {
         const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll
