@@ -6,7 +6,7 @@
 // equal ones the lower beam, then the lower token.
 //
 // k_beam_rows: a workgroup's part of a row lies in registers, read once.  Its
-// lanes' maxima serve twice: as the reference of each lane's sum of exponentials,
+// lanes' maxima serve twice: for the reference of a wave's sum of exponentials,
 // and for a bound T, the n_out-th largest of the 256 maxima (found bit by bit, by
 // counting the lanes at or above).  At least n_out values are >= T, so nothing
 // below T is of use; less than n_out lanes hold values > T, so those fit a list in
@@ -111,12 +111,14 @@ __device__ __forceinline__ U bm_kth(const U (&k)[N], int K, int low) {
     return t;
 }
 
-// e^x for x <= 0
-__device__ __forceinline__ float bm_exp(float x) {
-    return __builtin_amdgcn_exp2f(fmaf(x, 1.92596299e-08f, x * 1.44269502e+00f));
+// what a sum relative to `from` counts relative to `to` >= from (-inf: an empty sum),
+// off by the exponential's 2^-23 alone: what the argument's rounding takes is made up for
+__device__ __forceinline__ double bm_scale(float from, float to) {
+    if (from == -INFINITY) return 0.0;
+    const double x = fmax(((double)from - (double)to) * 1.4426950408889634, -200.0);  // (2^-200: 0)
+    const float r = (float)x;
+    return (double)__builtin_amdgcn_exp2f(r) * fma(x - (double)r, 0.6931471805599453, 1.0);
 }
-// what a sum relative to `from` counts relative to `to` >= from (-inf: an empty sum)
-__device__ __forceinline__ float bm_scale(float from, float to) { return from == -INFINITY ? 0.0f : bm_exp(from - to); }
 
 // How many of a list's C members are ahead of member e, counted by a quad (its lanes
 // have the same e); ahead(q): whether member q is.
@@ -127,6 +129,19 @@ __device__ __forceinline__ int bm_rank(int C, F ahead) {
     for (int q = threadIdx.x & 3; q < C; q += 4) n += ahead(q);
     n += dpp_i<0xb1>(n);
     return n + dpp_i<0x4e>(n);
+}
+
+// The wave's largest, in all lanes.
+__device__ __forceinline__ float bm_wave_max(float v) {
+    const int m = __builtin_bit_cast(int, group16_max(v));
+    auto row = [&](int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(m, 16 * i)); };
+    return fmaxf(fmaxf(row(0), row(1)), fmaxf(row(2), row(3)));
+}
+// f(0) + .. + f(N - 1) in pairs.
+template <int N, typename F>
+__device__ __forceinline__ float bm_pairs(F f) {
+    if constexpr (N == 1) return f(0);
+    else return bm_pairs<N / 2>(f) + bm_pairs<N / 2>([&](int j) { return f(j + N / 2); });
 }
 
 // Workspace: candidates [row][split][K] (value, token; token -1: none), then the
@@ -226,34 +241,31 @@ __global__ __launch_bounds__(BM_NT) void k_beam_rows(BeamSelect p, int span, int
     }
     if (!Bm<T>::exact && __builtin_amdgcn_ballot_w64(!(top > 0.0f)) != 0) each_value();
     tops[tid] = top;
-    // the sum relative to the lane's largest, of 2^(x L - c), c the rounded top L.  With
+    // the sum relative to the wave's largest, of 2^(x L - c), c the rounded top L.  With
     // log2(e) = L + LT the exponent is (x - top) (L + LT) = (x L - c) + (c - top L) +
-    // (x - top) LT: the second part is the same for all, a factor of the sum, and the
-    // third is left out, 2^-26 of x - top.  Past 4,096 c lacks too much: there by
-    // differences.
-    const float L = 1.44269502e+00f, c = top * L;
-    float sum = 0.0f;
-    if (__builtin_amdgcn_ballot_w64(fabsf(top) > 4096.0f && top != -INFINITY) == 0) {
-        const float ref = top == -INFINITY ? 0.0f : c;
+    // (x - top) LT: the second part is the same for all, a factor of the sum (at most
+    // 2^-12 from 1: its series), and the third is left out, 2^-26 of x - top.  Past 4,096
+    // c lacks too much: there by differences.  A load's values are added in f32, in
+    // pairs, and those sums in f64: all one after the other in f32, values that repeat
+    // were off by up to 36 2^-24, this way by 3 (434 rows of 256,000 bf16 0.7 us slower).
+    const float wt = bm_wave_max(top), L = 1.44269502e+00f, c = wt * L;
+    double sum = 0.0;
+    if (__builtin_amdgcn_ballot_w64(fabsf(wt) > 4096.0f && wt != -INFINITY) == 0) {  // (by a ballot: 8 registers fewer)
+        const float ref = wt == -INFINITY ? 0.0f : c;
 #pragma unroll
         for (int i = 0; i < NL; ++i)
-#pragma unroll
-            for (int j = 0; j < PER; ++j) sum = sum + __builtin_amdgcn_exp2f(fmaf(Bm<T>::at(r[i], j), L, -ref));
-        if (top != -INFINITY) sum = sum * __builtin_amdgcn_exp2f(fmaf(-top, L, c));
+            sum = sum + (double)bm_pairs<PER>([&](int j) { return __builtin_amdgcn_exp2f(fmaf(Bm<T>::at(r[i], j), L, -ref)); });
+        const double t = wt == -INFINITY ? 0.0 : (double)fmaf(-wt, L, c) * 0.6931471805599453;
+        sum = wave_dsum(sum) * fma(t, fma(t, 0.5, 1.0), 1.0);
     } else {
-        const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll
         for (int i = 0; i < NL; ++i)
-#pragma unroll
-            for (int j = 0; j < PER; ++j) sum = sum + bm_exp(Bm<T>::at(r[i], j) - ref);
+            sum = sum + (double)bm_pairs<PER>([&](int j) { return __builtin_amdgcn_exp2f((Bm<T>::at(r[i], j) - wt) * L); });
+        sum = wave_dsum(sum);
     }
-    {
-        const float wt = group_max<64>(top);
-        const double ws = wave_dsum((double)sum * (double)bm_scale(top, wt));
-        if (lane == 0) {
-            wsum[wave] = ws;
-            wtop[wave] = wt;
-        }
+    if (lane == 0) {
+        wsum[wave] = sum;
+        wtop[wave] = wt;
     }
     __syncthreads();
     uint32_t k4[4];
@@ -307,14 +319,15 @@ __global__ __launch_bounds__(BM_NT) void k_beam_rows(BeamSelect p, int span, int
         if (rank < K && (tid & 3) == 0) out[rank] = BmCand{bm_value((uint32_t)(k >> 32)), from + (int)~(uint32_t)k};
     }
     for (int e = C + tid; e < K; e += BM_NT) out[e] = BmCand{-INFINITY, -1};
-    if (tid == 0) {
-        float wt = wtop[0];
-#pragma unroll
-        for (int w = 1; w < BM_WAVES; ++w) wt = fmaxf(wt, wtop[w]);
-        double s = 0.0;
-#pragma unroll
-        for (int w = 0; w < BM_WAVES; ++w) s += wsum[w] * (double)bm_scale(wtop[w], wt);
-        bm_sums(p)[part] = BmSum{s, wt, 0};
+    if (tid < BM_WAVES) {  // (a quad)
+        static_assert(BM_WAVES == 4, "a lane a wave");
+        const float t = wtop[tid];
+        float wt = fmaxf(t, dpp_f<0xb1>(t));
+        wt = fmaxf(wt, dpp_f<0x4e>(wt));
+        double s = wsum[tid] * bm_scale(t, wt);
+        s = s + dpp_d<0xb1>(s);
+        s = s + dpp_d<0x4e>(s);
+        if (tid == 0) bm_sums(p)[part] = BmSum{s, wt, 0};
     }
 }
 
@@ -357,10 +370,10 @@ __global__ __launch_bounds__(NT) void k_beam_join(BeamSelect p, int n_split) {
         double s = 0.0;
         if (st == 1) {
             for (int i = lane; i < n_split; i += WAVE) top = fmaxf(top, from[i].top);
-            top = group_max<64>(top);
+            top = bm_wave_max(top);
             for (int i = lane; i < n_split; i += WAVE) {
                 const BmSum q = from[i];
-                s += q.sum * (double)bm_scale(q.top, top);
+                s += q.sum * bm_scale(q.top, top);
             }
             s = wave_dsum(s);
         }

@@ -52,3 +52,60 @@ def test_beam_order_of_unlike_beams(vocab, places):
             assert token[0].tolist() == [places[0]] * 2
             # (e^-50 of the whole: within the score's rounding)
             assert (np.abs(score[0] - np.sort(s[0])[::-1]) <= 12 * U).all(), (score, s)
+
+
+def check_closely(logits, scores, n_out):
+    """Each place's score within the documented error of that place's in 64 bits, the
+    very candidate where its neighbours are further off.  An exponential is off by
+    2 u, its argument by up to 2.3 u times the distance from its wave's top, which over
+    a wave's 8,192 values is at most 6.2 on average (E exp(1 + E) = 8,191), three
+    additions in f32, and a wave's and a part's scale 2 u each: 23.3 u."""
+    tol = 23.3 * U
+    parent, token, score = run_beam(logits, scores, n_out)
+    vocab, x = logits.shape[2], logits.float().numpy()
+    for r in range(len(x)):
+        s = beam_scores(x[r], scores[r], None, 0)
+        flat = np.argsort(-s, axis=None, kind="stable")[:n_out + 1]
+        best = s.flatten()[flat]
+        got = np.array([s[p - r * x.shape[1], t] for p, t in zip(parent[r], token[r])])
+        assert (np.abs(got - best[:n_out]) <= 2 * tol).all(), r
+        assert (np.abs(score[r] - got) <= tol + U * np.abs(got)).all(), (r, np.abs(score[r] - got).max() / U)
+        gap = np.concatenate([[np.inf], -np.diff(best)])
+        sure = np.minimum(gap[:-1], gap[1:]) > 2 * tol
+        at = (parent[r] - r * x.shape[1]) * vocab + token[r]
+        assert (at[sure] == flat[:n_out][sure]).all(), r
+    return score
+
+
+@pytest.mark.parametrize("n,beams,vocab,kind,n_out", [
+    (1, 4, 32000, "f32", 4), (3, 5, 50021, "f16", 10), (2, 8, 256000, "bf16", 16), (70, 4, 40001, "f32", 2),
+    (1, 16, 98304, "bf16", 64), (5, 3, 257, "f16", 8)])
+@pytest.mark.parametrize("spread,mean", [(1e-3, 0.0), (0.7, 15.0), (2.5, 0.0), (4.0, -900.0), (8.0, 3000.0), (1000.0, 5000.0)])
+def test_beam_error(n, beams, vocab, kind, n_out, spread, mean):
+    rng = np.random.default_rng(vocab)
+    x = torch.from_numpy((rng.standard_normal((n, beams, vocab), dtype=np.float32) * spread + mean).astype(np.float32)).to(TYPES[kind])
+    check_closely(x, -rng.uniform(0, 3, (n, beams)).astype(np.float32), n_out)
+
+
+@pytest.mark.parametrize("kind,vocab,per", [("f32", 32768, 4), ("f16", 65536, 8), ("bf16", 65536, 8)])
+def test_beam_sums_that_repeat(kind, vocab, per):
+    """Rows whose every lane has the same values, a 0 and p - 1 of -d again and again:
+    roundings that do not average out.  129 rows of two parts of 16 loads a lane.  All tops
+    are 0, so that c and the scales are exact: an exponential 2 u, its argument 1.3 u
+    times the distance (2.8 at most on average), three additions: 9 u.
+    The beam's score is its row's log-sum-exp, so that S is next to 0."""
+    rng = np.random.default_rng(3)
+    col = np.arange(vocab)
+    place = col // (256 * per) * per + col % per  # of the lane's values
+    period = 2 ** rng.integers(1, 6, 129)
+    d = np.exp(rng.uniform(np.log(0.05), np.log(4.0), 129))
+    d[:6], period[:6] = [2.5625, 2.9375, 3.15625, 2.58984375, 2.741, 3.9695], [32, 16, 32, 32, 32, 32]
+    x = torch.from_numpy(np.where(place[None] % period[:, None] == 0, 0.0, -d[:, None]).astype(np.float32)).to(TYPES[kind])
+    v = x.double().numpy()
+    lse = np.log(np.exp(v).sum(1))
+    scores = lse.astype(np.float32)[:, None]
+    parent, token, score = run_beam(x[:, None], scores, 1)
+    want = scores[:, 0].astype(np.float64) - lse
+    assert (parent[:, 0] == np.arange(129)).all() and (token == 0).all()
+    err = np.abs(score[:, 0] - want)
+    assert (err <= 9 * U + U * np.abs(want)).all(), (err.max() / U, int(err.argmax()))
