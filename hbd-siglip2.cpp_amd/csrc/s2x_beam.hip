@@ -3,7 +3,9 @@
 //   S[b, v] = score_b + logit[b, v] - log sum_u exp(logit[b, u])
 //
 // and the n_out largest of each request, over all its beams b and tokens v; of
-// equal ones the lower beam, then the lower token.
+// equal ones the lower beam, then the larger logit (S need not tell two small ones
+// apart), then the lower token.  Within a beam that is the order of the logits, so
+// that a part of a row knows its own.
 //
 // k_beam_rows: a workgroup's part of a row lies in registers, read once.  Its
 // lanes' maxima serve twice: for the reference of a wave's sum of exponentials,
@@ -339,10 +341,13 @@ __global__ __launch_bounds__(NT) void k_beam_join(BeamSelect p, int n_split) {
     static_assert((BEAM_MAX_OUT - 1) * (BJ_PER + 1) + WAVES * BEAM_MAX_OUT <= BJ_CAP, "the list's largest length");
     __shared__ double add[BEAM_MAX_OUT];  // score - lse of the beams; -inf: none
     __shared__ uint8_t state[BEAM_MAX_OUT];
-    __shared__ uint64_t tops[NT], lk[BJ_CAP];
-    __shared__ int32_t lp[BJ_CAP], lt[BJ_CAP], lb[BJ_CAP];
-    __shared__ uint64_t bk[BEAM_MAX_OUT];  // the best so far, in order
-    __shared__ int32_t bt[BEAM_MAX_OUT], bb[BEAM_MAX_OUT];
+    // a member's key, what orders equal ones (63 - beam, the logit's key, ~place: 6, 32
+    // and 14 bits) and its token
+    static_assert(BEAM_MAX_OUT <= 64 && NT * (BJ_PER + 1) <= 1 << 14, "beam and place in their bits");
+    __shared__ uint64_t tops[NT], lk[BJ_CAP], lo[BJ_CAP];
+    __shared__ int32_t lt[BJ_CAP];
+    __shared__ uint64_t bk[BEAM_MAX_OUT], bo[BEAM_MAX_OUT];  // the best so far, in order
+    __shared__ int32_t bt[BEAM_MAX_OUT];
     __shared__ BmSum ls[BJ_SUMS];
     __shared__ int count, ties;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, req = blockIdx.x, K = p.n_out;
@@ -360,7 +365,8 @@ __global__ __launch_bounds__(NT) void k_beam_join(BeamSelect p, int n_split) {
     if (tid < p.n_beam) state[tid] = bm_state(p, req * p.n_beam + tid);
     if (tid < K) {
         bk[tid] = bm_key(-(double)INFINITY);
-        bt[tid] = bb[tid] = -1;
+        bo[tid] = 0;
+        bt[tid] = -1;
     }
     __syncthreads();
     for (int b = wave; b < p.n_beam; b += WAVES) {
@@ -390,16 +396,19 @@ __global__ __launch_bounds__(NT) void k_beam_join(BeamSelect p, int n_split) {
         // this round's candidates, and the best of those before as places below
         // all of them
         const uint64_t none = bm_key(-(double)INFINITY);
-        uint64_t key[BJ_PER + 1];
+        uint64_t key[BJ_PER + 1], beams = 0;  // (63 - beam in 6 bits each)
+        uint32_t logit[BJ_PER + 1];
         int32_t tok[BJ_PER + 1];
-        int beam[BJ_PER + 1];
         key[0] = none;
-        tok[0] = beam[0] = -1;
+        logit[0] = 0;
+        tok[0] = -1;
         if (tid < K) {
             key[0] = bk[tid];
+            logit[0] = (uint32_t)(bo[tid] >> 14);
+            beams = bo[tid] >> 46;
             tok[0] = bt[tid];
-            beam[0] = bb[tid];
         }
+        auto ord = [&](int i) { return (beams >> 6 * i & 63) << 32 | logit[i]; };
         int b = (e0 + tid) / per_beam, rest = e0 + tid - b * per_beam;
 #pragma unroll
         for (int i = 1; i <= BJ_PER; ++i) {
@@ -412,10 +421,11 @@ __global__ __launch_bounds__(NT) void k_beam_join(BeamSelect p, int n_split) {
                 }
             }
             key[i] = none;
-            tok[i] = beam[i] = -1;
+            logit[i] = 0;
+            tok[i] = -1;
             const int e = e0 + (i - 1) * NT + tid;
             if (e >= all) continue;
-            beam[i] = b;
+            beams |= (uint64_t)(63 - b) << 6 * i;
             if (state[b] == 2) {
                 if (rest == 0) {
                     key[i] = bm_key(add[b]);
@@ -424,6 +434,7 @@ __global__ __launch_bounds__(NT) void k_beam_join(BeamSelect p, int n_split) {
             } else if (add[b] > -INFINITY) {
                 const BmCand c = e0 ? cands[e] : first[i - 1];
                 if (c.token >= 0) key[i] = bm_key(add[b] + (double)c.x);
+                logit[i] = bm_key(c.x);
                 tok[i] = c.token;
             }
         }
@@ -434,20 +445,15 @@ __global__ __launch_bounds__(NT) void k_beam_join(BeamSelect p, int n_split) {
         __syncthreads();
         // a bound by the upper halves of the keys first: enough unless more keys
         // than the list takes share the bound's (many equal scores), then by whole keys
-        uint64_t k4[WAVES];
         uint32_t h4[WAVES];
 #pragma unroll
-        for (int i = 0; i < WAVES; ++i) {
-            k4[i] = tops[i * WAVE + lane];
-            h4[i] = (uint32_t)(k4[i] >> 32);
-        }
+        for (int i = 0; i < WAVES; ++i) h4[i] = (uint32_t)(tops[i * WAVE + lane] >> 32);
         const uint32_t hb = bm_kth(h4, K, 0);
         auto put = [&](int i) {
             const int at = atomicAdd(&count, 1);
             lk[at] = key[i];
-            lp[at] = i * NT + tid;
+            lo[at] = ord(i) << 14 | (uint64_t)((1 << 14) - 1 - (i * NT + tid));
             lt[at] = tok[i];
-            lb[at] = beam[i];
         };
         int eq = 0;
 #pragma unroll
@@ -460,12 +466,28 @@ __global__ __launch_bounds__(NT) void k_beam_join(BeamSelect p, int n_split) {
             for (int i = 0; i <= BJ_PER; ++i)
                 if ((uint32_t)(key[i] >> 32) >= hb && key[i] > none) put(i);
         } else {
+            // and of those equal to the bound by their order, in the same way: lanes
+            // whose largest is above the bound are above all of them
+            uint64_t k4[WAVES];
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) k4[i] = tops[i * WAVE + lane];
             const uint64_t bound = bm_kth(k4, K, 0);
+            __syncthreads();
+            uint64_t first_of = top > bound ? ~0ull : 0;
+#pragma unroll
+            for (int i = 0; i <= BJ_PER; ++i)
+                if (key[i] == bound) first_of = max(first_of, ord(i));
+            tops[tid] = first_of;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) k4[i] = tops[i * WAVE + lane];
+            const uint64_t bound_o = bm_kth(k4, K, 0);
             int taken = 0;
 #pragma unroll
             for (int i = 0; i <= BJ_PER; ++i) {
-                if (key[i] > bound) put(i);
-                const bool is = key[i] == bound && bound > none;
+                const bool at = key[i] == bound && bound > none;
+                if (key[i] > bound || (at && ord(i) > bound_o)) put(i);
+                const bool is = at && ord(i) == bound_o;
                 const uint64_t m = __builtin_amdgcn_ballot_w64(is);
                 if (is && taken + __builtin_popcountll(m & ((1ull << lane) - 1)) < K) put(i);
                 taken += __builtin_popcountll(m);
@@ -474,25 +496,25 @@ __global__ __launch_bounds__(NT) void k_beam_join(BeamSelect p, int n_split) {
         __syncthreads();
         const int C = min(count, BJ_CAP);
         for (int e = tid >> 2; e < C; e += NT / 4) {
-            const uint64_t k = lk[e];
-            const int at = lp[e];
-            const int rank = bm_rank(C, [&](int q) { return lk[q] > k || (lk[q] == k && lp[q] < at); });
+            const uint64_t k = lk[e], o = lo[e];
+            const int rank = bm_rank(C, [&](int q) { return lk[q] > k || (lk[q] == k && lo[q] > o); });
             if (rank < K && (tid & 3) == 0) {
                 bk[rank] = k;
+                bo[rank] = o;
                 bt[rank] = lt[e];
-                bb[rank] = lb[e];
             }
         }
         for (int e = C + tid; e < K; e += NT) {
             bk[e] = none;
-            bt[e] = bb[e] = -1;
+            bo[e] = 0;
+            bt[e] = -1;
         }
     }
     __syncthreads();
     if (tid < K) {
         const bool there = bk[tid] > bm_key(-(double)INFINITY);
         const int64_t at = (int64_t)req * K + tid;
-        p.parent[at] = there ? req * p.n_beam + bb[tid] : -1;
+        p.parent[at] = there ? req * p.n_beam + 63 - (int)(bo[tid] >> 46) : -1;
         p.token[at] = there ? bt[tid] : -1;
         p.score[at] = there ? (float)bm_value(bk[tid]) : -INFINITY;
     }

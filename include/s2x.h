@@ -551,10 +551,10 @@ int s2x_add_rmsnorm_quantize_q8_1(const void *x, int32_t x_type, int64_t ld_x, c
  * in f64, but for the exponentials and the sums of 4 (f32) or 8 of them, which are f32:
  * S is off by 2^-22 or less mostly, by 2^-19 at most whatever the logits are.  A row is
  * read in parts, which depend on the call's sizes, n_req among them: another number of
- * requests may change S within that.  The n_out largest come out
- * in order, equal ones by the lower beam, then the lower token: parent (the row of
- * the beam), token, score (S in f32), each n_req x n_out.  A logit of -inf is a
- * token that cannot follow; the lowest finite value is a value like any other.
+ * requests may change S within that.  The n_out largest come out in order, equal ones
+ * by the lower beam, then the larger logit (f64 does not always tell S of two apart),
+ * then the lower token: parent (the row of the beam), token, score (S in f32), each
+ * n_req x n_out.  A logit of -inf is a token that cannot follow; the lowest finite value is a value like any other.
  * done (optional, a byte a beam): not 0, the beam has ended; it is a candidate as it
  * is, with done_token and its score.  A beam whose score is no finite number is
  * none (the first step: -inf for all but one), nor has one with a NaN, +inf or no

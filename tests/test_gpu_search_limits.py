@@ -109,3 +109,42 @@ def test_beam_sums_that_repeat(kind, vocab, per):
     assert (parent[:, 0] == np.arange(129)).all() and (token == 0).all()
     err = np.abs(score[:, 0] - want)
     assert (err <= 9 * U + U * np.abs(want)).all(), (err.max() / U, int(err.argmax()))
+
+
+def same_s_order(x, scores, n_out):
+    """Places of a request whose every beam has one S for all its tokens (logits too
+    small to change it): by beam's score, then the lower beam, the larger logit, the
+    lower token."""
+    beams, vocab = x.shape
+    out = []
+    for b in sorted(range(beams), key=lambda b: (-scores[b], b)):
+        out += [(b, int(t)) for t in np.argsort(-x[b].astype(np.float64), kind="stable")[:n_out]]
+    return out[:n_out]
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("beams,vocab,n_out", [(1, 3, 3), (1, 3000, 64), (2, 70000, 5), (4, 32000, 4), (1, 300001, 64), (3, 1000003, 64),
+                                               (64, 9000, 64), (8, 200000, 60)])
+def test_beam_order_of_equal_scores(beams, vocab, n_out, kind):
+    """Logits of some 1e-20 that differ where S, in f64, does not: of one beam's the
+    larger logit is ahead, in whatever part or round of the join it lies, then the
+    lower token; of two beams' the lower beam.  Few of them among others, and rows of
+    nothing else (more equal scores than a list takes)."""
+    rng = np.random.default_rng(vocab + beams)
+    for values, dense in ((40, True), (1 << 30, True), (40, False)):
+        tiny = rng.integers(0, values, (beams, vocab)).astype(np.float32) * np.float32(1e-20 / values * 40)
+        x = tiny if dense else np.where(rng.random((beams, vocab)) < max(0.01, 5.0 / vocab), tiny, np.float32(-1.0))
+        x[1:] = x[0]  # (one sum in all beams)
+        t = torch.from_numpy(x[None].copy()).to(TYPES[kind])
+        v = t[0].float().numpy()
+        for scores in (np.full(beams, -3.0), np.where(np.arange(beams) == beams - 1, -2.0, -3.0), -2.0 - np.arange(beams) % 3):
+            want = same_s_order(v, scores, n_out)
+            if not dense:  # (the others lie a whole 1 below)
+                want = [w for w in want if v[w] > -0.5]
+            parent, token, score = run_beam(t, scores[None].astype(np.float32), n_out)
+            n = min(len(want), n_out)
+            if not dense:  # only of the first beam are the next in order known
+                n = next((i for i, w in enumerate(want) if w[0] != want[0][0]), n)
+            got = [(int(p), int(k)) for p, k in zip(parent[0], token[0])]
+            assert got[:n] == want[:n], (dense, values, scores[:4])
+            assert (np.diff(score[0]) <= 0).all()
