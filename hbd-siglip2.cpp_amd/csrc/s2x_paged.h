@@ -102,6 +102,21 @@ __device__ __forceinline__ PaGroup pa_group(const AttnPrefix &p, int g) {
     r.len = min((int64_t)min(max(p.prefix_len[g], 0), p.max_prefix), p.a.ld_table << p.a.kv.page_shift);
     return r;
 }
+// Whether sequence s is one that has been freed: no tokens, and a table that begins
+// with no page (ld_table > 0).
+__device__ __forceinline__ bool pa_freed(const AttnPaged &p, int s) {
+    return p.kv_len[s] <= 0 && (uint32_t)p.table[s * p.ld_table] >= (uint32_t)p.kv.n_pages;
+}
+// The sequence whose pages are the group's prefix: the first that has not been freed
+// (none: the first).  Of the whole wave.
+__device__ __forceinline__ int pa_holder(const AttnPaged &p, const PaGroup &g) {
+    for (int i0 = 0; i0 < g.size; i0 += WAVE) {
+        const bool live = !pa_freed(p, g.first + min(i0 + (int)(threadIdx.x & 63), g.size - 1));
+        const uint64_t m = __builtin_amdgcn_ballot_w64(live);
+        if (m) return g.first + i0 + __builtin_ctzll(m);
+    }
+    return g.first;
+}
 // The last group that begins at or before sequence s (starts ascend; none: the
 // first), and where it begins: each lane of the wave looks at one of 64 parts of
 // the groups left, until one is.
@@ -225,7 +240,7 @@ __device__ __forceinline__ void pa_body(const ARGS &args, const PaWork &w, int c
     const bool ragged = MODE == PA_PREFIX && __builtin_amdgcn_ballot_w64(lim < end) != 0;
 
     const TC *kp = (const TC *)p.kv.k + hk * p.kv.ld_head, *vp = (const TC *)p.kv.v + hk * p.kv.ld_head;
-    const int32_t *row = p.table + s * p.ld_table;
+    const int32_t *row = p.table + s * p.ld_table;  // (PREFIX: of the first sequence, unless that has been freed)
     const uint32_t pmask = (1u << p.kv.page_shift) - 1, ldp = (uint32_t)p.kv.ld_page, ldt = (uint32_t)p.kv.ld_tok;
     TC *vl = reinterpret_cast<TC *>(lds) + place * TILE * d;
 
@@ -306,8 +321,15 @@ __device__ __forceinline__ void pa_body(const ARGS &args, const PaWork &w, int c
     int64_t t0 = start + wave * TILE;
     int32_t next = -1;
     if (t0 < end) {
-        load(t0, entry_of(t0));
+        int32_t here = entry_of(t0);
         next = entry_of(t0 + STEP);
+        // (asked while the entries are on their way; uniform)
+        if (MODE == PA_PREFIX && pa_freed(p, gr.first)) {
+            row = p.table + pa_holder(p, gr) * p.ld_table;
+            here = entry_of(t0);
+            next = entry_of(t0 + STEP);
+        }
+        load(t0, here);
     }
     for (; t0 < end; t0 += STEP) {
         const uint32_t mask = seen;

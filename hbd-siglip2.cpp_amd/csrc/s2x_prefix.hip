@@ -162,8 +162,13 @@ __device__ __forceinline__ void px_wide(const AttnPrefix &args, const PxPlan &P,
     };
     Entries next;
     {
-        const Entries e0 = entries(start), e1 = entries(start + PX_TK);
+        Entries e0 = entries(start), e1 = entries(start + PX_TK);
         next = AHEAD == 2 ? entries(start + 2 * PX_TK) : e1;
+        if (pa_freed(p, gr.first)) {  // (asked while the entries are on their way; uniform)
+            row = p.table + (int64_t)pa_holder(p, gr) * p.ld_table;
+            e0 = entries(start), e1 = entries(start + PX_TK);
+            next = AHEAD == 2 ? entries(start + 2 * PX_TK) : e1;
+        }
         load(even, start, e0);
         if constexpr (AHEAD == 2) load(odd, start + PX_TK, e1);
     }
@@ -457,13 +462,16 @@ __global__ __launch_bounds__(NT) void k_prefix_join(AttnPrefix args, PxPlan P) {
         i0 += PXJ_AHEAD * GROUPS;
         fetch(i0, np, n);
     }
-    if (redo == redo) {
-        const int share = p.n_q_head / p.kv.n_head, ec = min(e, nq - 1);
-        const v4f y = px_seen_only<TC>(p, gr.first, h / share, (const TC *)p.q + qrow * p.ld_q + (int64_t)h * d, 4 * ec,
-                                       (int64_t)ends * P.chunk_p, own.first, redo);
-        const float f = __builtin_amdgcn_exp2f(redo - (M == -INFINITY ? 0.0f : M));
+    if (__builtin_amdgcn_ballot_w64(redo == redo) != 0) {
+        const int holder = pa_holder(p, gr);
+        if (redo == redo) {
+            const int share = p.n_q_head / p.kv.n_head, ec = min(e, nq - 1);
+            const v4f y = px_seen_only<TC>(p, holder, h / share, (const TC *)p.q + qrow * p.ld_q + (int64_t)h * d, 4 * ec,
+                                           (int64_t)ends * P.chunk_p, own.first, redo);
+            const float f = __builtin_amdgcn_exp2f(redo - (M == -INFINITY ? 0.0f : M));
 #pragma unroll
-        for (int c = 0; c < 4; ++c) a[c] = fmaf(y[c], f, a[c]);
+            for (int c = 0; c < 4; ++c) a[c] = fmaf(y[c], f, a[c]);
+        }
     }
     *reinterpret_cast<v4f *>(&part[grp][(tid % LANES) * 4]) = a;
     if (tid % LANES == 0) {

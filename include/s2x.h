@@ -625,8 +625,9 @@ int s2x_kv_copy_pages(const s2x_kv_cache *caches, int64_t n_cache, const int32_t
  * first tokens: group g is sequences group_start[g] .. group_start[g + 1] - 1
  * (n_group + 1 ascending entries on the device), whose tokens before prefix_len[g]
  * are the same.  Their keys and values are read once for the whole group, from the
- * pages of its first sequence; what the other rows of block_table have there is not
- * looked at.  Sequence s sees the first kv_len[s] tokens as ever: fewer than the
+ * pages of its first sequence (a sequence that has been freed, with no tokens and no
+ * page at its row's begin, as s2x_kv_fork leaves it, is passed over); what the other
+ * rows of block_table have there is not looked at.  Sequence s sees the first kv_len[s] tokens as ever: fewer than the
  * prefix, and it sees that much of it.  tok_start as in s2x_attn_paged_rows, or
  * NULL: row s of q is sequence s's.  A prefix counts as at most max_prefix tokens
  * (the others are its sequences' own), a sequence's own tokens as the first max_own

@@ -8,8 +8,8 @@ import torch
 
 from decode_util import TYPES
 from search_util import beam_scores
-from test_gpu_decode import U
-from test_gpu_search import INF, run_beam
+from test_gpu_decode import NAN, U
+from test_gpu_search import INF, compare, ints, prefix_inputs, run_beam, run_fork, run_prefix
 
 pytestmark = pytest.mark.gpu
 
@@ -148,3 +148,41 @@ def test_beam_order_of_equal_scores(beams, vocab, n_out, kind):
             got = [(int(p), int(k)) for p, k in zip(parent[0], token[0])]
             assert got[:n] == want[:n], (dense, values, scores[:4])
             assert (np.diff(score[0]) <= 0).all()
+
+
+@pytest.mark.parametrize("share,size,d,kind,freed", [
+    (2, 5, 128, "f16", [0]), (1, 6, 72, "bf16", [0, 1, 3]), (2, 20, 64, "bf16", [0]), (4, 40, 128, "f16", [0, 1, 2, 39]),
+    (4, 33, 128, "bf16", [0]), (3, 9, 256, "f16", [0, 8]), (8, 6, 200, "bf16", [0]), (1, 90, 64, "f16", list(range(70))),
+    (1, 12, 64, "f16", list(range(12)))])
+def test_prefix_of_a_freed_first_sequence(share, size, d, kind, freed):
+    """Sequences of a group that s2x_kv_fork frees, its first among them: the others
+    see the prefix as before, from the first that is left, also one that ends inside
+    it behind which the values are no numbers."""
+    rng = np.random.default_rng(size)
+    p, at = 700, 333
+    owns = [int(o) for o in rng.integers(0, 30, size)]
+    groups = [(90, [3, 4]), (p, owns), (40, [7])]
+    q, cache, table, ref, lens, starts, plen = prefix_inputs(rng, groups, 2 * share, 2, d, kind, 16, "head")
+    table = ref.copy()  # (every row's own: those of freed ones go)
+    parent = np.arange(len(lens))
+    parent[np.array(freed) + 2] = -1
+    out, lens2, src, dst, _, _, _ = run_fork(parent, lens, table, 16, cache.n_pages, pinned=np.zeros(cache.n_pages))
+    live = np.setdiff1d(np.arange(len(lens)), np.array(freed) + 2)
+    # (rows of a group share its whole pages only: nothing to copy)
+    assert (src == -1).all() and (out[live] == table[live]).all() and (out[np.array(freed) + 2] == -1).all()
+    assert (lens2[np.array(freed) + 2] == 0).all()
+    # what the other rows have at the prefix is not looked at
+    left = [i for i in range(size) if i not in freed]
+    for i in left[1:]:
+        out[2 + i, :p // 16] = rng.integers(-1, cache.n_pages, p // 16)
+    table[np.array(freed) + 2] = -1
+    if size - 2 in left:
+        lens2[size] = at  # (ends inside the prefix)
+    got, lse = run_prefix(q, cache, out, lens2, starts, plen, 0.1, "f32", max_own=40)
+    compare(got, lse, q, cache, table, lens2, 0.1, "f32")
+    if size - 2 in left:
+        cache.v[int(ref[2 + left[0], (at + 20) // 16]), :, 3] = NAN
+        got, lse = run_prefix(q, cache, out, lens2, starts, plen, 0.1, "f32", max_own=40)
+        rows = np.array([0, 1, size, size + 2])
+        assert np.isnan(got[np.setdiff1d(live, rows)]).all(axis=2).all() if len(left) > 1 else True
+        compare(got[rows], lse[rows], q[rows], cache, table[rows], lens2[rows], 0.1, "f32")
