@@ -605,7 +605,11 @@ int s2x_kv_fork(const int32_t *parent, int64_t n_out, const int32_t *kv_len, con
  * takes: page copy_src[k] goes to copy_dst[k], k < count[1], both in order, -1
  * behind them (n_pages / 2 entries each).  No copy_dst is a copy_src, so
  * s2x_kv_copy_pages does them in any order.  table_out as the tables read then, -1
- * past a row's last page.  Limits, overlaps and workspace as s2x_kv_fork's. */
+ * past a row's last page.  Pages that no row holds are given up, written over or left
+ * past count[0]: those that s2x_kv_fork was told are pinned among them, if they are not
+ * passed as further rows of the tables (each kv_len its entries times page_size), whose
+ * rows of table_out then say where they are, and which bytes of `pinned` to set from
+ * there on.  Limits, overlaps and workspace as s2x_kv_fork's. */
 int s2x_kv_compact(const int32_t *kv_len, const int32_t *block_table, int64_t n_seq, int64_t ld_table,
                    int64_t page_size, int64_t n_pages, int32_t *table_out, int64_t ld_out,
                    int32_t *copy_src, int32_t *copy_dst, int64_t *count, void *workspace,

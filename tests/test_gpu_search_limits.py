@@ -1,15 +1,17 @@
 """What the header says of the beam search's operators at its ends: the selection's
-error, its order.
+error and order, prefixes of freed sequences, pinned pages in a compaction.
 
 u = 2^-24, the half step of an f32 at 1."""
 import numpy as np
 import pytest
 import torch
 
-from decode_util import TYPES
-from search_util import beam_scores
+import s2x
+from decode_util import TYPES, Cache
+from gpu_util import ptr, stream
+from search_util import beam_scores, compact_ref
 from test_gpu_decode import NAN, U
-from test_gpu_search import INF, compare, ints, prefix_inputs, run_beam, run_fork, run_prefix
+from test_gpu_search import INF, check_compact, compare, ints, prefix_inputs, run_beam, run_fork, run_prefix
 
 pytestmark = pytest.mark.gpu
 
@@ -186,3 +188,44 @@ def test_prefix_of_a_freed_first_sequence(share, size, d, kind, freed):
         rows = np.array([0, 1, size, size + 2])
         assert np.isnan(got[np.setdiff1d(live, rows)]).all(axis=2).all() if len(left) > 1 else True
         compare(got[rows], lse[rows], q[rows], cache, table[rows], lens2[rows], 0.1, "f32")
+
+
+def test_compact_with_pinned_pages():
+    """A fork that keeps pinned pages while their sequence is freed, then a compaction
+    that is given them as further rows: their content is where those rows say, and
+    that of the sequences where theirs do."""
+    rng = np.random.default_rng(11)
+    page, n_pages, n, ld = 16, 300, 12, 9
+    ids = rng.permutation(n_pages).astype(np.int32)
+    lens = rng.integers(1, ld * page + 1, n)
+    table = np.full((n, ld), -1, np.int32)
+    for s in range(n):
+        have = -(-int(lens[s]) // page)
+        table[s, :have] = ids[s * ld:s * ld + have]
+    # the pages of rows 0 and 5, which go, and two of no row
+    keep = np.concatenate([table[0][table[0] >= 0], table[5][table[5] >= 0], ids[200:202]])
+    pinned = np.zeros(n_pages, np.uint8)
+    pinned[keep] = 1
+    parent = np.array([-1, 1, 2, 3, 4, -1, 6, 7, 7, 8, 9, 10])
+    cache = Cache(n_pages, 2, page, 64, "f16", fill=lambda shape: torch.randn(shape, device="cuda:0"))
+    out, lens2, src, dst, tok, free, count = run_fork(parent, lens, table, page, n_pages, pinned=pinned)
+    assert not set(keep.tolist()) & (set(free.tolist()) | set(dst.tolist()))
+    t = [ints(a) for a in (src, dst, tok)]
+    s2x.call("s2x_kv_copy_pages", cache.ref(), 1, ptr(t[0]), ptr(t[1]), ptr(t[2]), n, None, stream())
+    torch.cuda.synchronize()
+    k, v = (c.clone() for c in (cache.k, cache.v))
+    rows = -(-len(keep) // ld)
+    more = np.full((rows, ld), -1, np.int32)
+    more.flat[:len(keep)] = keep
+    table2 = np.concatenate([out, more])
+    lens3 = np.concatenate([lens2, [page * int((r >= 0).sum()) for r in more]])
+    new, src, dst, count = check_compact(lens3, table2, page, n_pages)
+    a, b, c = ints(src), ints(dst), torch.tensor([int(count[1])], dtype=torch.int64, device="cuda:0")
+    s2x.call("s2x_kv_copy_pages", cache.ref(), 1, ptr(a), ptr(b), None, len(src), ptr(c), stream())
+    torch.cuda.synchronize()
+    held = table2 >= 0
+    assert new[held].max() == count[0] - 1 and ((new >= 0) == held).all()
+    to, fro = (torch.from_numpy(x[held].astype(np.int64)).to("cuda:0") for x in (new, table2))
+    assert torch.equal(cache.k[to], k[fro]) and torch.equal(cache.v[to], v[fro])
+    # without those rows the pages are given up
+    assert count[0] > compact_ref(lens2, out, page, n_pages, ld)[3][0]
