@@ -1,17 +1,21 @@
 """What the header says of the beam search's operators at its ends: the selection's
-error and order, prefixes of freed sequences, pinned pages in a compaction.
+error and order, prefixes of freed and of odd groups, pinned pages in a compaction,
+calls at once and over one workspace.
 
 u = 2^-24, the half step of an f32 at 1."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
 
 import s2x
 from decode_util import TYPES, Cache
-from gpu_util import ptr, stream
-from search_util import beam_scores, compact_ref
+from gpu_util import assert_same, dev, host, ptr, say, stream
+from search_util import beam_scores, compact_ref, fork_ref
 from test_gpu_decode import NAN, U
-from test_gpu_search import INF, check_compact, compare, ints, prefix_inputs, run_beam, run_fork, run_prefix
+from test_gpu_search import (INF, beam_case, beams_case, check_compact, compare, ints, nans, prefix_inputs, rms_case, run_beam,
+                             run_fork, run_prefix)
 
 pytestmark = pytest.mark.gpu
 
@@ -190,6 +194,19 @@ def test_prefix_of_a_freed_first_sequence(share, size, d, kind, freed):
         compare(got[rows], lse[rows], q[rows], cache, table[rows], lens2[rows], 0.1, "f32")
 
 
+@pytest.mark.parametrize("share", [2, 4, 16])
+def test_prefix_group_behind_one_that_is_none(share):
+    """Starts of -3, 2, 10: the first group is none, the second its first three
+    sequences, whose prefix lies in the first one's pages; all other rows stay."""
+    rng = np.random.default_rng(12)
+    groups = [(200, [20, 100, 9, 64, 7]), (90, [50, 5, 5]), (333, [1, 30])]
+    q, cache, _, ref, lens, _, _ = prefix_inputs(rng, groups, 2 * share, 2, 72, "f16", 16, "token", gap=8)
+    got, lse = run_prefix(q, cache, ref, lens, np.array([-3, 2, 10]), np.array([200, 90]), 0.12, "f32", max_group=3, max_own=300)
+    rows = np.array([2, 3, 4])
+    compare(got, lse, q, cache, ref, lens, 0.12, "f32", rows)
+    assert np.isnan(np.delete(got, rows, 0)).all() and np.isnan(np.delete(lse, rows, 0)).all()
+
+
 def test_compact_with_pinned_pages():
     """A fork that keeps pinned pages while their sequence is freed, then a compaction
     that is given them as further rows: their content is where those rows say, and
@@ -229,3 +246,180 @@ def test_compact_with_pinned_pages():
     assert torch.equal(cache.k[to], k[fro]) and torch.equal(cache.v[to], v[fro])
     # without those rows the pages are given up
     assert count[0] > compact_ref(lens2, out, page, n_pages, ld)[3][0]
+
+
+# ---------------------------------------------------------------------------
+# calls at once, and one after the other over one workspace
+# ---------------------------------------------------------------------------
+class Job:
+    """A call over buffers of its own: outputs `out`, filled before every run, a
+    workspace of `need` bytes, `call(ws, stream)`."""
+
+    def __init__(self, name, keep, out, need, call):
+        self.name, self.keep, self.out, self.need, self.call = name, keep, out, need, call
+
+    def clear(self):
+        for o in self.out:
+            o.fill_(NAN if o.is_floating_point() else -77)
+
+    def values(self):
+        return [o.clone() for o in self.out]
+
+    def check(self, want, what):
+        for i, (o, w) in enumerate(zip(self.out, want)):
+            a, b = (t.contiguous().view(torch.uint8) for t in (o, w))
+            assert torch.equal(a, b), (self.name, i, what)
+
+
+def workspace(n):
+    return torch.full((max(1, n),), 0xff, dtype=torch.uint8, device="cuda:0")
+
+
+def full(shape, dtype):
+    return torch.zeros(shape, dtype=dtype, device="cuda:0")
+
+
+def fork_job(seed, *shape):
+    parent, lens, table, page, n_pages = case = beams_case(np.random.default_rng(seed), *shape)
+    n, ld = table.shape
+    t = [ints(a) for a in (parent, lens, table)]
+    out = [full((n, ld), torch.int32), *(full((n,), torch.int32) for _ in range(4)), full((n_pages,), torch.int32), full((2,), torch.int64)]
+    need = s2x.lib.s2x_kv_pages_workspace_size(n_pages)
+    job = Job(f"fork {shape}", t, out, need, lambda ws, st: s2x.call(
+        "s2x_kv_fork", ptr(t[0]), n, ptr(t[1]), ptr(t[2]), n, ld, page, n_pages, None, ptr(out[0]), ld, *[ptr(o) for o in out[1:]],
+        ptr(ws), need, st))
+    job.ref = fork_ref(parent, lens, table, page, n_pages, None, ld)
+    return job
+
+
+def compact_job(seed, n_seq, most, n_pages):
+    rng = np.random.default_rng(seed)
+    lens = rng.integers(0, most + 1, n_seq)
+    have = -(-lens // 16)
+    ids, at = rng.permutation(n_pages), 0
+    table = np.full((n_seq, int(have.max())), -1, np.int32)
+    for s, h in enumerate(have):
+        table[s, :h] = ids[at:at + h]
+        at += h
+    ld, half = table.shape[1], n_pages // 2
+    t = [ints(lens), ints(table)]
+    cache = Cache(n_pages, 1, 16, 8, "f16", fill=lambda shape: torch.randn(shape, device="cuda:0"))
+    out = [full((n_seq, ld), torch.int32), full((half,), torch.int32), full((half,), torch.int32), full((2,), torch.int64)]
+    need = s2x.lib.s2x_kv_pages_workspace_size(n_pages)
+
+    def call(ws, st):
+        s2x.call("s2x_kv_compact", ptr(t[0]), ptr(t[1]), n_seq, ld, 16, n_pages, ptr(out[0]), ld, ptr(out[1]), ptr(out[2]),
+                 ptr(out[3]), ptr(ws), need, st)
+        # (no copy_dst is a copy_src: the same again and again)
+        s2x.call("s2x_kv_copy_pages", cache.ref(), 1, ptr(out[1]), ptr(out[2]), None, half, ctypes.c_void_p(out[3].data_ptr() + 8), st)
+    job = Job(f"compact {n_seq} {n_pages}", [t, cache], out, need, call)
+    job.ref = compact_ref(lens, table, 16, n_pages, ld)
+    job.cache, job.before = cache, [c.clone() for c in (cache.k, cache.v)]
+    return job
+
+
+def prefix_job(seed, groups, hq, hkv, d, kind):
+    q, cache, table, _, lens, starts, plen = prefix_inputs(np.random.default_rng(seed), groups, hq, hkv, d, kind, 16, "head")
+    n, mg, mp = len(lens), int(np.diff(starts).max()), int(plen.max())
+    mo = max(max(o) for _, o in groups)
+    t = [q.to("cuda:0"), *(ints(a) for a in (table, lens, starts, plen))]
+    out = [nans(n, hq * d), nans(n, hq)]
+    need = s2x.lib.s2x_attn_paged_prefix_workspace_size(len(plen), mg, mp, mo, hq, hkv, d)
+    return Job(f"prefix {hq}/{hkv} x {d}", [t, cache], out, need, lambda ws, st: s2x.call(
+        "s2x_attn_paged_prefix", ptr(t[0]), hq * d, n, None, cache.ref(), ptr(t[1]), table.shape[1], ptr(t[2]), n, ptr(t[3]), ptr(t[4]),
+        len(plen), mg, mp, mo, hq, 0.09, ptr(out[0]), 0, hq * d, ptr(out[1]), ptr(ws), need, st))
+
+
+def beam_job(seed, n, beams, vocab, kind, n_out):
+    x, s = beam_case(seed, n, beams, vocab, kind)
+    t = [x.to("cuda:0"), dev(s)]
+    out = [full((n, n_out), d) for d in (torch.int32, torch.int32, torch.float32)]
+    need = s2x.lib.s2x_beam_select_workspace_size(n, beams, vocab, n_out)
+    code = {"f32": 0, "f16": 1, "bf16": 2}[kind]
+    return Job(f"beam {n} {beams} {vocab}", t, out, need, lambda ws, st: s2x.call(
+        "s2x_beam_select", ptr(t[0]), code, vocab, n, beams, vocab, ptr(t[1]), None, 0, n_out, *[ptr(o) for o in out], ptr(ws), need, st))
+
+
+def rms_job(seed, m, h):
+    x, r, w = rms_case(seed, m, h, "f32", "f32")
+    k = -(-h // 32) * 32
+    t = [x.to("cuda:0"), r.to("cuda:0"), dev(w)]
+    out = [nans(m, h), full((m, k), torch.int8), full((m, k // 32), torch.int32), nans(m, h)]
+    return Job(f"norm {m} x {h}", t, out, 0, lambda ws, st: s2x.call(
+        "s2x_add_rmsnorm_quantize_q8_1", ptr(t[0]), 0, h, ptr(t[1]), 0, h, h, m, ptr(t[2]), 1e-6, ptr(out[0]), h, k, ptr(out[1]),
+        ptr(out[2]), ptr(out[3]), 0, h, st))
+
+
+def page_jobs():
+    """Forks in one workgroup, of few pages and of many tiles of them, and compactions
+    of few and of many, two of each."""
+    return [fork_job(1, 3, 4, 90, 30, 16, 40), fork_job(2, 9, 5, 300, 60, 16, 700), fork_job(3, 60, 8, 900, 90, 16, 3000),
+            fork_job(4, 200, 6, 40, 30, 16, 21000), fork_job(5, 40, 8, 500, 90, 16, 50000), fork_job(6, 7, 300, 70, 20, 8, 90000),
+            compact_job(7, 40, 900, 9000), compact_job(8, 300, 200, 12000), compact_job(9, 200, 1500, 70000),
+            compact_job(10, 5, 9000, 40001)]
+
+
+def settled(job):
+    """The call alone: its outputs, those of the pages against the plain form."""
+    ws = workspace(job.need)
+    job.clear()
+    torch.cuda.synchronize()
+    job.call(ws, stream())
+    torch.cuda.synchronize()
+    for i, r in enumerate(getattr(job, "ref", [])):
+        assert_same(host(job.out[i]).reshape(r.shape), r, f"{job.name} {i}")
+    if hasattr(job, "cache"):
+        src, dst, n = host(job.out[1]), host(job.out[2]), int(host(job.out[3])[1])
+        for c, b in zip((job.cache.k, job.cache.v), job.before):
+            b[dst[:n].tolist()] = b[src[:n].tolist()].clone()
+            assert torch.equal(c, b), job.name
+    return job.values()
+
+
+def test_every_operator_on_two_streams_at_once():
+    """All launches on both streams before any wait, each over buffers and a workspace
+    of its own: the bits of the call alone."""
+    jobs = page_jobs() + [
+        prefix_job(1, [(700, [30, 5, 60]), (90, [3, 4])], 8, 2, 128, "f16"), prefix_job(2, [(900, [30, 5, 60, 1] * 5)], 8, 2, 128, "bf16"),
+        prefix_job(3, [(400, [9] * 40)], 4, 1, 72, "f16"), prefix_job(4, [(50, [300, 2])] * 9, 4, 4, 64, "bf16"),
+        beam_job(5, 3, 4, 20011, "f32", 8), beam_job(6, 30, 4, 30000, "bf16", 4), beam_job(7, 1, 32, 40000, "f16", 64),
+        rms_job(8, 33, 2100), rms_job(9, 700, 512), rms_job(10, 3000, 100)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    handles = [ctypes.c_void_p(s.cuda_stream) for s in streams]
+    want = [settled(j) for j in jobs]
+    spaces = [workspace(j.need) for j in jobs]
+    for r in range(4):
+        say(f"round {r}")
+        for j in jobs:
+            j.clear()
+        torch.cuda.synchronize()
+        for i, j in enumerate(jobs):
+            j.call(spaces[i], handles[(i + r) % 2])
+        torch.cuda.synchronize()
+        for j, w in zip(jobs, want):
+            j.check(w, f"round {r}")
+
+
+def test_page_calls_over_one_workspace():
+    """Captured forks and compactions of different rows and pages, replayed in turn
+    over the same workspace with eager work between: nothing of one is left for
+    another."""
+    jobs = page_jobs()
+    want = [settled(j) for j in jobs]
+    ws = workspace(max(j.need for j in jobs))
+    graphs = []
+    for j in jobs:
+        j.call(ws, stream())
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            j.call(ws, stream())
+        graphs.append(g)
+    rng = np.random.default_rng(1)
+    for r in range(3):
+        for i in rng.permutation(len(jobs)):
+            jobs[i].clear()
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            jobs[i].check(want[i], f"round {r}")
+            torch.randn(300, 300, device="cuda:0").sum()
