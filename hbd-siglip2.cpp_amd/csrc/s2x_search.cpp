@@ -14,14 +14,20 @@ namespace s2x {
 struct Span {
     const void *p;
     int64_t     bytes;
+    int64_t     row = 0, pitch = 0;  // bytes of a row, and from one to the next (0: all one)
 };
 static bool meet(const Span &a, const Span &b) {
     const uintptr_t x = (uintptr_t)a.p, z = (uintptr_t)b.p;
-    return a.p && b.p && a.bytes && b.bytes && x < z + (uintptr_t)b.bytes && z < x + (uintptr_t)a.bytes;
+    if (!a.p || !b.p || !a.bytes || !b.bytes || x >= z + (uintptr_t)b.bytes || z >= x + (uintptr_t)a.bytes) return false;
+    if (a.pitch && a.pitch == b.pitch) {  // rows of one buffer: b's between a's
+        const int64_t d = ((int64_t)(z - x) % a.pitch + a.pitch) % a.pitch;
+        if (d >= a.row && d + b.row <= a.pitch) return false;
+    }
+    return true;
 }
 // rows `ld` apart of which `n` elements of `size` bytes count
 static Span rows_of(const void *p, int64_t rows, int64_t ld, int64_t n, int64_t size) {
-    return Span{p, rows > 0 ? ((rows - 1) * ld + n) * size : 0};
+    return Span{p, rows > 0 ? ((rows - 1) * ld + n) * size : 0, n * size, rows > 1 ? ld * size : 0};
 }
 template <int NI, int NO>
 static const char *overlap(const Span (&in)[NI], const Span (&out)[NO]) {

@@ -536,8 +536,9 @@ int s2x_attn_paged_rows(const void *q, int64_t ld_q, int64_t n_row, const int32_
  * Q8_1 of y as s2x_quantize_q8_1(y, K = H) writes it, bit for bit (qs: M rows of
  * K_pad int8, 16-byte aligned; ds: M rows of K_pad/32 words; H <= K_pad < H + 32,
  * columns past H zero), and y itself in y_type.  h_out may be resid or x (same
- * type and stride); nothing else may overlap.  Rows need only their elements'
- * alignment (16 bytes are faster).  H <= 32,768, M <= 2^30. */
+ * type and stride); nothing else may overlap (columns of one buffer, its stride in
+ * all of them, do not).  Rows need only their elements' alignment (16 bytes are
+ * faster).  H <= 32,768, M <= 2^30. */
 int s2x_add_rmsnorm_quantize_q8_1(const void *x, int32_t x_type, int64_t ld_x, const void *resid,
                                   int32_t resid_type, int64_t ld_resid, int64_t H, int64_t M,
                                   const float *w, float eps, void *h_out, int64_t ld_h, int64_t K_pad,

@@ -15,7 +15,7 @@ from gpu_util import assert_same, dev, host, ptr, say, stream
 from search_util import beam_scores, compact_ref, fork_ref
 from test_gpu_decode import NAN, U
 from test_gpu_search import (INF, beam_case, beams_case, check_compact, compare, ints, nans, prefix_inputs, rms_case, run_beam,
-                             run_fork, run_prefix)
+                             run_fork, run_prefix, run_rms)
 
 pytestmark = pytest.mark.gpu
 
@@ -423,3 +423,22 @@ def test_page_calls_over_one_workspace():
             torch.cuda.synchronize()
             jobs[i].check(want[i], f"round {r}")
             torch.randn(300, 300, device="cuda:0").sum()
+
+
+@pytest.mark.parametrize("m,h", [(1, 64), (2, 33), (37, 1157), (200, 4096)])
+@pytest.mark.parametrize("order", [(0, 1, 2, 3), (3, 2, 1, 0), (2, 0, 3, 1)])
+def test_rms_columns_of_one_buffer(m, h, order):
+    """x, the residual, h and y as columns of one buffer, with columns of none between."""
+    x, r, w = rms_case(h, m, h, "f32", "f32")
+    wd, gap = dev(w), 5
+    mem = nans(m, 4 * h + gap)
+    at = [i * h + (gap if i > 1 else 0) for i in order]
+    xs, rs, hs, ys = (mem[:, a:a + h] for a in at)
+    xs.copy_(x)
+    rs.copy_(r)
+    s2x.call("s2x_add_rmsnorm_quantize_q8_1", ptr(xs), 0, mem.shape[1], ptr(rs), 0, mem.shape[1], h, m, ptr(wd), 1e-6, ptr(hs), mem.shape[1],
+             0, None, None, ptr(ys), 0, mem.shape[1], stream())
+    ho, y, _, _ = run_rms(x, r, w, out="y")
+    torch.cuda.synchronize()
+    assert torch.equal(hs, ho) and torch.equal(ys, y)
+    assert torch.equal(xs.cpu(), x) and torch.equal(rs.cpu(), r) and torch.isnan(mem[:, 2 * h:2 * h + gap]).all()

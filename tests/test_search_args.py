@@ -191,3 +191,16 @@ def test_prefix_sizes():
     assert size(1, 32768, 100, 50, 64, 64, 64) > 0 and size(1, 32769, 100, 50, 64, 64, 64) == 0
     assert size(1, 16384, 100, 50, 1024, 64, 64) > 0 and size(1, 18724, 100, 50, 1008, 56, 64) > 0
     assert size(1, 18725, 100, 50, 1008, 56, 64) == 0
+
+
+def test_rms_columns_of_one_buffer():
+    """Rows between one another's: one element too near is an overlap (that none is
+    shows where there is a GPU)."""
+    one = dict(x_type=F32, ld_x=400, ld_resid=400, ld_h=400, ld_y=400, qs=None, ds=None, x=A[0], resid=A[0] + 400,
+               h_out=A[0] + 800, y=A[0] + 1200)
+    for name, offset in (("resid", 404), ("h_out", 796), ("y", 1196), ("y", 1204), ("h_out", 1600 - 4), ("y", 2 * 1600 + 4)):
+        bad = {**one, name: A[0] + offset}
+        if name == "resid":
+            bad["h_out"] = A[0] + 800
+        assert rms(**bad) == INVALID, (name, offset)
+    assert rms(**{**one, "ld_y": 404}) == INVALID
