@@ -16,7 +16,7 @@
 // in the order of tokens, are enough.  The list's members count the larger ones
 // among them, which is their rank.
 // Bound by the issue of instructions more than by the bytes (an fma, an exponential and
-// an addition a logit): 434 live rows of 256,000 bf16 54.9 us = 4.0 TB/s; 4 rows of
+// an addition a logit): 434 live rows of 256,000 bf16 55.5 us = 4.0 TB/s; 4 rows of
 // 32,000 f32 6.0 us, of which a launch is 2 to 3.
 // k_beam_join: per request, the parts' sums, and the same over their candidates
 // with S in f64: the order of two beams' candidates hangs on two sums of many
@@ -162,11 +162,11 @@ struct BmPlan {
 };
 // Parts of a row: up to 16 loads a lane, fewer where rows are few, as long as that
 // takes no more than 512 workgroups and the join has a request's candidates in one
-// round.  2, 4, 8, 16 loads, both launches: 1 request of 4 beams of 32,000 f32 12.6, 13.2,
-// 14.0, 14.7 us; 14 of 5 of 56,284 20.9, 18.8, 17.9, 19.0; 60 of 2 of 30,000 18.1, 15.8,
-// 15.0, 15.3; 1 of 8 of 100,000 (8 out) 22.2, 16.5, 16.9, 17.8; 13 of 12 of 50,000 (24 out)
-// 54.7, 36.0, 28.6, 29.1; 1 of 32 of 32,000 (64 out) 86, 51, 35, 38; 64 of 8 of 256,000
-// bf16 (16 out) 137, 91, 70, 64.
+// round.  2, 4, 8, 16 loads, both launches, f32: 1 request of 4 beams of 32,000 12.5, 13.0,
+// 13.8, 14.5 us; 14 of 5 of 56,284 20.6, 18.4, 17.7, 18.7; 60 of 2 of 30,000 17.8, 15.6,
+// 14.9, 14.9; 1 of 8 of 100,000 (8 out) 24.9, 16.5, 16.9, 17.6; 13 of 12 of 50,000 (24 out)
+// 42.2, 35.7, 28.6, 29.1; 1 of 32 of 32,000 (64 out) 86, 52, 36, 39; 64 of 8 of 256,000
+// bf16 (16 out) 123, 94, 67, 64.
 constexpr int BJ_PER = 8, BJ_TILE = BM_NT * BJ_PER;  // candidates of a round of 256 threads
 static BmPlan bm_plan(int64_t n_req, int64_t n_beam, int64_t n_vocab, int64_t n_out, int per) {
     auto parts = [&](int loads) { return (n_vocab + loads * BM_NT * per - 1) / (loads * BM_NT * per); };
@@ -529,7 +529,7 @@ static hipError_t run_beam(const BeamSelect &p, hipStream_t stream) {
                                                                                                      : k_beam_rows<T, 2>;
     hipLaunchKernelGGL(kern, dim3(P.n_split, rows), dim3(BM_NT), (size_t)cap * 8, stream, p, P.span, P.n_split, cap);
     // (1,024 threads where 256 need more than a round: 7 requests of 32 beams of 4 parts of
-    // 64 candidates 48.6 us, both launches, 75.5 with 256; 64 of 8 of 8 of 16 71.8 and 63.8)
+    // 64 candidates 50.5 us, both launches, 74.9 with 256; 64 of 8 of 8 of 16 73.9 and 65.2)
     const bool wide = (int64_t)p.n_beam * P.n_split * p.n_out > BJ_TILE;
     hipLaunchKernelGGL(wide ? k_beam_join<1024> : k_beam_join<256>, dim3(p.n_req), dim3(wide ? 1024 : 256), 0, stream, p, P.n_split);
     return hipGetLastError();
